@@ -56,6 +56,15 @@ SIGNATURES = {
     "apa_adamw_cast": [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _F, _F, _F, _F, _F, _I64, _VP, _I, _I64, _VP, _I64,
                        _VP, _VP],
     "apa_bias_grad_noalloc": [_VP, _I, _I64, _I64, _I64, _I, _VP, _I, _VP],
+    "apa_block_cast": [_VP, _I, _I64, _I64, _I64, _VP, _VP, _I, _I, _VP, _I64, _VP, _VP, _I64, _VP, _VP, _VP],
+    "apa_block_dequant": [_VP, _I64, _VP, _I64, _I64, _VP, _I, _I64, _VP],
+    "apa_block_colsum": [_VP, _I64, _I64, _VP, _I, _VP],
+    "apa_block_gemm": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _I, _VP],
+    "apa_rmsnorm_fwd": [_VP, _I64, _VP, _I64, _VP, _I, _I, _I64, _I64, _F, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP,
+                        _VP],
+    "apa_rmsnorm_bwd_workspace": [_I64, _I64, _VP],
+    "apa_rmsnorm_bwd": [_VP, _I64, _VP, _I64, _VP, _VP, _I, _VP, _I64, _VP, _I64, _I, _I64, _I64, _VP, _VP, _I64,
+                        _VP],
     "apa_ladder_pack": [_I, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP],
     "apa_ladder_eval": [_I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _I64, _I64,
                         ctypes.c_double, ctypes.c_double, _VP, _VP, _VP],

@@ -1,0 +1,612 @@
+"""Block-scaled FP8: E4M3 tensors with one power-of-two scale per 128 elements,
+their products, and the root-mean-square norm that feeds them.
+
+``APALinear`` keeps the reference's arithmetic, which casts to E4M3 without a
+scale and climbs to wider types when that loses too much. The operators here
+scale every block of 128 elements into E4M3's range instead, so a layer stays
+in FP8 whatever the size of its activations, weights and gradients:
+
+    x   activations   one scale per token and 128 features
+    W   weights       one scale per 128 x 128
+    dy  gradients     one scale per token and 128 features; for the weight
+                      gradient one per feature and 128 tokens
+
+Serving:
+
+    wq = block_cast(weight, square=True)            # once
+    y = block_linear(x, wq, bias)                   # every call
+    q, r = rms_norm(x, gamma, residual=r, quantize=True)
+    y = block_linear(q, wq)                         # the norm's E4M3 output as it is
+
+Training (any optimizer; beside ``APALinear`` under one ``APAManager``, whose
+overflow checks see these layers' output gradients through its leaf hooks):
+
+    norm = APARMSNorm(d)
+    lin = APABlockLinear(d, 4 * d)
+    y = lin(x)                                      # or
+    y, r = lin(x, norm=norm, residual=r)            # r = x + r; y = lin(norm(r))
+
+All functions run on the current stream of their tensors' device, allocate
+with torch's caching allocator, and can be captured in a CUDA graph. Scales
+and codes are those of the definition, bit for bit: the smallest power of two
+that brings a block's largest finite magnitude to 448 or below (not below
+2^-126), and round to nearest even. NaN and infinities become NaN codes and do
+not affect the scale.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .config import APAConfig
+
+BLOCK = 128
+MAX_NORM_FEATURES = 32768
+
+_E4M3 = torch.float8_e4m3fn
+_REAL = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """One library call on the tensors' device, whichever is current."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args), name)
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args), name)
+
+
+def _real(dtype: torch.dtype, what: str) -> int:
+    code = _REAL.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: expected float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x as a 2-D matrix with unit column stride, rows a positive distance apart."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(x).__name__}")
+    if x.dim() < 1:
+        raise ValueError(f"{what}: expected at least one dimension")
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    n = m.shape[1]
+    if n == 0:
+        raise ValueError(f"{what}: has no columns")
+    if m.stride(1) != 1 and n > 1 or (m.shape[0] > 1 and m.stride(0) < n):
+        m = m.contiguous()
+    return m
+
+
+def _ld(m: torch.Tensor) -> int:
+    """Row pitch of a matrix from _matrix (a single row's stride may be anything)."""
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+
+
+def _same_device(what: str, device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _vector(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what}: expected shape [{n}], got {list(t.shape)}")
+    _real(t.dtype, what)
+    _same_device(what, device, t)
+    return t if t.stride(0) == 1 else t.contiguous()
+
+
+def _codes(rows: int, cols: int, device) -> torch.Tensor:
+    """[rows, cols] E4M3 view whose row pitch is a multiple of 16 bytes."""
+    pitch = (cols + 15) & ~15
+    t = torch.empty(rows, pitch, dtype=_E4M3, device=device)
+    return t if pitch == cols else t[:, :cols]
+
+
+def _scale_bytes(rows: int, cols: int) -> int:
+    return ((cols + 511) >> 9) * ((rows + 127) & ~127) * 4
+
+
+class APABlockTensor:
+    """A [rows, cols] matrix held as E4M3 codes with one scale per row and 128
+    columns. ``data`` holds the codes; ``scales`` one byte per block (2^(b-127))
+    in the order the tensor cores take, see ``exponents()`` for the plain one.
+    """
+
+    __slots__ = ("data", "scales")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        self.data = data
+        self.scales = scales
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.data.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    def __repr__(self) -> str:
+        return f"APABlockTensor({list(self.shape)}, device={self.device})"
+
+    @classmethod
+    def from_parts(cls, data: torch.Tensor, exponents: torch.Tensor) -> "APABlockTensor":
+        """From E4M3 codes [rows, cols] and integer exponents p (scale 2^p,
+        -127 <= p <= 127) of shape [rows, ceil(cols / 128)], or
+        [ceil(rows / 128), ceil(cols / 128)] for 128 x 128 blocks."""
+        if data.dim() != 2 or data.dtype != _E4M3:
+            raise ValueError("APABlockTensor.from_parts: data must be a 2-D float8_e4m3fn tensor")
+        rows, cols = data.shape
+        if rows == 0 or cols == 0:
+            raise ValueError("APABlockTensor.from_parts: data is empty")
+        kb = (cols + 127) // 128
+        e = exponents
+        if e.is_floating_point() or e.is_complex() or e.dtype == torch.bool:
+            raise TypeError("APABlockTensor.from_parts: exponents must be integers")
+        _same_device("APABlockTensor.from_parts", data.device, e)
+        if tuple(e.shape) == (rows, kb):
+            pass
+        elif tuple(e.shape) == ((rows + 127) // 128, kb):
+            e = e.repeat_interleave(128, dim=0)[:rows]
+        else:
+            raise ValueError(f"APABlockTensor.from_parts: exponents of shape {list(exponents.shape)} for codes "
+                             f"{list(data.shape)}")
+        e = e.to(torch.int32)
+        if int(e.min()) < -127 or int(e.max()) > 127:
+            raise ValueError("APABlockTensor.from_parts: exponents must lie in -127 .. 127")
+        rp, kp = (rows + 127) & ~127, (kb + 3) & ~3
+        full = torch.full((rp, kp), 127, dtype=torch.uint8, device=data.device)
+        full[:rows, :kb] = (e + 127).to(torch.uint8)
+        # [row group, quarter, lane, word, byte] -> [word, row group, lane, quarter, byte]
+        scales = full.view(rp // 128, 4, 32, kp // 4, 4).permute(3, 0, 2, 1, 4).contiguous().view(-1)
+        q = _codes(rows, cols, data.device)
+        q.view(torch.uint8).copy_(data.view(torch.uint8))
+        return cls(q, scales)
+
+    def exponents(self) -> torch.Tensor:
+        """int32 [rows, ceil(cols / 128)]: block b of row r has the scale 2^exponents[r, b]."""
+        rows, cols = self.shape
+        rp, kb = (rows + 127) & ~127, (cols + 127) // 128
+        kg = (kb + 3) // 4
+        full = self.scales.view(kg, rp // 128, 32, 4, 4).permute(1, 3, 2, 0, 4).reshape(rp, kg * 4)
+        return full[:rows, :kb].to(torch.int32) - 127
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values code * scale, in ``dtype`` (exact in float32 and, within
+        its range, bfloat16)."""
+        code = _real(dtype, "APABlockTensor.dequantize")
+        _lib.require_cuda(self.data, "APABlockTensor.dequantize")
+        rows, cols = self.shape
+        out = torch.empty(rows, cols, dtype=dtype, device=self.device)
+        if rows:
+            _call(self.device, "apa_block_dequant", self.data.data_ptr(), _ld(self.data) if rows > 1 else
+                  (cols + 15) & ~15, self.scales.data_ptr(), rows, cols, out.data_ptr(), code, cols,
+                  _lib.stream_handle(self.device))
+        return out
+
+
+def _new_block(rows: int, cols: int, device) -> APABlockTensor:
+    return APABlockTensor(_codes(rows, cols, device),
+                          torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))
+
+
+def _pitch(t: APABlockTensor) -> int:
+    return t.data.stride(0) if t.data.shape[0] > 1 else (t.data.shape[1] + 15) & ~15
+
+
+def _cast(x2: torch.Tensor, rows_form: bool, cols_form: bool, square: bool = False, colsum=None, row_mul=None,
+          col_mul=None):
+    rows, cols = x2.shape
+    dev = x2.device
+    q = _new_block(rows, cols, dev) if rows_form else None
+    qt = _new_block(cols, rows, dev) if cols_form else None
+    if rows == 0:
+        return q, qt
+    _call(dev, "apa_block_cast", x2.data_ptr(), _REAL[x2.dtype], rows, cols, _ld(x2), _lib.ptr(row_mul),
+          _lib.ptr(col_mul), _REAL[col_mul.dtype] if col_mul is not None else 0, int(square),
+          q.data.data_ptr() if q else None, _pitch(q) if q else 0, q.scales.data_ptr() if q else None,
+          qt.data.data_ptr() if qt else None, _pitch(qt) if qt else 0, qt.scales.data_ptr() if qt else None,
+          _lib.ptr(colsum), _lib.stream_handle(dev))
+    return q, qt
+
+
+def block_cast(x: torch.Tensor, form: str = "rows", square: bool = False):
+    """Cast a matrix (leading dimensions are flattened) to an APABlockTensor.
+
+    ``form`` "rows": x itself, scales per row and 128 columns; "cols": its
+    transpose [cols, rows], scales per column of x and 128 rows (the operand
+    of a product that reduces over x's rows); "both": the pair. ``square``:
+    one scale per 128 x 128 block (weights), so both forms hold the same
+    values. Not differentiable; ``APABlockLinear`` is.
+    """
+    if form not in ("rows", "cols", "both"):
+        raise ValueError(f"block_cast: form must be 'rows', 'cols' or 'both', got {form!r}")
+    x2 = _matrix(x, "block_cast")
+    _real(x2.dtype, "block_cast")
+    _lib.require_cuda(x2, "block_cast")
+    if x2.shape[0] == 0 and form != "rows":
+        raise ValueError("block_cast: the transpose of a matrix without rows has no columns")
+    q, qt = _cast(x2, form != "cols", form != "rows", square)
+    return (q, qt) if form == "both" else q if form == "rows" else qt
+
+
+def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool) -> None:
+    M, K = a.shape
+    _call(a.device, "apa_block_gemm", a.data.data_ptr(), _pitch(a), a.scales.data_ptr(), b.data.data_ptr(), _pitch(b),
+          b.scales.data_ptr(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, out.data_ptr(),
+          _REAL[out.dtype], _ld(out), M, b.shape[0], K, int(accumulate), _lib.stream_handle(a.device))
+
+
+def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,
+                 out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
+                 accumulate: bool = False) -> torch.Tensor:
+    """a [M, K] times the transpose of b [N, K], plus bias [N]: [M, N].
+
+    Accumulated in fp32 and rounded once to ``out_dtype`` (float32, float16
+    or bfloat16). ``out``: written in place (unit column stride); with
+    ``accumulate`` the product is added to a float32 ``out``."""
+    if not isinstance(a, APABlockTensor) or not isinstance(b, APABlockTensor):
+        raise TypeError("block_matmul: both operands must be APABlockTensors")
+    _lib.require_cuda(a.data, "block_matmul")
+    _same_device("block_matmul", a.device, b.data)
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K:
+        raise ValueError(f"block_matmul: operands reduce over {K} and {b.shape[1]} columns")
+    if N == 0:
+        raise ValueError("block_matmul: the second operand has no rows")
+    if bias is not None:
+        bias = _vector(bias, N, a.device, "block_matmul: bias")
+    if accumulate and out is None:
+        raise ValueError("block_matmul: accumulate needs out")
+    if out is None:
+        _real(out_dtype, "block_matmul: out_dtype")
+        out = torch.empty(M, N, dtype=out_dtype, device=a.device)
+    else:
+        _real(out.dtype, "block_matmul: out")
+        _same_device("block_matmul: out", a.device, out)
+        if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError(f"block_matmul: out must be a row-major [{M}, {N}] tensor")
+        if accumulate and out.dtype != torch.float32:
+            raise ValueError("block_matmul: accumulate needs a float32 out")
+    if M:
+        _matmul(a, b, bias, out, accumulate)
+    return out
+
+
+def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor, bias: Optional[torch.Tensor] = None,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x W^T + bias for serving. x [..., K] is cast to E4M3 here, or comes as an
+    APABlockTensor (from ``rms_norm(..., quantize=True)``); ``weight`` [N, K] is
+    ``block_cast(w, square=True)``. ``out_dtype`` defaults to x's type
+    (bfloat16 for an APABlockTensor). Not differentiable."""
+    if isinstance(x, APABlockTensor):
+        return block_matmul(x, weight, bias, out_dtype or torch.bfloat16)
+    if not isinstance(weight, APABlockTensor):
+        raise TypeError("block_linear: the weight must be an APABlockTensor (block_cast(w, square=True))")
+    x2 = _matrix(x, "block_linear")
+    _real(x2.dtype, "block_linear")
+    _lib.require_cuda(x2, "block_linear")
+    if x2.shape[1] != weight.shape[1]:
+        raise ValueError(f"block_linear: x has {x2.shape[1]} features, the weight {weight.shape[1]}")
+    q, _ = _cast(x2, True, False)
+    y = block_matmul(q, weight, bias, out_dtype or x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+
+
+# ---------------------------------------------------------------------------
+# root-mean-square norm
+# ---------------------------------------------------------------------------
+def _norm_args(x, weight, residual, what: str):
+    x2 = _matrix(x, what)
+    _real(x2.dtype, what)
+    _lib.require_cuda(x2, what)
+    K = x2.shape[1]
+    if K > MAX_NORM_FEATURES:
+        raise ValueError(f"{what}: at most {MAX_NORM_FEATURES} features, got {K}")
+    g = _vector(weight, K, x2.device, f"{what}: weight")
+    r2 = None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"{what}: residual {residual.dtype} {list(residual.shape)} does not match x {x.dtype} "
+                             f"{list(x.shape)}")
+        _same_device(what, x2.device, residual)
+        r2 = _matrix(residual, what)
+    return x2, g, r2
+
+
+def _check_eps(eps: float, what: str) -> float:
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"{what}: eps must be finite and not negative")
+    return eps
+
+
+def _norm_forward(x2, g, res2, eps: float, quantize: bool, want_rstd: bool):
+    """(output, stream, rstd): output an APABlockTensor or a matrix of x's type."""
+    M, K = x2.shape
+    dev = x2.device
+    stream = torch.empty(M, K, dtype=x2.dtype, device=dev) if res2 is not None else None
+    q = _new_block(M, K, dev) if quantize else None
+    y = None if quantize else torch.empty(M, K, dtype=x2.dtype, device=dev)
+    rstd = torch.empty(M, dtype=torch.float32, device=dev) if want_rstd else None
+    if M:
+        _call(dev, "apa_rmsnorm_fwd", x2.data_ptr(), _ld(x2), _lib.ptr(res2), _ld(res2) if res2 is not None else 0,
+              g.data_ptr(), _REAL[g.dtype], _REAL[x2.dtype], M, K, eps, _lib.ptr(stream), K, _lib.ptr(y), K,
+              q.data.data_ptr() if q else None, _pitch(q) if q else 0, q.scales.data_ptr() if q else None,
+              _lib.ptr(rstd), _lib.stream_handle(dev))
+    return (q if quantize else y), stream, rstd
+
+
+def _norm_backward(dh2, r2, rstd, g, dr2):
+    """(dx, dgamma)."""
+    M, K = r2.shape
+    dev = r2.device
+    dx = torch.empty(M, K, dtype=r2.dtype, device=dev)
+    dg = torch.empty(K, dtype=g.dtype, device=dev)
+    if M == 0:
+        return dx, dg.zero_()
+    n = ctypes.c_int64(0)
+    _call(dev, "apa_rmsnorm_bwd_workspace", M, K, ctypes.addressof(n))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
+          _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K, _REAL[r2.dtype], M, K,
+          dg.data_ptr(), ws.data_ptr(), n.value, _lib.stream_handle(dev))
+    return dx, dg
+
+
+def _grad_matrix(g, dtype, K: int):
+    """A gradient from autograd as a matrix of the operator's type (None stays None)."""
+    if g is None:
+        return None
+    g2 = g.reshape(-1, K)
+    if g2.dtype != dtype:
+        g2 = g2.to(dtype)
+    return _matrix(g2, "gradient")
+
+
+class _RMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        x2, g, res2 = _norm_args(x, weight, residual, "rms_norm")
+        y, stream, rstd = _norm_forward(x2, g, res2, eps, False, True)
+        ctx.set_materialize_grads(False)
+        ctx.has_res = residual is not None
+        ctx.shape = x.shape
+        y = y.view(x.shape)
+        if residual is None:
+            ctx.save_for_backward(x, weight)
+            ctx.rstd = rstd
+            return y
+        stream = stream.view(x.shape)
+        ctx.save_for_backward(stream, weight)
+        ctx.rstd = rstd
+        return y, stream
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dr=None):
+        r, weight = ctx.saved_tensors
+        K = weight.shape[0]
+        if dy is None:
+            return dr, None, dr if ctx.has_res else None, None
+        dx, dg = _norm_backward(_grad_matrix(dy, r.dtype, K), _matrix(r, "rms_norm"), ctx.rstd, weight.contiguous(),
+                                _grad_matrix(dr, r.dtype, K))
+        dx = dx.view(ctx.shape)
+        return dx, dg, dx if ctx.has_res else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             quantize: bool = False):
+    """Root-mean-square norm over the last dimension, with the residual's
+    addition: r = x + residual (rounded to x's type), y = r / sqrt(mean(r^2) +
+    eps) * weight. Returns y, or (y, r) when a residual is given.
+
+    ``quantize``: y as an APABlockTensor [rows, K], rounded once from fp32 to
+    E4M3 under its blocks' scales (not differentiable; use ``APABlockLinear``
+    with ``norm=`` for training). Otherwise y has x's type and gradients flow
+    to x, residual and weight."""
+    eps = _check_eps(eps, "rms_norm")
+    if not quantize:
+        return _RMSNormFn.apply(x, weight, residual, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
+        raise RuntimeError("rms_norm: the E4M3 output has no gradient; call it under torch.no_grad(), or train through "
+                           "APABlockLinear(...)(x, norm=norm, residual=residual)")
+    x2, g, res2 = _norm_args(x, weight, residual, "rms_norm")
+    q, stream, _ = _norm_forward(x2, g, res2, eps, True, False)
+    return q if residual is None else (q, stream.view(x.shape))
+
+
+class APARMSNorm(nn.Module):
+    """``rms_norm`` with its weight: ``norm(x)`` or ``y, r = norm(x, residual)``."""
+
+    def __init__(self, features: int, eps: float = 1e-6, dtype: torch.dtype = torch.float32,
+                 config: APAConfig = APAConfig()):
+        super().__init__()
+        if not 0 < features <= MAX_NORM_FEATURES:
+            raise ValueError(f"APARMSNorm: features must lie in 1 .. {MAX_NORM_FEATURES}, got {features}")
+        _real(dtype, "APARMSNorm")
+        self.features = features
+        self.eps = _check_eps(eps, "APARMSNorm")
+        self.weight = nn.Parameter(torch.ones(features, dtype=dtype, device=torch.device(config.device)))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, quantize: bool = False):
+        return rms_norm(x, self.weight, residual, self.eps, quantize)
+
+    def extra_repr(self) -> str:
+        return f"{self.features}, eps={self.eps}"
+
+
+# ---------------------------------------------------------------------------
+# linear layer
+# ---------------------------------------------------------------------------
+class _BlockLinearFn(torch.autograd.Function):
+    """y = (norm of x + residual, or x) W^T + b with E4M3 operands; the casts
+    pass gradients straight through."""
+
+    @staticmethod
+    def forward(ctx, x, residual, gamma, weight, bias, eps):
+        ctx.set_materialize_grads(False)
+        need_in = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        need_dw = ctx.needs_input_grad[3]
+        N, K = weight.shape
+        ctx.shape, ctx.has_res, ctx.has_norm = x.shape, residual is not None, gamma is not None
+        ctx.bias_dtype = bias.dtype if bias is not None else None
+        ctx.weight_dtype = weight.dtype
+        stream = rstd = xt = None
+        if gamma is None:
+            x2 = _matrix(x, "APABlockLinear")
+            xq, xt = _cast(x2, True, need_dw and x2.shape[0] > 0)
+        else:
+            x2, g, res2 = _norm_args(x, gamma, residual, "APABlockLinear")
+            xq, stream, rstd = _norm_forward(x2, g, res2, eps, True, True)
+        w2 = _matrix(weight, "APABlockLinear: weight")
+        wq, wt = _cast(w2, True, need_in, square=True)
+        M = x2.shape[0]
+        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        if M:
+            _matmul(xq, wq, bias, y, False)
+        ctx.xt, ctx.wt, ctx.rstd = xt, wt, rstd
+        ctx.M, ctx.N, ctx.K, ctx.dtype = M, N, K, x.dtype
+        y = y.view(*x.shape[:-1], N)
+        if gamma is None:
+            return y
+        stream = x if stream is None else stream.view(x.shape)
+        ctx.save_for_backward(stream, gamma)
+        return (y, stream) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dr=None):
+        need = ctx.needs_input_grad
+        need_in = need[0] or need[1] or need[2]
+        M, N, K = ctx.M, ctx.N, ctx.K
+        if dy is None:
+            return (dr if need[0] else None, dr if ctx.has_res and need[1] else None, None, None, None, None)
+        dev = dy.device
+        dx = dg = dw = db = None
+        if M == 0:
+            dx = torch.zeros(ctx.shape, dtype=ctx.dtype, device=dev) if need[0] or need[1] else None
+            dg = torch.zeros(K, dtype=ctx.saved_tensors[1].dtype, device=dev) if need[2] else None
+            dw = torch.zeros(N, K, dtype=ctx.weight_dtype, device=dev) if need[3] else None
+            db = torch.zeros(N, dtype=ctx.bias_dtype, device=dev) if need[4] else None
+            return dx, dx if ctx.has_res else None, dg, dw, db, None
+        dy2 = _grad_matrix(dy, ctx.dtype, N)
+        parts = (M + 127) // 128
+        sums = torch.empty(parts, N, dtype=torch.float32, device=dev) if need[4] else None
+        dyq, dyt = _cast(dy2, need_in or not need[3], need[3], colsum=sums)
+        if need[4]:
+            db = torch.empty(N, dtype=ctx.bias_dtype, device=dev)
+            _call(dev, "apa_block_colsum", sums.data_ptr(), parts, N, db.data_ptr(), _REAL[ctx.bias_dtype],
+                  _lib.stream_handle(dev))
+        if ctx.has_norm:
+            stream, gamma = ctx.saved_tensors
+            r2, g = _matrix(stream, "APABlockLinear"), gamma.contiguous()
+        if need[3]:
+            xt = ctx.xt
+            if ctx.has_norm:
+                # the norm's output again, from the stream, with scales along the tokens
+                _, xt = _cast(r2, False, True, row_mul=ctx.rstd, col_mul=g)
+            dw = torch.empty(N, K, dtype=ctx.weight_dtype, device=dev)
+            _matmul(dyt, xt, None, dw, False)
+        if need_in:
+            dh = torch.empty(M, K, dtype=ctx.dtype, device=dev)
+            _matmul(dyq, ctx.wt, None, dh, False)
+            if ctx.has_norm:
+                dx, dg = _norm_backward(dh, r2, ctx.rstd, g, _grad_matrix(dr, ctx.dtype, K))
+            else:
+                dx = dh
+            dx = dx.view(ctx.shape)
+        return (dx if need[0] else None, dx if ctx.has_res and need[1] else None, dg if need[2] else None, dw, db,
+                None)
+
+
+class APABlockLinear(nn.Module):
+    """A linear layer whose three products run on block-scaled E4M3 operands.
+
+    ``weight_master`` [out, in] and ``bias_master`` [out] are ordinary
+    parameters in ``dtype`` (float32 masters, or bfloat16); their gradients come
+    in the same type. Output and input gradient have x's type. In training
+    every forward casts the weight anew; without gradients the layer keeps its
+    cast weight and renews it when the parameter changed (in place through
+    autograd's version counter; call ``refresh_working_copy()`` after changes
+    made behind it, through ``.data``).
+
+    ``forward(x, norm=None, residual=None)``: with ``norm`` (an ``APARMSNorm``)
+    the layer is applied to ``norm(x)``, or to the normalised sum x + residual;
+    the norm writes the E4M3 operand itself. With a residual the result is
+    (y, x + residual)."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float32,
+                 config: APAConfig = APAConfig()):
+        super().__init__()
+        if in_features <= 0 or out_features <= 0:
+            raise ValueError("APABlockLinear: in_features and out_features must be positive")
+        _real(dtype, "APABlockLinear")
+        self.in_features = in_features
+        self.out_features = out_features
+        dev = torch.device(config.device)
+        # initialised on the CPU generator and then moved, as APALinear does,
+        # so that a seed gives the same weights on every device
+        w = torch.empty(out_features, in_features)
+        nn.init.kaiming_uniform_(w, a=math.sqrt(5))
+        self.weight_master = nn.Parameter(w.to(device=dev, dtype=dtype))
+        if bias:
+            b = torch.empty(out_features).uniform_(-1 / math.sqrt(in_features), 1 / math.sqrt(in_features))
+            self.bias_master = nn.Parameter(b.to(device=dev, dtype=dtype))
+        else:
+            self.register_parameter("bias_master", None)
+        self._wq: Optional[APABlockTensor] = None
+        self._wq_key: Optional[Tuple] = None
+
+    def refresh_working_copy(self) -> None:
+        """Cast the weight for calls without gradients (buffers are kept, so a
+        captured graph of such a call sees the new values)."""
+        W = self.weight_master
+        _lib.require_cuda(W, "APABlockLinear.refresh_working_copy")
+        with torch.no_grad():
+            q, _ = _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True)
+            if self._wq is not None and self._wq.device == q.device:
+                self._wq.data.view(torch.uint8).copy_(q.data.view(torch.uint8))
+                self._wq.scales.copy_(q.scales)
+            else:
+                self._wq = q
+        self._wq_key = (W._version, W.device, W.dtype)
+
+    def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
+        W, b = self.weight_master, self.bias_master
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"APABlockLinear: expected a tensor, got {type(x).__name__}")
+        if residual is not None and norm is None:
+            raise ValueError("APABlockLinear: residual needs norm")
+        if x.dim() < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"APABlockLinear: input of shape {list(x.shape)}, expected {self.in_features} features")
+        if norm is not None and norm.features != self.in_features:
+            raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
+        _real(x.dtype, "APABlockLinear")
+        _lib.require_cuda(x, "APABlockLinear")
+        _same_device("APABlockLinear", x.device, W, residual)
+        gamma = norm.weight if norm is not None else None
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gamma, W, b)):
+            return _BlockLinearFn.apply(x, residual, gamma, W, b, norm.eps if norm is not None else 0.0)
+        if self._wq is None or self._wq_key != (W._version, W.device, W.dtype):
+            self.refresh_working_copy()
+        if norm is None:
+            return block_linear(x, self._wq, b)
+        out = rms_norm(x.detach(), gamma.detach(), residual.detach() if residual is not None else None, norm.eps, True)
+        q = out if residual is None else out[0]
+        y = block_linear(q, self._wq, b, x.dtype).view(*x.shape[:-1], self.out_features)
+        return y if residual is None else (y, out[1])
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias_master is not None}"

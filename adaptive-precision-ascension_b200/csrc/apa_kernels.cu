@@ -9,3 +9,6 @@
 #include "forensic.cu"
 #include "adamw.cu"
 #include "dp_nvls.cu"
+#include "block_cast.cu"
+#include "rmsnorm.cu"
+#include "block_gemm.cu"

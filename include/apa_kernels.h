@@ -370,6 +370,81 @@ int apa_linear_wgrad_dp(int rung, const void* dyqt, int64_t lddyt, const void* x
                         const unsigned int* epoch_local, unsigned int* deferred_local, int world, int rank,
                         void* stream);
 
+/*
+ * Block-scaled FP8 and the norm that feeds it. No counterpart in the
+ * reference (it casts to E4M3 without a scale); they stand beside apa_cast and
+ * apa_linear_*.
+ *
+ * A block tensor [rows, K] is E4M3 codes (row pitch a multiple of 16 bytes,
+ * 16-byte aligned) and one byte b per row and 128 columns, standing for
+ * 2^(b-127): value = code * 2^(b-127). Scale bytes: ceil(K/512) *
+ * ceil(rows/128)*128 words of 32 bits; the byte of (row r, 128-column block
+ * kb) lies at 4 * ((kb/4) * ceil(rows/128)*128 + r/128*128 + r%32*4 +
+ * r%128/32) + kb%4. 16-byte aligned. Bytes of rows past the end or of blocks
+ * past K may hold anything.
+ */
+
+/*
+ * Cast src [rows, cols] (F32, F16, BF16; row pitch ld_src) to block tensors:
+ * dst [rows, cols] with a scale per row and 128 columns, and/or dst_t
+ * [cols, rows], the transpose, with a scale per column of src and 128 of its
+ * rows. square != 0: one scale per 128 x 128 block in both. A scale is the
+ * smallest power of two (at least 2^-126) that brings the block's largest
+ * finite magnitude to 448 or below; an empty block has 1. NaN and infinities
+ * become NaN codes. row_mul (fp32 [rows]) and col_mul ([cols]), both or
+ * neither: the source is src[r, c] * row_mul[r] * col_mul[c] in fp32.
+ * colsum_partial (nullable): fp32 [ceil(rows/128), cols] column sums of the
+ * source, before the cast. Writes no code past column cols (rows for dst_t).
+ */
+int apa_block_cast(const void* src, int src_dtype, int64_t rows, int64_t cols, int64_t ld_src,
+                   const float* row_mul, const void* col_mul, int col_mul_dtype, int square,
+                   void* dst, int64_t ld_dst, void* scales, void* dst_t, int64_t ld_dst_t, void* scales_t,
+                   float* colsum_partial, void* stream);
+
+/* Values of a block tensor in dst_dtype (F32, F16, BF16). */
+int apa_block_dequant(const void* src, int64_t ld, const void* scales, int64_t rows, int64_t cols, void* dst,
+                      int dst_dtype, int64_t ld_dst, void* stream);
+
+/* Sum of the rows of partial [parts, cols] in a fixed order, rounded once to
+ * out_dtype (F32, F16, BF16): a bias or norm weight gradient. */
+int apa_block_colsum(const float* partial, int64_t parts, int64_t cols, void* out, int out_dtype, void* stream);
+
+/*
+ * out[M, N] = a[M, K] . b[N, K]^T + bias[N] for block tensors a and b,
+ * accumulated in fp32, rounded once to out_dtype (F32, F16, BF16). bias
+ * (nullable): F32, F16 or BF16. accumulate != 0 (F32 only): add to out.
+ * Deterministic; no workspace.
+ */
+int apa_block_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
+                   const void* b_scales, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo,
+                   int64_t M, int64_t N, int64_t K, int accumulate, void* stream);
+
+/*
+ * Root-mean-square norm: r = x + residual rounded to dtype and stored in
+ * stream_out (both null: r = x), then r * (mean r^2 + eps)^(-1/2) * gamma,
+ * either to y (dtype) or to the block tensor (q, scales); exactly one of y and
+ * q is given. rstd (nullable): fp32 [rows], what the backward needs. dtype and
+ * gamma_dtype: F32, F16 or BF16. cols <= 32768 (else APA_ERR_UNSUPPORTED).
+ */
+int apa_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t ld_res, const void* gamma,
+                    int gamma_dtype, int dtype, int64_t rows, int64_t cols, float eps, void* stream_out,
+                    int64_t ld_stream, void* y, int64_t ld_y, void* q, int64_t ld_q, void* scales, float* rstd,
+                    void* stream);
+
+/* Scratch bytes of apa_rmsnorm_bwd on the current device. */
+int apa_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int64_t* bytes_out);
+
+/*
+ * Gradients of apa_rmsnorm_fwd from dy (of the output), r (the stream), rstd
+ * and dr (nullable: the gradient of the stream itself): dx, of x and residual
+ * alike (dtype), and dgamma (gamma_dtype). Deterministic. workspace: 16-byte
+ * aligned, apa_rmsnorm_bwd_workspace bytes, used only during the call.
+ */
+int apa_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* r, int64_t ld_r, const float* rstd,
+                    const void* gamma, int gamma_dtype, const void* dr, int64_t ld_dr, void* dx, int64_t ld_dx,
+                    int dtype, int64_t rows, int64_t cols, void* dgamma, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
 int apa_ladder_pack(int L, const float* const* amax_ptr, const float* const* ratio_ptr,
                     const int32_t* const* flag_ptr, int O, const float* const* oamax_ptr,
                     const int32_t* const* oflag_ptr, int32_t* packed, void* stream);
