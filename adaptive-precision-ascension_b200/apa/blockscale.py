@@ -239,11 +239,11 @@ def block_cast(x: torch.Tensor, form: str = "rows", square: bool = False):
     return (q, qt) if form == "both" else q if form == "rows" else qt
 
 
-def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool) -> None:
+def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool, plan: int = 0) -> None:
     M, K = a.shape
     _call(a.device, "apa_block_gemm", a.data.data_ptr(), _pitch(a), a.scales.data_ptr(), b.data.data_ptr(), _pitch(b),
           b.scales.data_ptr(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, out.data_ptr(),
-          _REAL[out.dtype], _ld(out), M, b.shape[0], K, int(accumulate), _lib.stream_handle(a.device))
+          _REAL[out.dtype], _ld(out), M, b.shape[0], K, int(accumulate), plan, _lib.stream_handle(a.device))
 
 
 def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,

@@ -20,6 +20,12 @@
 //   tile keep every SM's loads in flight; for a small weight gradient over
 //   many tokens the split is what fills the SMs. No workspace, no atomics: the
 //   result does not depend on timing.
+//
+// pair_kernel  256 x 256 tiles on CTA pairs (tcgen05 cta_group::2), persistent,
+//   for everything large: bound by the tensor cores. Two accumulators of 256
+//   columns fill tensor memory, which leaves none for the scales, so they
+//   overlap by 16 columns: the next tile's MMAs start as soon as the epilogue
+//   has read the shared columns, which it reads first.
 #include <cuda.h>
 #include <mutex>
 #include "block_scale.cuh"
@@ -98,64 +104,38 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 
-// C consecutive accumulator columns of one row. Not swapped: row m, columns
-// n0 ..; swapped: weight row n of tokens m0 .. (neighbouring lanes hold
-// neighbouring n, so every store instruction writes whole sectors).
-template <int C>
-__device__ __forceinline__ void put(const OutArgs& o, bool swap, int row, int col, float (&v)[C]) {
-  if (swap) {
-    const int n = row;
-    if (n >= o.N) return;
-    const float b = o.bias ? to_f32(o.bias, o.bias_dt, n) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int m = col + j;
-      if (m < o.M) {
-        const int64_t at = (int64_t)m * o.ldo + n;
-        float x = v[j] + b;
-        if (o.accumulate) x += static_cast<const float*>(o.out)[at];
-        from_f32(o.out, o.out_dt, at, x);
-      }
-    }
-    return;
-  }
-  const int m = row;
-  if (m >= o.M || col >= o.N) return;
-  const int64_t at = (int64_t)m * o.ldo + col;
+// Four neighbouring elements of one output row: bias, accumulation, rounding.
+// vec: the row's addresses allow one store.
+__device__ __forceinline__ void put4(const OutArgs& o, int m, int n, float4 x) {
+  float v[4] = {x.x, x.y, x.z, x.w};
+  const int64_t at = (int64_t)m * o.ldo + n;
+  const int c = min(4, o.N - n);
   if (o.bias) {
 #pragma unroll
-    for (int j = 0; j < C; ++j)
-      if (col + j < o.N) v[j] += to_f32(o.bias, o.bias_dt, col + j);
+    for (int j = 0; j < 4; ++j)
+      if (j < c) v[j] += to_f32(o.bias, o.bias_dt, n + j);
   }
-  if (C % 8 == 0 && o.vec && col + C <= o.N) {
+  if (o.vec && c == 4) {
     if (o.out_dt == APA_DT_F32) {
       float4* d = reinterpret_cast<float4*>(static_cast<float*>(o.out) + at);
-#pragma unroll
-      for (int q = 0; q < C / 4; ++q) {
-        float4 x = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        if (o.accumulate) {
-          const float4 y = d[q];
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-        }
-        d[q] = x;
+      if (o.accumulate) {
+        const float4 y = *d;
+        v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
       }
+      *d = make_float4(v[0], v[1], v[2], v[3]);
     } else {
-      uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(o.out) + at);
-      uint32_t w[C / 2];
-#pragma unroll
-      for (int j = 0; j < C / 2; ++j)
-        w[j] = o.out_dt == APA_DT_BF16 ? bf16x2(v[2 * j], v[2 * j + 1]) : f16x2_from_f32(v[2 * j], v[2 * j + 1]);
-#pragma unroll
-      for (int q = 0; q < C / 8; ++q) d[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      uint2 w;
+      if (o.out_dt == APA_DT_BF16) w = make_uint2(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]));
+      else w = make_uint2(f16x2_from_f32(v[0], v[1]), f16x2_from_f32(v[2], v[3]));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(o.out) + at) = w;
     }
     return;
   }
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    if (col + j < o.N) {
-      float x = v[j];
-      if (o.accumulate) x += static_cast<const float*>(o.out)[at + j];
-      from_f32(o.out, o.out_dt, at + j, x);
+  for (int j = 0; j < 4; ++j) {
+    if (j < c) {
+      if (o.accumulate) v[j] += static_cast<const float*>(o.out)[at + j];
+      from_f32(o.out, o.out_dt, at + j, v[j]);
     }
   }
 }
@@ -173,7 +153,7 @@ template <int BN> struct SplitCfg {
   static constexpr int kTmemCols = BN == 128 ? 256 : BN == 64 ? 128 : BN == 32 ? 64 : 32;
   static constexpr int kSmemBytes = kStages * (kStageBytes + kScaleBytes) + 1024 + 256;
   static constexpr int kThreads = 192;
-  static_assert(BN * BM * 4 <= kStages * kStageBytes, "the partial tile reuses the stages");
+  static_assert((BN + 4) * BM * 4 <= kStages * kStageBytes, "the tile reuses the stages");
   static_assert(BN + 8 <= kTmemCols, "tensor memory");
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 };
@@ -257,7 +237,8 @@ __global__ void __launch_bounds__(192, 2)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      // rows b0 .. of a chunk of 128 start at scale column (b0 % 128) / 32
+      // rows b0 .. of a chunk of 128 start at scale column (b0 % 128) / 32: 0
+      // or, for the second tile of 64 rows, 2 (an odd column faults)
       const uint32_t sfb0 = sfb + (uint32_t)((b0 & 127) >> 5);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&full[stage], phase, kStatusTimeoutFull)) { ok = false; break; }
@@ -290,71 +271,348 @@ __global__ void __launch_bounds__(192, 2)
     fence_after();
   }
   const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-  const int row = a0 + q * 32 + lane;
   constexpr int kC = BN >= 32 ? 32 : 16;
-  if (p.split == 1) {
-    if (warp >= 2 && ready) {
+  // The tile goes through shared memory in the output's order, over the
+  // operand stages (every load has landed and every MMA has read it once
+  // `done` completes): [128][BN + 4], or [BN][128] when swapped. Both orders
+  // are written and read without bank conflicts.
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2 && ready) {
 #pragma unroll 1
-      for (int c = 0; c < BN; c += kC) {
-        if (b0 + c >= p.rows_b) break;
-        uint32_t r[kC];
-        if constexpr (kC == 32) gemm::tmem_ld32_nowait(lanes + c, r);
-        else tmem_ld16(lanes + c, r);
-        gemm::tmem_wait_ld();
-        float v[kC];
-#pragma unroll
-        for (int j = 0; j < kC; ++j) v[j] = fu(r[j]);
-        put<kC>(p.o, p.swap != 0, row, b0 + c, v);
-      }
-    }
-  } else {
-    // partial tiles, column major ([BN][128] fp32), over the operand stages:
-    // every load has landed and every MMA has read it once `done` completes
-    float* part = reinterpret_cast<float*>(smem);
-    if (warp >= 2 && ready) {
-#pragma unroll 1
-      for (int c = 0; c < BN; c += kC) {
-        uint32_t r[kC];
-        if constexpr (kC == 32) gemm::tmem_ld32_nowait(lanes + c, r);
-        else tmem_ld16(lanes + c, r);
-        gemm::tmem_wait_ld();
+    for (int c = 0; c < BN; c += kC) {
+      if (b0 + c >= p.rows_b) break;
+      uint32_t r[kC];
+      if constexpr (kC == 32) gemm::tmem_ld32_nowait(lanes + c, r);
+      else tmem_ld16(lanes + c, r);
+      gemm::tmem_wait_ld();
+      if (p.swap) {
 #pragma unroll
         for (int j = 0; j < kC; ++j) part[(c + j) * BM + q * 32 + lane] = fu(r[j]);
+      } else {
+        float4* d = reinterpret_cast<float4*>(part + (q * 32 + lane) * (BN + 4) + c);
+#pragma unroll
+        for (int j = 0; j < kC / 4; ++j)
+          d[j] = make_float4(fu(r[4 * j]), fu(r[4 * j + 1]), fu(r[4 * j + 2]), fu(r[4 * j + 3]));
       }
     }
-    __syncwarp();
-    gemm::cluster_sync();
-    if (warp >= 2 && ready) {
-      // this rank's columns (split <= 8), in groups that make 16-byte stores
-      // where a rank has eight columns or more
-      constexpr int kG = BN >= 64 ? 8 : 2;
-      const int per = BN / p.split;
-      for (int c = rank * per; c < (rank + 1) * per; c += kG) {
-        if (b0 + c >= p.rows_b) break;
-        float v[kG];
+  }
+  __syncwarp();
+  if (p.split == 1) __syncthreads();
+  else gemm::cluster_sync();
+  if (warp >= 2 && ready) {
+    // units of four elements along the output's rows, the ranks' shares one
+    // after the other; a unit's partials are added in rank order
+    const int outer = p.swap ? min(BN, p.rows_b - b0) : min(BM, p.rows_a - a0);
+    const int per = p.swap ? BM / 4 : BN / 4;
+    const int pitch = p.swap ? BM : BN + 4;
+    const int m0 = p.swap ? b0 : a0, n0 = p.swap ? a0 : b0;
+    const int units = outer * per;
+    const int u1 = units * (rank + 1) / p.split;
+    for (int u = units * rank / p.split + (int)threadIdx.x - 64; u < u1; u += 128) {
+      const int i = u / per, j = u - i * per;
+      if (n0 + 4 * j >= p.o.N) continue;
+      const float* at = part + i * pitch + 4 * j;
+      float4 x;
+      if (p.split == 1) {
+        x = *reinterpret_cast<const float4*>(at);
+      } else {
+        float4 y[8];
 #pragma unroll
-        for (int j = 0; j < kG; ++j) v[j] = 0.0f;
-        for (int s = 0; s < p.split; ++s) {
-          const uint32_t at = gemm::map_to_cta(part + c * BM + q * 32 + lane, (uint32_t)s);
-#pragma unroll
-          for (int j = 0; j < kG; ++j) {
-            float x;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at + (uint32_t)(j * BM * 4)));
-            v[j] += x;
+        for (int s = 0; s < 8; ++s) {
+          if (s < p.split) {
+            const uint32_t a = gemm::map_to_cta(at, (uint32_t)s);
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(y[s].x), "=f"(y[s].y), "=f"(y[s].z), "=f"(y[s].w)
+                         : "r"(a));
           }
         }
-        put<kG>(p.o, p.swap != 0, row, b0 + c, v);
+        x = y[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) {
+          if (s < p.split) { x.x += y[s].x; x.y += y[s].y; x.z += y[s].z; x.w += y[s].w; }
+        }
       }
+      put4(p.o, m0 + i, n0 + 4 * j, x);
     }
-    __syncwarp();
-    gemm::cluster_sync();   // no CTA leaves while another reads its partials
   }
+  __syncwarp();
+  if (p.split > 1) gemm::cluster_sync();   // no CTA leaves while another reads its partials
   fence_before();
   __syncthreads();
   fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::kTmemCols)
                  : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// pair_kernel
+// ---------------------------------------------------------------------------
+constexpr int kEpiBox = 4096;      // one staging buffer: 32 rows x 128 bytes
+constexpr int kAccStride = 240;    // second accumulator: columns 240 .. 495
+constexpr int kPairSfa = 496, kPairSfb = 500;   // 4 columns of A's scales, 8 of B's
+
+template <int EW> struct PairCfg {
+  static constexpr int kTile = 256;
+  static constexpr int kHalfBytes = BM * kSlab;                 // this CTA's rows of A, and of B
+  static constexpr int kStageBytes = 2 * kHalfBytes;
+  static constexpr int kScaleBytes = 512 + 1024;                // own 128 rows of A, all 256 of B
+  static constexpr int kStages = EW == 4 ? 6 : 5;
+  static constexpr int kWarpCols = 1024 / EW;                   // columns per epilogue warp
+  static constexpr int kUnits = kWarpCols / 64;
+  static constexpr int kThreads = 64 + 32 * EW;
+  static constexpr int kSmemBytes =
+      kStages * (kStageBytes + kScaleBytes) + EW * (kEpiBox + kWarpCols * 4) + 256 + 1024;
+  static_assert(kSmemBytes <= 232448, "shared memory");
+};
+
+struct PairArgs {
+  int kb_count;
+  int tma_out;          // out written by TMA stores (aligned, not accumulated)
+  OutArgs o;
+};
+
+// A staged box (32 rows of 128 bytes, 128-byte swizzle) to rows that TMA
+// cannot store to (unaligned, a ragged last 16 bytes, or accumulated): one row
+// per step, one 4-byte word per lane, so a warp's store covers whole lines.
+__device__ __forceinline__ void put_box(const OutArgs& o, const uint8_t* box, int lane, int row0, int col0) {
+  const bool out16 = o.out_dt != APA_DT_F32;
+  const int rows = min(32, o.M - row0);
+  const int col = col0 + (out16 ? 2 * lane : lane);
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const uint32_t w =
+        *reinterpret_cast<const uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    const int64_t at = (int64_t)(row0 + r) * o.ldo + col;
+    if (out16) {
+      uint16_t* d = static_cast<uint16_t*>(o.out) + at;
+      if (col + 1 < o.N && (reinterpret_cast<uintptr_t>(d) & 3u) == 0) {
+        *reinterpret_cast<uint32_t*>(d) = w;
+      } else {
+        if (col < o.N) d[0] = (uint16_t)w;
+        if (col + 1 < o.N) d[1] = (uint16_t)(w >> 16);
+      }
+    } else if (col < o.N) {
+      float* d = static_cast<float*>(o.out) + at;
+      *d = o.accumulate ? *d + fu(w) : fu(w);
+    }
+  }
+}
+
+template <int EW>
+__global__ void __launch_bounds__(64 + 32 * EW, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                const __grid_constant__ CUtensorMap tmO, PairArgs p) {
+  using C = PairCfg<EW>;
+  constexpr int kStages = C::kStages;
+  pdl_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* smA = smem;
+  uint8_t* smB = smem + kStages * C::kHalfBytes;
+  uint8_t* smE = smem + kStages * C::kStageBytes;                         // staging boxes, 128-byte swizzled
+  uint8_t* smS = smE + EW * kEpiBox;
+  float* smBias = reinterpret_cast<float*>(smS + kStages * C::kScaleBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smBias + EW * C::kWarpCols);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* tshared = tempty + 2;          // the overlapping columns of the current tile have been read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tshared + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = gemm::cluster_rank();
+  const int num_m = (p.o.M + 255) / 256, num_n = (p.o.N + 255) / 256;
+  const int tiles = num_m * num_n;
+  const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+  constexpr int kGroup = gemm::kGroupM / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], EW * 2);
+    }
+    mbar_init(tshared, 4 * 2);             // four warps of each CTA hold those columns
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  gemm::cluster_sync();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int mb, nb;
+        gemm::tile_coords(t, num_m, num_n, kGroup, mb, nb);
+        const int a_row = mb * 256 + (int)rank * BM, b_row = nb * 256 + (int)rank * BM;
+        for (int kb = 0; kb < p.kb_count; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty)) { ok = false; break; }
+          const bool scales = (kb & 3) == 0;
+          // the even CTA's barrier expects both CTAs' bytes
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * (C::kStageBytes + (scales ? C::kScaleBytes : 0)));
+          const uint32_t bar = gemm::map_to_cta(&full[stage], 0);
+          gemm::tma_load_2d_pair(smA + stage * C::kHalfBytes, &tmA, kb * kSlab, a_row, bar);
+          gemm::tma_load_2d_pair(smB + stage * C::kHalfBytes, &tmB, kb * kSlab, b_row, bar);
+          if (scales) {
+            uint8_t* s = smS + stage * C::kScaleBytes;
+            gemm::tma_load_2d_pair(s, &tmSA, a_row, kb >> 2, bar);
+            gemm::tma_load_2d_pair(s + 512, &tmSB, nb * 256, kb >> 2, bar);
+          }
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // until the MMAs have released every stage
+      for (int i = 0; ok && i < kStages; ++i) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty)) ok = false;
+        if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t sfa = tmem + kPairSfa, sfb = tmem + kPairSfb;
+      for (int t = first; ok && t < tiles; t += step, ++local) {
+        const int acc = local & 1;
+        if (!mbar_wait<true>(&tempty[acc], ((uint32_t)(local >> 1) & 1u) ^ 1u, kStatusTimeoutAcc)) { ok = false; break; }
+        // the previous tile's shared columns
+        if (local > 0 && !mbar_wait<true>(tshared, (uint32_t)(local - 1) & 1u, kStatusTimeoutAcc)) { ok = false; break; }
+        fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * kAccStride);
+        for (int kb = 0; kb < p.kb_count; ++kb) {
+          if (!mbar_wait(&full[stage], phase, kStatusTimeoutFull)) { ok = false; break; }
+          fence_after();
+          const uint32_t j = (uint32_t)(kb & 3);
+          if (j == 0) {
+            const uint32_t s = smem_u32(smS + stage * C::kScaleBytes);
+            scale_copy<true>(sfa, s);
+            scale_copy<true>(sfb, s + 512);
+            scale_copy<true>(sfb + 4, s + 1024);
+          }
+          const uint32_t id = mx_idesc<256, 256>() | (j << 4) | (j << 29);
+          const uint32_t a = smem_u32(smA + stage * C::kHalfBytes), b = smem_u32(smB + stage * C::kHalfBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx_mma<true>(d, sdesc(a + 32 * k), sdesc(b + 32 * k), id, sfa, sfb, (kb != 0 || k != 0) ? 1u : 0u);
+          gemm::mma_commit<true>(&empty[stage]);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) gemm::mma_commit<true>(&tfull[acc]);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, e = warp - 2, part = e >> 2;
+    uint8_t* box = smE + e * kEpiBox;
+    float* sb = smBias + e * C::kWarpCols;
+    const bool out16 = p.o.out_dt != APA_DT_F32;
+    int local = 0;
+    bool pending = false;                 // a TMA store of this warp may still read its box
+    const uint32_t te0 = gemm::map_to_cta(&tempty[0], 0), te1 = gemm::map_to_cta(&tempty[1], 0);
+    const uint32_t ts = gemm::map_to_cta(tshared, 0);
+    auto arrive = [&](uint32_t bar) {
+      fence_before();
+      __syncwarp();
+      if (lane == 0) gemm::mbar_arrive_cluster(bar);
+    };
+    for (int t = first; t < tiles; t += step, ++local) {
+      int mb, nb;
+      gemm::tile_coords(t, num_m, num_n, kGroup, mb, nb);
+      const int acc = local & 1;
+      const int row0 = mb * 256 + (int)rank * BM + q * 32;
+      const int col_base = nb * 256 + part * C::kWarpCols;
+      if (p.o.bias != nullptr) {
+        __syncwarp();
+        for (int c = lane; c < C::kWarpCols; c += 32)
+          sb[c] = col_base + c < p.o.N ? to_f32(p.o.bias, p.o.bias_dt, col_base + c) : 0.0f;
+        __syncwarp();
+      }
+      bool ready = true;
+      if (lane == 0) ready = mbar_wait(&tfull[acc], (uint32_t)(local >> 1) & 1u, kStatusTimeoutAcc);
+      ready = __shfl_sync(0xFFFFFFFFu, ready ? 1 : 0, 0) != 0;
+      if (!ready) break;
+      fence_after();
+      const uint32_t tb = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kAccStride + part * C::kWarpCols);
+      // the columns the two accumulators share are the last of the first one
+      // and the first of the second: those go first
+      const int shared_part = acc == 0 ? EW / 4 - 1 : 0;
+#pragma unroll 1
+      for (int i = 0; i < C::kUnits; ++i) {
+        const int u = acc == 0 ? C::kUnits - 1 - i : i;
+        const int col0 = col_base + u * 64;
+        uint32_t r[64];
+        gemm::tmem_ld32_nowait(tb + (uint32_t)(u * 64), r);
+        gemm::tmem_ld32_nowait(tb + (uint32_t)(u * 64 + 32), r + 32);
+        gemm::tmem_wait_ld();
+        if (i == 0 && part == shared_part) arrive(ts);
+        if (i == C::kUnits - 1) arrive(acc ? te1 : te0);
+        if (col0 >= p.o.N || row0 >= p.o.M) continue;      // warp-uniform
+        if (p.o.bias != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float4 b = reinterpret_cast<const float4*>(sb + u * 64)[c];
+            gemm::add2(r[4 * c], r[4 * c + 1], b.x, b.y);
+            gemm::add2(r[4 * c + 2], r[4 * c + 3], b.z, b.w);
+          }
+        }
+        if (out16) {
+          if (p.o.out_dt == APA_DT_BF16) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = bf16x2(fu(r[2 * k]), fu(r[2 * k + 1]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = f16x2_from_f32(fu(r[2 * k]), fu(r[2 * k + 1]));
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int x = col0 + 32 * b;
+          if ((out16 && b == 1) || x >= p.o.N) break;
+          if (pending && lane == 0) gemm::bulk_wait_read<0>();
+          __syncwarp();
+          gemm::stage_row(box, lane, r + 32 * b);
+          if (p.tma_out) {
+            gemm::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              gemm::tma_store_2d(&tmO, box, x, row0);
+              gemm::bulk_commit();
+            }
+            pending = true;
+          } else {
+            __syncwarp();
+            put_box(p.o, box, lane, row0, x);
+          }
+        }
+      }
+    }
+    if (pending && lane == 0) gemm::bulk_wait_all();
+    __syncwarp();
+  }
+
+  // neither CTA leaves while the other may signal its barriers or read its tensor memory
+  fence_before();
+  gemm::cluster_sync();
+  fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -387,6 +645,8 @@ int scale_map(CUtensorMap* tm, const void* p, int64_t rows, int64_t kb_count, in
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? APA_OK : APA_ERR_CUDA;
 }
+
+int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Operand { const void* q; int64_t ld; const void* sc; int64_t rows; };
 
@@ -425,22 +685,119 @@ int launch_split(const Operand& A, const Operand& B, int64_t K, const OutArgs& o
                        tsb, p) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }
 
-struct BlockPlan { int kind, bn, split, swap; };   // kind 0: split_kernel
+// Output: dims {N, M}, box {128 bytes, 32 rows}, 128-byte swizzle.
+int out_map(CUtensorMap* tm, const OutArgs& o) {
+  gemm::EncodeFn enc = gemm::get_encode();
+  if (!enc) return APA_ERR_CUDA;
+  const int es = elem_bytes(o.out_dt);
+  const CUtensorMapDataType dt = o.out_dt == APA_DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : o.out_dt == APA_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)o.N, (cuuint64_t)o.M};
+  cuuint64_t strides[1] = {(cuuint64_t)(o.ldo * es)};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
+  cuuint32_t one[2] = {1, 1};
+  return enc(tm, dt, 2, o.out, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? APA_OK
+                                                                                                 : APA_ERR_CUDA;
+}
 
-int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// CTA pairs of the kernel that run at once on the current device (0: none).
+template <int EW>
+int pair_slots() {
+  using C = PairCfg<EW>;
+  static unsigned long long attr = 0;
+  static int slots[64];        // per device; written before its bit of `known`
+  static unsigned long long known = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  dev &= 63;
+  if (__atomic_load_n(&known, __ATOMIC_ACQUIRE) >> dev & 1ull) return slots[dev];
+  if (allow_smem(pair_kernel<EW>, C::kSmemBytes, &attr)) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * num_sms(), 1, 1);
+  cfg.blockDim = dim3(C::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<EW>, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    n = 0;
+  }
+  slots[dev] = n;
+  __atomic_fetch_or(&known, 1ull << dev, __ATOMIC_RELEASE);
+  return n;
+}
+
+template <int EW>
+int launch_pair(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, cudaStream_t s) {
+  using C = PairCfg<EW>;
+  int slots = pair_slots<EW>();
+  if (slots < 1) return APA_ERR_UNSUPPORTED;
+  if (g_gemm_sm_limit > 0) slots = std::max(1, std::min(slots, g_gemm_sm_limit / 2));
+  const int64_t kb = (K + kSlab - 1) / kSlab;
+  CUtensorMap ta, tb, tsa, tsb, to;
+  if (int st = code_map(&ta, A.q, A.rows, K, A.ld, BM)) return st;
+  if (int st = code_map(&tb, B.q, B.rows, K, B.ld, BM)) return st;
+  if (int st = scale_map(&tsa, A.sc, A.rows, kb, 128)) return st;
+  if (int st = scale_map(&tsb, B.sc, B.rows, kb, 256)) return st;
+  PairArgs p;
+  p.kb_count = (int)kb; p.o = o;
+  // a TMA store writes whole 16-byte pieces, past N too where N ends inside one
+  p.tma_out = o.vec && !o.accumulate && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0;
+  to = ta;
+  if (p.tma_out)
+    if (int st = out_map(&to, o)) return st;
+  const int64_t tiles = cdiv64(o.M, 256) * cdiv64(o.N, 256);
+  const int grid = 2 * (int)std::min<int64_t>(tiles, slots);
+  return launch_kernel(pair_kernel<EW>, dim3(grid), dim3(C::kThreads), C::kSmemBytes, s, 2, ta, tb, tsa, tsb, to, p) ==
+                 cudaSuccess ? APA_OK : APA_ERR_CUDA;
+}
+
+// kind 0: split_kernel with `bn`, `split` and `swap`; 1: pair_kernel with `ew`
+// epilogue warps.
+struct BlockPlan { int kind, bn, split, swap, ew; int64_t rows_m; };
 
 BlockPlan block_plan(int64_t M, int64_t N, int64_t K) {
-  BlockPlan p{0, 128, 1, 0};
+  BlockPlan p{0, 128, 1, 0, 4, M};
   const int64_t kb = cdiv64(K, kSlab);
   p.swap = M <= 128 && M < N;
   const int64_t small = p.swap ? M : N, big = p.swap ? N : M;
   p.bn = small <= 16 ? 16 : small <= 32 ? 32 : small <= 64 ? 64 : 128;
   const int64_t tiles = cdiv64(big, BM) * cdiv64(small, p.bn);
   while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && p.split * 2 * 2 <= kb) p.split *= 2;
+  const int64_t pt = cdiv64(M, 256) * cdiv64(N, 256);
+  if (pt >= 64) p.kind = 1;
   return p;
 }
 
+// A caller's choice (APA_BLOCK_*): the automatic plan stands where it is 0.
+int force_plan(int code, int64_t N, int64_t K, BlockPlan* p) {
+  if (code == APA_BLOCK_AUTO) return APA_OK;
+  if (code == APA_BLOCK_PAIR_4 || code == APA_BLOCK_PAIR_8) {
+    p->kind = 1;
+    p->ew = code == APA_BLOCK_PAIR_4 ? 4 : 8;
+    return APA_OK;
+  }
+  const int bn = code & 0xFF, split = (code >> 8) & 0xFF, swap = (code >> 16) & 1;
+  if ((code >> 17) != 0 || (bn != 16 && bn != 32 && bn != 64 && bn != 128)) return APA_ERR_INVALID;
+  if (split != 1 && split != 2 && split != 4 && split != 8) return APA_ERR_INVALID;
+  if (split > cdiv64(K, kSlab)) return APA_ERR_INVALID;       // no CTA without a slab
+  p->kind = 0;
+  p->bn = bn; p->split = split; p->swap = swap;
+  // the MMA takes scales from even columns of tensor memory only, 64 rows
+  // apart: narrower tiles are for a side of one tile
+  return bn < 64 && (swap ? p->rows_m : N) > bn ? APA_ERR_INVALID : APA_OK;
+}
+
 int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, const BlockPlan& p, cudaStream_t s) {
+  if (p.kind == 1) return p.ew == 8 ? launch_pair<8>(A, B, K, o, s) : launch_pair<4>(A, B, K, o, s);
   const Operand& x = p.swap ? B : A;
   const Operand& y = p.swap ? A : B;
   switch (p.bn) {
@@ -456,7 +813,7 @@ int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, 
 
 extern "C" int apa_block_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
                               const void* b_scales, const void* bias, int bias_dtype, void* out, int out_dtype,
-                              int64_t ldo, int64_t M, int64_t N, int64_t K, int accumulate, void* stream) {
+                              int64_t ldo, int64_t M, int64_t N, int64_t K, int accumulate, int plan, void* stream) {
   using namespace apa::blk;
   if (M <= 0 || N <= 0 || K <= 0) return APA_ERR_INVALID;
   if (M > (1ll << 31) - 256 || N > (1ll << 31) - 256 || K > (1ll << 31) - 256) return APA_ERR_INVALID;
@@ -468,6 +825,7 @@ extern "C" int apa_block_gemm(const void* a, int64_t lda, const void* a_scales, 
   if (((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 15u) != 0) return APA_ERR_ALIGN;
   OutArgs o{out, ldo, out_dtype, bias, bias_dtype, accumulate ? 1 : 0, vec16(out, ldo, es) ? 1 : 0, (int)M, (int)N};
   const Operand A{a, lda, a_scales, M}, B{b, ldb, b_scales, N};
-  const BlockPlan p = block_plan(M, N, K);
+  BlockPlan p = block_plan(M, N, K);
+  if (int st = force_plan(plan, N, K, &p)) return st;
   return block_gemm(A, B, K, o, p, static_cast<cudaStream_t>(stream));
 }

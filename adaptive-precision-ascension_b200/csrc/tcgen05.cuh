@@ -8,6 +8,11 @@
 #include "apa_common.cuh"
 
 namespace apa {
+
+// Upper bound on the persistent grid (0 = one CTA per SM). Set while a
+// collective runs concurrently, so its kernel finds free SMs.
+static int g_gemm_sm_limit = 0;
+
 namespace gemm {
 
 constexpr int BM = 128;
@@ -238,6 +243,41 @@ __device__ __forceinline__ uint32_t bf16x2_from_f32(float lo, float hi) {
 }
 
 __device__ __forceinline__ float fu(uint32_t u) { return __uint_as_float(u); }
+
+// x0 += b0, x1 += b1 (fp32 words) in one packed instruction; add.rn.f32x2
+// rounds each lane exactly as add.rn.f32 does.
+__device__ __forceinline__ void add2(uint32_t& x0, uint32_t& x1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+r"(x0), "+r"(x1)
+      : "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+
+// Stage 32 words (128 bytes) of this lane's row into the warp's 4 KB buffer
+// in the 128-byte-swizzled layout the output tensor map expects (16-byte
+// chunk c of row r lands at chunk c ^ (r % 8)): conflict-free stores.
+__device__ __forceinline__ void stage_row(uint8_t* buf, int lane, const uint32_t* w) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+
+// Tile order: groups of kGroupM consecutive M blocks, N advancing across a
+// group and M fastest inside it, so the CTAs running at the same time share
+// their B tiles (and a group's A rows) in L2 even when B is larger than L2
+// (e.g. a 50k-row vocabulary projection).
+constexpr int kGroupM = 16;
+
+__device__ __forceinline__ void tile_coords(int tile, int num_m, int num_n, int group, int& m_blk, int& n_blk) {
+  const int group_tiles = group * num_n;
+  const int g = tile / group_tiles;
+  const int first_m = g * group;
+  const int gs = min(group, num_m - first_m);
+  const int local = tile - g * group_tiles;
+  m_blk = first_m + local % gs;
+  n_blk = local / gs;
+}
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

@@ -241,3 +241,111 @@ def test_graph_capture():
         torch.cuda.synchronize()
         assert torch.equal(y, block_linear(x, wq))
     assert not torch.equal(ref, y)
+
+
+# plans of apa_block_gemm: the CTA pair with 4 or 8 epilogue warps, and the
+# split tile (columns, CTAs per tile, swapped)
+PAIRS = {"pair4": 1, "pair8": 2}
+
+
+def split_plan(bn, split, swap):
+    return bn | split << 8 | swap << 16
+
+
+def exact_operands(m, n, k, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    a = torch.randint(-4, 5, (m, k), generator=g, device="cuda").float()
+    b = torch.randint(-4, 5, (n, k), generator=g, device="cuda").float()
+    ea = torch.randint(-1, 2, (m, (k + 127) // 128), generator=g, device="cuda")
+    eb = torch.randint(-1, 2, (n, (k + 127) // 128), generator=g, device="cuda")
+    A = APABlockTensor.from_parts(a.to(torch.float8_e4m3fn), ea)
+    B = APABlockTensor.from_parts(b.to(torch.float8_e4m3fn), eb)
+    want = A.dequantize().double() @ B.dequantize().double().t()
+    return A, B, want
+
+
+@pytest.mark.parametrize("plan", sorted(PAIRS))
+@pytest.mark.parametrize("m,n,k", [
+    (256, 256, 128), (257, 1, 1), (1, 257, 600), (300, 500, 1000), (1023, 777, 520),
+    (2560, 2560, 256),      # 100 tiles: more than one on some CTA pairs
+    (5000, 2600, 384),      # 220 tiles: both accumulators of a pair reused
+    (4096, 4096, 128)])     # 256 tiles of one slab: the epilogue is the bound
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pair_plan_exact(plan, m, n, k, dtype):
+    from apa import blockscale
+    A, B, want = exact_operands(m, n, k, m + n)
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    blockscale._matmul(A, B, None, out, False, PAIRS[plan])
+    assert torch.equal(out, want.to(dtype))
+    bias = torch.randint(-9, 9, (n,), device="cuda").float()
+    blockscale._matmul(A, B, bias, out, False, PAIRS[plan])
+    assert torch.equal(out, (want + bias.double()).to(dtype))
+
+
+@pytest.mark.parametrize("plan", [*sorted(PAIRS), split_plan(128, 1, 0), split_plan(128, 4, 0), split_plan(64, 2, 1)])
+@pytest.mark.parametrize("pitch,off", [(0, 0), (1, 0), (8, 4), (5, 3)])
+def test_plans_write_inside_their_output(plan, pitch, off):
+    """Aligned and unaligned rows, overwrite and accumulate: the bytes around stay."""
+    from apa import blockscale
+    m, n, k = 700, 333, 1100
+    A, B, want = exact_operands(m, n, k, 5)
+    code = PAIRS.get(plan, plan)
+    for dtype in DTYPES:
+        buf = torch.full((m + 2, n + pitch + off + 3), 3.0, dtype=dtype, device="cuda")
+        out = buf[1:m + 1, off:off + n]
+        blockscale._matmul(A, B, None, out, False, code)
+        assert torch.equal(out, want.to(dtype))
+        if dtype == torch.float32:
+            blockscale._matmul(A, B, None, out, True, code)
+            assert torch.equal(out, (2 * want).float())
+        out.fill_(3.0)
+        assert bool((buf == 3.0).all())
+
+
+@pytest.mark.parametrize("bn", [16, 32, 64, 128])
+@pytest.mark.parametrize("split", [1, 2, 4, 8])
+@pytest.mark.parametrize("swap", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_split_plan_exact(bn, split, swap, dtype):
+    """Every tile width, split and orientation, over ragged sizes and uneven splits of the slabs."""
+    from apa import blockscale
+    small = {16: 13, 32: 29, 64: 139, 128: 300}[bn]
+    for big, k in ((200, 1024), (129, 1157)):
+        m, n = (small, big) if swap else (big, small)
+        A, B, want = exact_operands(m, n, k, bn + split)
+        bias = torch.randint(-9, 9, (n,), device="cuda").float()
+        out = torch.empty(m, n, dtype=dtype, device="cuda")
+        blockscale._matmul(A, B, bias, out, False, split_plan(bn, split, swap))
+        assert torch.equal(out, (want + bias.double()).to(dtype))
+
+
+def test_plans_agree_on_real_data():
+    from apa import blockscale
+    a = block_cast(rnd((1500, 1300), 1).cuda())
+    b = block_cast(rnd((900, 1300), 2).cuda(), square=True)
+    av, bv = f64(a.dequantize()), f64(b.dequantize())
+    want, tol = av @ bv.T, None
+    for plan in (1, 2, split_plan(128, 1, 0), split_plan(128, 8, 1), split_plan(64, 4, 0)):
+        out = torch.empty(1500, 900, device="cuda")
+        blockscale._matmul(a, b, None, out, False, plan)
+        tol = matmul_bound(av, bv, 1300, want, torch.float32) if tol is None else tol
+        assert np.all(np.abs(f64(out) - want) <= tol)
+
+
+@pytest.mark.parametrize("plan", [1, 2, split_plan(128, 2, 0), split_plan(32, 1, 1)])
+def test_codes_past_the_last_column_do_not_count(plan):
+    """The bytes between a row's last code and its pitch, and the scales of rows and blocks past the end, hold NaN."""
+    from apa import blockscale
+    m, n, k = 30, 200, 1157
+    A, B, want = exact_operands(m, n, k, 3)
+    for t in (A, B):
+        full = t.data.as_strided((t.shape[0], t.data.stride(0)), (t.data.stride(0), 1)).view(torch.uint8)
+        full[:, k:] = 0x7F
+        rp, kb = (t.shape[0] + 127) // 128 * 128, (k + 127) // 128
+        v = t.scales.view((kb + 3) // 4, rp // 128, 32, 4, 4)
+        live = torch.zeros(rp, (kb + 3) // 4 * 4, dtype=torch.bool, device="cuda")
+        live[:t.shape[0], :kb] = True
+        v[~live.view(rp // 128, 4, 32, -1, 4).permute(3, 0, 2, 1, 4)] = 0xFF
+    out = torch.empty(m, n, device="cuda")
+    blockscale._matmul(A, B, None, out, False, plan)
+    assert torch.equal(out, want.float())
