@@ -59,7 +59,9 @@ SIGNATURES = {
     "apa_block_cast": [_VP, _I, _I64, _I64, _I64, _VP, _VP, _I, _I, _VP, _I64, _VP, _VP, _I64, _VP, _VP, _VP],
     "apa_block_dequant": [_VP, _I64, _VP, _I64, _I64, _VP, _I, _I64, _VP],
     "apa_block_colsum": [_VP, _I64, _I64, _VP, _I, _VP],
-    "apa_block_gemm": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _I, _I, _VP],
+    "apa_block_gemm": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _I, _I, _VP,
+                       _I64, _VP],
+    "apa_block_gemm_workspace": [_I64, _I64, _I64, _I, _I, _VP],
     "apa_rmsnorm_fwd": [_VP, _I64, _VP, _I64, _VP, _I, _I, _I64, _I64, _F, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP,
                         _VP],
     "apa_rmsnorm_bwd_workspace": [_I64, _I64, _VP],

@@ -36,6 +36,7 @@ not affect the scale.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -239,11 +240,24 @@ def block_cast(x: torch.Tensor, form: str = "rows", square: bool = False):
     return (q, qt) if form == "both" else q if form == "rows" else qt
 
 
+@functools.lru_cache(maxsize=1024)
+def _matmul_workspace(M: int, N: int, K: int, dtype: int, plan: int, device: int) -> int:
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().apa_block_gemm_workspace(M, N, K, dtype, plan, ctypes.addressof(n)),
+                   "apa_block_gemm_workspace")
+    return n.value
+
+
 def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool, plan: int = 0) -> None:
     M, K = a.shape
+    N = b.shape[0]
+    dt = _REAL[out.dtype]
+    n = _matmul_workspace(M, N, K, dt, plan, a.device.index)
+    ws = torch.empty(n, dtype=torch.uint8, device=a.device) if n else None
     _call(a.device, "apa_block_gemm", a.data.data_ptr(), _pitch(a), a.scales.data_ptr(), b.data.data_ptr(), _pitch(b),
-          b.scales.data_ptr(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, out.data_ptr(),
-          _REAL[out.dtype], _ld(out), M, b.shape[0], K, int(accumulate), plan, _lib.stream_handle(a.device))
+          b.scales.data_ptr(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, out.data_ptr(), dt,
+          _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n, _lib.stream_handle(a.device))
 
 
 def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,

@@ -27,7 +27,7 @@
 //   overlap by 16 columns: the next tile's MMAs start as soon as the epilogue
 //   has read the shared columns, which it reads first.
 #include <cuda.h>
-#include <mutex>
+#include <cmath>
 #include "block_scale.cuh"
 #include "tcgen05.cuh"
 
@@ -85,6 +85,10 @@ __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint3
 // apart) to four tensor-memory columns, repeated in every lane quarter.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* tm) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
 }
 
 template <bool PAIR>
@@ -148,9 +152,9 @@ template <int BN> struct SplitCfg {
   static constexpr int kBBytes = BN * kSlab;
   static constexpr int kScaleBytes = 1024;          // 512 of A, 512 of B
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // two CTAs per SM (one loads while the other finishes)
-  static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : 5;
-  static constexpr int kTmemCols = BN == 128 ? 256 : BN == 64 ? 128 : BN == 32 ? 64 : 32;
+  // two CTAs per SM: one loads while the other finishes
+  static constexpr int kStages = BN == 64 ? 4 : 5;
+  static constexpr int kTmemCols = BN == 64 ? 128 : BN == 32 ? 64 : 32;
   static constexpr int kSmemBytes = kStages * (kStageBytes + kScaleBytes) + 1024 + 256;
   static constexpr int kThreads = 192;
   static_assert((BN + 4) * BM * 4 <= kStages * kStageBytes, "the tile reuses the stages");
@@ -203,6 +207,12 @@ __global__ void __launch_bounds__(192, 2)
                  "r"((uint32_t)C::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 32 * 2) {
+    prefetch_map(&tmA);
+    prefetch_map(&tmB);
+    prefetch_map(&tmSA);
+    prefetch_map(&tmSB);
   }
   fence_before();
   __syncthreads();
@@ -348,34 +358,90 @@ __global__ void __launch_bounds__(192, 2)
 // ---------------------------------------------------------------------------
 // pair_kernel
 // ---------------------------------------------------------------------------
+// Arrive on a barrier of either CTA of the pair. CTA scope: what is handed
+// over is tensor memory, ordered by the tcgen05 fences on both sides; a
+// cluster-scope release would flush this thread's ordinary stores first, in
+// the path between two tiles.
+__device__ __forceinline__ void arrive_peer(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 constexpr int kEpiBox = 4096;      // one staging buffer: 32 rows x 128 bytes
-constexpr int kAccStride = 240;    // second accumulator: columns 240 .. 495
-constexpr int kPairSfa = 496, kPairSfb = 500;   // 4 columns of A's scales, 8 of B's
+constexpr int kAccStride = 232;    // second accumulator: columns 232 .. 487
+// two sets of scales, used in turn, so that copying the next one does not wait
+// for the MMAs that still read the last: 4 columns of A's and 8 of B's each
+constexpr int kPairScales = 488, kScaleSet = 12;
 
 template <int EW> struct PairCfg {
   static constexpr int kTile = 256;
   static constexpr int kHalfBytes = BM * kSlab;                 // this CTA's rows of A, and of B
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kScaleBytes = 512 + 1024;                // own 128 rows of A, all 256 of B
-  static constexpr int kStages = EW == 4 ? 6 : 5;
+  static constexpr int kBoxes = EW == 4 ? 1 : 2;                // staging buffers per epilogue warp
+  static constexpr int kStages = EW == 4 ? 6 : 4;
   static constexpr int kWarpCols = 1024 / EW;                   // columns per epilogue warp
   static constexpr int kUnits = kWarpCols / 64;
   static constexpr int kThreads = 64 + 32 * EW;
   static constexpr int kSmemBytes =
-      kStages * (kStageBytes + kScaleBytes) + EW * (kEpiBox + kWarpCols * 4) + 256 + 1024;
+      kStages * (kStageBytes + kScaleBytes) + EW * (kBoxes * kEpiBox + kWarpCols * 4) + 256 + 1024;
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
 struct PairArgs {
   int kb_count;
-  int tma_out;          // out written by TMA stores (aligned, not accumulated)
+  int splits;           // the reduction is split over this many units per tile
+  int slice_rows;       // rows of one split's slice of the workspace (out is the workspace when splits > 1)
+  int chunk;            // slabs accumulated at once; later chunks are added to out
+  int tma_out;          // out written by TMA stores (or reductions)
   OutArgs o;
 };
 
+// One pass of the persistent schedule: slabs kb0 .. kb1 of an output tile.
+// Units (tile, split) go round the CTA pairs; a unit's chunks follow each
+// other on the same pair.
+struct Pass {
+  int unit, tile, split, first, kb0, kb1, end;
+};
+
+__device__ __forceinline__ void pass_unit(const PairArgs& p, int unit, Pass& a) {
+  a.unit = a.tile = unit;
+  a.split = 0;
+  a.first = 0;
+  a.end = p.kb_count;
+  if (p.splits > 1) {
+    // kb_count < 2^24 and splits < 2^7: 32 bits hold the products
+    a.tile = unit / p.splits;
+    a.split = unit - a.tile * p.splits;
+    a.first = (int)((uint32_t)p.kb_count * (uint32_t)a.split / (uint32_t)p.splits);
+    a.end = (int)((uint32_t)p.kb_count * (uint32_t)(a.split + 1) / (uint32_t)p.splits);
+  }
+  a.kb0 = a.first;
+  a.kb1 = min(a.kb0 + p.chunk, a.end);
+}
+
+__device__ __forceinline__ void pass_next(const PairArgs& p, int step, Pass& a) {
+  if (a.kb1 < a.end) {
+    a.kb0 = a.kb1;
+    a.kb1 = min(a.kb0 + p.chunk, a.end);
+  } else {
+    pass_unit(p, a.unit + step, a);
+  }
+}
+
+// A staged fp32 box added to out. Each element of out is added to by one warp,
+// in its program order, so the result does not depend on timing.
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* tm, const void* src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tm)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
 // A staged box (32 rows of 128 bytes, 128-byte swizzle) to rows that TMA
-// cannot store to (unaligned, a ragged last 16 bytes, or accumulated): one row
-// per step, one 4-byte word per lane, so a warp's store covers whole lines.
-__device__ __forceinline__ void put_box(const OutArgs& o, const uint8_t* box, int lane, int row0, int col0) {
+// cannot store to (unaligned, or a ragged last 16 bytes): one row per step,
+// one 4-byte word per lane, so a warp's store covers whole lines.
+__device__ __forceinline__ void put_box(const OutArgs& o, const uint8_t* box, int lane, int row0, int col0,
+                                        bool add) {
   const bool out16 = o.out_dt != APA_DT_F32;
   const int rows = min(32, o.M - row0);
   const int col = col0 + (out16 ? 2 * lane : lane);
@@ -394,7 +460,7 @@ __device__ __forceinline__ void put_box(const OutArgs& o, const uint8_t* box, in
       }
     } else if (col < o.N) {
       float* d = static_cast<float*>(o.out) + at;
-      *d = o.accumulate ? *d + fu(w) : fu(w);
+      *d = add ? *d + fu(w) : fu(w);
     }
   }
 }
@@ -412,7 +478,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
   uint8_t* smA = smem;
   uint8_t* smB = smem + kStages * C::kHalfBytes;
   uint8_t* smE = smem + kStages * C::kStageBytes;                         // staging boxes, 128-byte swizzled
-  uint8_t* smS = smE + EW * kEpiBox;
+  uint8_t* smS = smE + EW * C::kBoxes * kEpiBox;
   float* smBias = reinterpret_cast<float*>(smS + kStages * C::kScaleBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(smBias + EW * C::kWarpCols);
   uint64_t* empty = full + kStages;
@@ -423,7 +489,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = gemm::cluster_rank();
   const int num_m = (p.o.M + 255) / 256, num_n = (p.o.N + 255) / 256;
-  const int tiles = num_m * num_n;
+  const int units = num_m * num_n * p.splits;
   const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
   constexpr int kGroup = gemm::kGroupM / 2;
 
@@ -445,6 +511,13 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  if (threadIdx.x == 32 * 2) {
+    prefetch_map(&tmA);
+    prefetch_map(&tmB);
+    prefetch_map(&tmSA);
+    prefetch_map(&tmSB);
+    if (p.tma_out) prefetch_map(&tmO);
+  }
   fence_before();
   gemm::cluster_sync();
   fence_after();
@@ -456,13 +529,14 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = first; ok && t < tiles; t += step) {
+      Pass a;
+      for (pass_unit(p, first, a); ok && a.unit < units; pass_next(p, step, a)) {
         int mb, nb;
-        gemm::tile_coords(t, num_m, num_n, kGroup, mb, nb);
+        gemm::tile_coords(a.tile, num_m, num_n, kGroup, mb, nb);
         const int a_row = mb * 256 + (int)rank * BM, b_row = nb * 256 + (int)rank * BM;
-        for (int kb = 0; kb < p.kb_count; ++kb) {
+        for (int kb = a.kb0; kb < a.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty)) { ok = false; break; }
-          const bool scales = (kb & 3) == 0;
+          const bool scales = kb == a.kb0 || (kb & 3) == 0;
           // the even CTA's barrier expects both CTAs' bytes
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * (C::kStageBytes + (scales ? C::kScaleBytes : 0)));
           const uint32_t bar = gemm::map_to_cta(&full[stage], 0);
@@ -488,29 +562,33 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint32_t sfa = tmem + kPairSfa, sfb = tmem + kPairSfb;
-      for (int t = first; ok && t < tiles; t += step, ++local) {
+      uint32_t set = 0;
+      Pass a;
+      for (pass_unit(p, first, a); ok && a.unit < units; pass_next(p, step, a), ++local) {
         const int acc = local & 1;
-        if (!mbar_wait<true>(&tempty[acc], ((uint32_t)(local >> 1) & 1u) ^ 1u, kStatusTimeoutAcc)) { ok = false; break; }
+        if (!mbar_wait(&tempty[acc], ((uint32_t)(local >> 1) & 1u) ^ 1u, kStatusTimeoutAcc)) { ok = false; break; }
         // the previous tile's shared columns
-        if (local > 0 && !mbar_wait<true>(tshared, (uint32_t)(local - 1) & 1u, kStatusTimeoutAcc)) { ok = false; break; }
+        if (local > 0 && !mbar_wait(tshared, (uint32_t)(local - 1) & 1u, kStatusTimeoutAcc)) { ok = false; break; }
         fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * kAccStride);
-        for (int kb = 0; kb < p.kb_count; ++kb) {
+        for (int kb = a.kb0; kb < a.kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, kStatusTimeoutFull)) { ok = false; break; }
           fence_after();
           const uint32_t j = (uint32_t)(kb & 3);
-          if (j == 0) {
+          const bool scales = kb == a.kb0 || j == 0;
+          if (scales) set ^= 1u;
+          const uint32_t sfa = tmem + kPairScales + set * kScaleSet, sfb = sfa + 4;
+          if (scales) {
             const uint32_t s = smem_u32(smS + stage * C::kScaleBytes);
             scale_copy<true>(sfa, s);
             scale_copy<true>(sfb, s + 512);
             scale_copy<true>(sfb + 4, s + 1024);
           }
           const uint32_t id = mx_idesc<256, 256>() | (j << 4) | (j << 29);
-          const uint32_t a = smem_u32(smA + stage * C::kHalfBytes), b = smem_u32(smB + stage * C::kHalfBytes);
+          const uint32_t sa = smem_u32(smA + stage * C::kHalfBytes), sb = smem_u32(smB + stage * C::kHalfBytes);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mx_mma<true>(d, sdesc(a + 32 * k), sdesc(b + 32 * k), id, sfa, sfb, (kb != 0 || k != 0) ? 1u : 0u);
+            mx_mma<true>(d, sdesc(sa + 32 * k), sdesc(sb + 32 * k), id, sfa, sfb, (kb != a.kb0 || k != 0) ? 1u : 0u);
           gemm::mma_commit<true>(&empty[stage]);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
@@ -520,25 +598,31 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
     __syncwarp();
   } else {
     const int q = warp & 3, e = warp - 2, part = e >> 2;
-    uint8_t* box = smE + e * kEpiBox;
+    uint8_t* boxes = smE + e * C::kBoxes * kEpiBox;
     float* sb = smBias + e * C::kWarpCols;
     const bool out16 = p.o.out_dt != APA_DT_F32;
     int local = 0;
-    bool pending = false;                 // a TMA store of this warp may still read its box
+    int slot = 0, inflight = 0;           // staging ring; TMA stores that may still read their box
     const uint32_t te0 = gemm::map_to_cta(&tempty[0], 0), te1 = gemm::map_to_cta(&tempty[1], 0);
     const uint32_t ts = gemm::map_to_cta(tshared, 0);
     auto arrive = [&](uint32_t bar) {
       fence_before();
       __syncwarp();
-      if (lane == 0) gemm::mbar_arrive_cluster(bar);
+      if (lane == 0) arrive_peer(bar);
     };
-    for (int t = first; t < tiles; t += step, ++local) {
+    Pass a;
+    for (pass_unit(p, first, a); a.unit < units; pass_next(p, step, a), ++local) {
       int mb, nb;
-      gemm::tile_coords(t, num_m, num_n, kGroup, mb, nb);
+      gemm::tile_coords(a.tile, num_m, num_n, kGroup, mb, nb);
       const int acc = local & 1;
       const int row0 = mb * 256 + (int)rank * BM + q * 32;
+      const int orow = row0 + a.split * p.slice_rows;
       const int col_base = nb * 256 + part * C::kWarpCols;
-      if (p.o.bias != nullptr) {
+      // a unit's later chunks, and all of an accumulating product, are added to out
+      const bool later = a.kb0 != a.first;
+      const bool add = later || p.o.accumulate;
+      const bool bias = p.o.bias != nullptr && !later;
+      if (bias) {
         __syncwarp();
         for (int c = lane; c < C::kWarpCols; c += 32)
           sb[c] = col_base + c < p.o.N ? to_f32(p.o.bias, p.o.bias_dt, col_base + c) : 0.0f;
@@ -549,6 +633,13 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       ready = __shfl_sync(0xFFFFFFFFu, ready ? 1 : 0, 0) != 0;
       if (!ready) break;
       fence_after();
+      if (later && inflight > 0) {
+        // the earlier chunk's stores must have landed, not just left
+        if (lane == 0) gemm::bulk_wait_all();
+        __syncwarp();
+        inflight = 0;
+        slot = 0;
+      }
       const uint32_t tb = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kAccStride + part * C::kWarpCols);
       // the columns the two accumulators share are the last of the first one
       // and the first of the second: those go first
@@ -564,7 +655,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
         if (i == 0 && part == shared_part) arrive(ts);
         if (i == C::kUnits - 1) arrive(acc ? te1 : te0);
         if (col0 >= p.o.N || row0 >= p.o.M) continue;      // warp-uniform
-        if (p.o.bias != nullptr) {
+        if (bias) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float4 b = reinterpret_cast<const float4*>(sb + u * 64)[c];
@@ -585,25 +676,31 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
         for (int b = 0; b < 2; ++b) {
           const int x = col0 + 32 * b;
           if ((out16 && b == 1) || x >= p.o.N) break;
-          if (pending && lane == 0) gemm::bulk_wait_read<0>();
+          uint8_t* box = boxes + slot * kEpiBox;
+          if (inflight == C::kBoxes) {
+            if (lane == 0) gemm::bulk_wait_read<C::kBoxes - 1>();
+            --inflight;
+          }
           __syncwarp();
           gemm::stage_row(box, lane, r + 32 * b);
           if (p.tma_out) {
             gemm::fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              gemm::tma_store_2d(&tmO, box, x, row0);
+              if (add) tma_add_2d(&tmO, box, x, orow);
+              else gemm::tma_store_2d(&tmO, box, x, orow);
               gemm::bulk_commit();
             }
-            pending = true;
+            ++inflight;
+            slot = slot + 1 == C::kBoxes ? 0 : slot + 1;
           } else {
             __syncwarp();
-            put_box(p.o, box, lane, row0, x);
+            put_box(p.o, box, lane, row0, x, add);
           }
         }
       }
     }
-    if (pending && lane == 0) gemm::bulk_wait_all();
+    if (inflight > 0 && lane == 0) gemm::bulk_wait_all();
     __syncwarp();
   }
 
@@ -686,14 +783,14 @@ int launch_split(const Operand& A, const Operand& B, int64_t K, const OutArgs& o
 }
 
 // Output: dims {N, M}, box {128 bytes, 32 rows}, 128-byte swizzle.
-int out_map(CUtensorMap* tm, const OutArgs& o) {
+int out_map(CUtensorMap* tm, const OutArgs& o, int64_t rows) {
   gemm::EncodeFn enc = gemm::get_encode();
   if (!enc) return APA_ERR_CUDA;
   const int es = elem_bytes(o.out_dt);
   const CUtensorMapDataType dt = o.out_dt == APA_DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : o.out_dt == APA_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  cuuint64_t dims[2] = {(cuuint64_t)o.N, (cuuint64_t)o.M};
+  cuuint64_t dims[2] = {(cuuint64_t)o.N, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)(o.ldo * es)};
   cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
   cuuint32_t one[2] = {1, 1};
@@ -735,8 +832,46 @@ int pair_slots() {
   return n;
 }
 
+// The slices of a split product: fp32, rows padded to whole tiles (a store's
+// box never reaches into the next slice), columns to 16 bytes.
+int64_t slice_rows(int64_t M) { return cdiv64(M, 256) * 256; }
+int64_t slice_ld(int64_t N) { return (N + 3) / 4 * 4; }
+int64_t split_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? splits * slice_rows(M) * slice_ld(N) * 4 : 0; }
+
+struct SumArgs { const float* ws; int64_t slice, ld; int splits; OutArgs o; };
+
+// Adds the slices in order, then bias, accumulation and rounding.
+__global__ void __launch_bounds__(256) block_sum_kernel(SumArgs p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int per = (int)(p.ld / 4);
+  const int64_t total = (int64_t)p.o.M * per;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+    const int m = (int)(e / per), n = (int)(e - (int64_t)m * per) * 4;
+    const float4* at = reinterpret_cast<const float4*>(p.ws + (int64_t)m * p.ld + n);
+    float4 x = __ldcg(at);
+    for (int s = 1; s < p.splits; s += 4) {
+      float4 y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s + k < p.splits) y[k] = __ldcg(at + (int64_t)(s + k) * p.slice / 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (s + k < p.splits) { x.x += y[k].x; x.y += y[k].y; x.z += y[k].z; x.w += y[k].w; }
+    }
+    put4(p.o, m, n, x);
+  }
+}
+
+// Slabs accumulated at once for an fp32 output. The tensor core drops the bits
+// that the running sum cannot hold instead of rounding them, so the error grows
+// with the length of the chain (measured against 64 bits: 5e-7 of the result
+// after 8192 columns, 3e-6 after 32768, where rounded chunks stay below 5e-7).
+// A 16-bit output's own rounding is a thousand times that.
+constexpr int kChunkSlabs = 64;
+
 template <int EW>
-int launch_pair(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, cudaStream_t s) {
+int launch_pair(const Operand& A, const Operand& B, int64_t K, OutArgs o, int splits, void* ws, cudaStream_t s) {
   using C = PairCfg<EW>;
   int slots = pair_slots<EW>();
   if (slots < 1) return APA_ERR_UNSUPPORTED;
@@ -747,85 +882,174 @@ int launch_pair(const Operand& A, const Operand& B, int64_t K, const OutArgs& o,
   if (int st = code_map(&tb, B.q, B.rows, K, B.ld, BM)) return st;
   if (int st = scale_map(&tsa, A.sc, A.rows, kb, 128)) return st;
   if (int st = scale_map(&tsb, B.sc, B.rows, kb, 256)) return st;
+  const OutArgs final = o;
   PairArgs p;
-  p.kb_count = (int)kb; p.o = o;
+  p.kb_count = (int)kb; p.splits = splits; p.slice_rows = 0;
+  int64_t out_rows = o.M;
+  if (splits > 1) {
+    p.slice_rows = (int)slice_rows(o.M);
+    out_rows = p.slice_rows * (int64_t)splits;
+    o.out = ws; o.ldo = slice_ld(o.N); o.out_dt = APA_DT_F32; o.bias = nullptr; o.accumulate = 0; o.vec = 1;
+    o.N = (int)o.ldo;
+  }
+  // only an fp32 output can be added to
+  p.chunk = o.out_dt == APA_DT_F32 ? kChunkSlabs : (int)kb;
+  p.o = o;
   // a TMA store writes whole 16-byte pieces, past N too where N ends inside one
-  p.tma_out = o.vec && !o.accumulate && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0;
+  p.tma_out = o.vec && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0;
   to = ta;
   if (p.tma_out)
-    if (int st = out_map(&to, o)) return st;
-  const int64_t tiles = cdiv64(o.M, 256) * cdiv64(o.N, 256);
-  const int grid = 2 * (int)std::min<int64_t>(tiles, slots);
-  return launch_kernel(pair_kernel<EW>, dim3(grid), dim3(C::kThreads), C::kSmemBytes, s, 2, ta, tb, tsa, tsb, to, p) ==
-                 cudaSuccess ? APA_OK : APA_ERR_CUDA;
+    if (int st = out_map(&to, o, out_rows)) return st;
+  const int64_t units = cdiv64(o.M, 256) * cdiv64(o.N, 256) * splits;
+  if (units > (1ll << 31) - 1 - 2 * num_sms()) return APA_ERR_INVALID;
+  const int grid = 2 * (int)std::min<int64_t>(units, slots);
+  if (launch_kernel(pair_kernel<EW>, dim3(grid), dim3(C::kThreads), C::kSmemBytes, s, 2, ta, tb, tsa, tsb, to, p) !=
+      cudaSuccess)
+    return APA_ERR_CUDA;
+  if (splits > 1) {
+    SumArgs q{static_cast<const float*>(ws), p.slice_rows * o.ldo, o.ldo, splits, final};
+    const int64_t blocks = cdiv64(final.M * (o.ldo / 4), 256);
+    if (launch_kernel(block_sum_kernel, dim3((unsigned)std::min<int64_t>(blocks, 8 * num_sms())), dim3(256), 0, s, 1,
+                      q) != cudaSuccess)
+      return APA_ERR_CUDA;
+  }
+  return APA_OK;
 }
 
 // kind 0: split_kernel with `bn`, `split` and `swap`; 1: pair_kernel with `ew`
-// epilogue warps.
-struct BlockPlan { int kind, bn, split, swap, ew; int64_t rows_m; };
+// epilogue warps and `split` units per tile.
+struct BlockPlan { int kind, bn, split, swap, ew; };
 
-BlockPlan block_plan(int64_t M, int64_t N, int64_t K) {
-  BlockPlan p{0, 128, 1, 0, 4, M};
+// The faster of both kernels by a model fitted to timings on a B200 (us, back
+// to back). A 128 x 64 tile costs 5.3 + 0.36 per slab in each round of two
+// CTAs per SM, and its cluster 0.9, or 2.2 for eight CTAs on more than one
+// CTA per SM; clusters of four and eight leave an eighth of the slots empty.
+// A 256 x 256 tile costs 0.8 + 0.44 per slab in each wave of CTA pairs, after
+// 3 to start; the slices of a split product 3 for the second kernel and their
+// bytes at 12 TB/s (they stay in L2). Rows that TMA cannot store to cost the
+// pair 3.5 per wave. Both sides of the choice: 512 x 1024 x 4096 9.1 on tiles
+// of 64 (split 4), 11.7 on pairs; 512 x 1536 x 33280 44.7 (split 4 of 128 x 128
+// tiles) and 30.7.
+BlockPlan block_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
   const int64_t kb = cdiv64(K, kSlab);
-  p.swap = M <= 128 && M < N;
-  const int64_t small = p.swap ? M : N, big = p.swap ? N : M;
-  p.bn = small <= 16 ? 16 : small <= 32 ? 32 : small <= 64 ? 64 : 128;
-  const int64_t tiles = cdiv64(big, BM) * cdiv64(small, p.bn);
-  while (p.split < 8 && tiles * p.split * 2 <= 2 * num_sms() && p.split * 2 * 2 <= kb) p.split *= 2;
+  const int64_t small = std::min(M, N), big = std::max(M, N);
+  const double sms = g_gemm_sm_limit > 0 ? g_gemm_sm_limit : num_sms();
+  BlockPlan best{0, 0, 1, M <= N ? 1 : 0, 8};
+  best.bn = small <= 16 ? 16 : small <= 32 ? 32 : 64;
+  const int64_t tiles = cdiv64(big, BM) * cdiv64(small, best.bn);
+  double cost = 1e30;
+  for (int split = 1; split <= 8 && split <= kb; split *= 2) {
+    const int64_t ctas = tiles * split;
+    const double rounds = std::ceil((double)ctas / ((split > 2 ? 1.75 : 2.0) * num_sms()));
+    const double share = split == 1 ? 0.0 : split == 8 && ctas > num_sms() ? 2.2 : 0.9;
+    const double t = rounds * (5.3 + 0.36 * (double)cdiv64(kb, split) + share);
+    if (t < cost) { cost = t; best.split = split; }
+  }
   const int64_t pt = cdiv64(M, 256) * cdiv64(N, 256);
-  if (pt >= 64) p.kind = 1;
-  return p;
+  const int64_t pairs = std::max<int64_t>(1, (int64_t)(sms / 2));
+  for (int split = 1; split <= 64 && split <= kb; ++split) {
+    // a split pays where units would leave pairs idle, in whole waves
+    if (split > 1 && pt * split > 2 * pairs) break;
+    const double waves = (double)cdiv64(pt * split, pairs);
+    const int64_t slabs = cdiv64(kb, split);
+    double t = 3.0 + waves * (0.8 + 0.44 * (double)slabs + (aligned || split > 1 ? 0.0 : 3.5));
+    if (split > 1) t += 3.0 + 8.0 * (double)split * (double)M * (double)N / 12e6;
+    if (t < cost) {
+      cost = t;
+      // eight warps where the epilogue is exposed (one wave, few slabs, slow
+      // stores), else four and a deeper ring: 8192 x 4096 x 4096 107 against
+      // 111 us, 33280 x 1536 x 512 37 against 33
+      best = BlockPlan{1, 0, split, 0, slabs < 8 || waves <= 1.0 || !aligned ? 8 : 4};
+    }
+  }
+  return best;
 }
 
 // A caller's choice (APA_BLOCK_*): the automatic plan stands where it is 0.
-int force_plan(int code, int64_t N, int64_t K, BlockPlan* p) {
+int force_plan(int code, int64_t M, int64_t N, int64_t K, BlockPlan* p) {
   if (code == APA_BLOCK_AUTO) return APA_OK;
-  if (code == APA_BLOCK_PAIR_4 || code == APA_BLOCK_PAIR_8) {
+  const int bn = code & 0x7F, split = (code >> 7) & 0x7F, swap = (code >> 14) & 1, ew = (code >> 15) & 0xF;
+  if (code < 0 || (code >> 19) != 0 || split < 1 || split > cdiv64(K, kSlab)) return APA_ERR_INVALID;   // no unit without a slab
+  if (bn == 0) {
+    if ((ew != 4 && ew != 8) || swap) return APA_ERR_INVALID;
     p->kind = 1;
-    p->ew = code == APA_BLOCK_PAIR_4 ? 4 : 8;
-    return APA_OK;
+  } else {
+    if ((bn != 16 && bn != 32 && bn != 64) || split > 8 || ew != 0) return APA_ERR_INVALID;
+    // the MMA takes scales from even columns of tensor memory only, 64 rows
+    // apart: narrower tiles are for a side of one tile
+    if (bn < 64 && (swap ? M : N) > bn) return APA_ERR_INVALID;
+    p->kind = 0;
   }
-  const int bn = code & 0xFF, split = (code >> 8) & 0xFF, swap = (code >> 16) & 1;
-  if ((code >> 17) != 0 || (bn != 16 && bn != 32 && bn != 64 && bn != 128)) return APA_ERR_INVALID;
-  if (split != 1 && split != 2 && split != 4 && split != 8) return APA_ERR_INVALID;
-  if (split > cdiv64(K, kSlab)) return APA_ERR_INVALID;       // no CTA without a slab
-  p->kind = 0;
-  p->bn = bn; p->split = split; p->swap = swap;
-  // the MMA takes scales from even columns of tensor memory only, 64 rows
-  // apart: narrower tiles are for a side of one tile
-  return bn < 64 && (swap ? p->rows_m : N) > bn ? APA_ERR_INVALID : APA_OK;
+  p->bn = bn; p->split = split; p->swap = swap; p->ew = ew;
+  return APA_OK;
 }
 
-int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, const BlockPlan& p, cudaStream_t s) {
-  if (p.kind == 1) return p.ew == 8 ? launch_pair<8>(A, B, K, o, s) : launch_pair<4>(A, B, K, o, s);
+int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, const BlockPlan& p, void* ws,
+               cudaStream_t s) {
+  if (p.kind == 1)
+    return p.ew == 8 ? launch_pair<8>(A, B, K, o, p.split, ws, s) : launch_pair<4>(A, B, K, o, p.split, ws, s);
   const Operand& x = p.swap ? B : A;
   const Operand& y = p.swap ? A : B;
   switch (p.bn) {
     case 16: return launch_split<16>(x, y, K, o, p.swap, p.split, s);
     case 32: return launch_split<32>(x, y, K, o, p.swap, p.split, s);
-    case 64: return launch_split<64>(x, y, K, o, p.swap, p.split, s);
-    default: return launch_split<128>(x, y, K, o, p.swap, p.split, s);
+    default: return launch_split<64>(x, y, K, o, p.swap, p.split, s);
   }
 }
 
 }  // namespace blk
 }  // namespace apa
 
+namespace {
+
+int gemm_dims(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return APA_ERR_INVALID;
+  const int64_t top = (1ll << 31) - 256;
+  return M > top || N > top || K > top ? APA_ERR_INVALID : APA_OK;
+}
+
+}  // namespace
+
+extern "C" int apa_block_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dtype, int plan, int64_t* bytes_out) {
+  using namespace apa::blk;
+  if (!bytes_out) return APA_ERR_INVALID;
+  if (int st = gemm_dims(M, N, K)) return st;
+  if (elem_bytes(out_dtype) == 0) return APA_ERR_UNSUPPORTED;
+  BlockPlan p{};
+  if (plan != APA_BLOCK_AUTO) {
+    if (int st = force_plan(plan, M, N, K, &p)) return st;
+  } else {
+    p = block_plan(M, N, K, (N * elem_bytes(out_dtype)) % 16 == 0);
+  }
+  *bytes_out = p.kind == 1 ? split_bytes(M, N, p.split) : 0;
+  return APA_OK;
+}
+
 extern "C" int apa_block_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
                               const void* b_scales, const void* bias, int bias_dtype, void* out, int out_dtype,
-                              int64_t ldo, int64_t M, int64_t N, int64_t K, int accumulate, int plan, void* stream) {
+                              int64_t ldo, int64_t M, int64_t N, int64_t K, int accumulate, int plan, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
   using namespace apa::blk;
-  if (M <= 0 || N <= 0 || K <= 0) return APA_ERR_INVALID;
-  if (M > (1ll << 31) - 256 || N > (1ll << 31) - 256 || K > (1ll << 31) - 256) return APA_ERR_INVALID;
+  if (int st = gemm_dims(M, N, K)) return st;
   if (!a || !a_scales || !b || !b_scales || !out || lda < K || ldb < K || ldo < N) return APA_ERR_INVALID;
   const int es = elem_bytes(out_dtype);
   if (es == 0 || (bias && elem_bytes(bias_dtype) == 0)) return APA_ERR_UNSUPPORTED;
   if (accumulate && out_dtype != APA_DT_F32) return APA_ERR_UNSUPPORTED;
   if (!vec16(a, lda, 1) || !vec16(b, ldb, 1)) return APA_ERR_ALIGN;
-  if (((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 15u) != 0) return APA_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+    return APA_ERR_ALIGN;
   OutArgs o{out, ldo, out_dtype, bias, bias_dtype, accumulate ? 1 : 0, vec16(out, ldo, es) ? 1 : 0, (int)M, (int)N};
   const Operand A{a, lda, a_scales, M}, B{b, ldb, b_scales, N};
-  BlockPlan p = block_plan(M, N, K);
-  if (int st = force_plan(plan, N, K, &p)) return st;
-  return block_gemm(A, B, K, o, p, static_cast<cudaStream_t>(stream));
+  BlockPlan p{};
+  if (plan != APA_BLOCK_AUTO) {
+    if (int st = force_plan(plan, M, N, K, &p)) return st;
+  } else {
+    p = block_plan(M, N, K, o.vec && (N * es) % 16 == 0);
+  }
+  if (p.kind == 1 && p.split > 1 && (!workspace || workspace_bytes < split_bytes(M, N, p.split))) {
+    if (plan != APA_BLOCK_AUTO) return APA_ERR_INVALID;
+    p.split = 1;      // without room for the slices: one unit per tile
+  }
+  return block_gemm(A, B, K, o, p, workspace, static_cast<cudaStream_t>(stream));
 }

@@ -73,13 +73,17 @@ template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned int why) {
   if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
-  while (!mbar_try_wait<CLUSTER>(bar, parity)) {
+  // the clock is read once per 64 tries: reading it takes longer than a try,
+  // and a phase that completes meanwhile would be seen that much later
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait<CLUSTER>(bar, parity)) return true;
     if (global_ns() - t0 > kWaitLimitNs) {
       atomicOr(&g_status, why);
       return false;
     }
   }
-  return true;
 }
 
 // --- cluster (CTA pair) helpers ---

@@ -413,20 +413,26 @@ int apa_block_colsum(const float* partial, int64_t parts, int64_t cols, void* ou
  * out[M, N] = a[M, K] . b[N, K]^T + bias[N] for block tensors a and b,
  * accumulated in fp32, rounded once to out_dtype (F32, F16, BF16). bias
  * (nullable): F32, F16 or BF16. accumulate != 0 (F32 only): add to out.
- * Deterministic; no workspace. plan: APA_BLOCK_AUTO picks the kernel by a
- * model of both; the others force one, to time and test it: the 256 x 256 CTA
- * pair with 4 or 8 epilogue warps, or APA_BLOCK_SPLIT(bn, split, swap), the
- * 128 x bn tile (bn 16, 32, 64 or 128; 16 and 32 only where that side has at
- * most bn rows) whose reduction is split over 1, 2, 4 or 8 CTAs (at most one per 128
- * columns of K), with b on the 128 side when swap is 1.
+ * Deterministic. workspace (nullable, 16-byte aligned): used only during the
+ * call, apa_block_gemm_workspace bytes of it let a long reduction over a small
+ * output be split over more SMs (fp32 slices, added in order). plan:
+ * APA_BLOCK_AUTO picks the kernel by a model of both; the others force one, to
+ * time and test it: APA_BLOCK_PAIR(ew, split), 256 x 256 tiles on CTA pairs
+ * with ew (4 or 8) epilogue warps and split (1 to 127) units per tile, or
+ * APA_BLOCK_SPLIT(bn, split, swap), 128 x bn tiles (bn 16, 32 or 64; 16 and 32
+ * only where that side has at most bn rows) whose reduction is split over 1 to
+ * 8 CTAs of a cluster, with b on the 128 side when swap is 1. split is at most
+ * the number of 128-column slabs of K; a forced plan without its workspace is
+ * refused.
  */
 #define APA_BLOCK_AUTO 0
-#define APA_BLOCK_PAIR_4 1
-#define APA_BLOCK_PAIR_8 2
-#define APA_BLOCK_SPLIT(bn, split, swap) ((bn) | (split) << 8 | (swap) << 16)
+#define APA_BLOCK_SPLIT(bn, split, swap) ((bn) | (split) << 7 | (swap) << 14)
+#define APA_BLOCK_PAIR(ew, split) ((split) << 7 | (ew) << 15)
+int apa_block_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dtype, int plan, int64_t* bytes_out);
 int apa_block_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb,
                    const void* b_scales, const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo,
-                   int64_t M, int64_t N, int64_t K, int accumulate, int plan, void* stream);
+                   int64_t M, int64_t N, int64_t K, int accumulate, int plan, void* workspace,
+                   int64_t workspace_bytes, void* stream);
 
 /*
  * Root-mean-square norm: r = x + residual rounded to dtype and stored in

@@ -104,16 +104,35 @@ def test_entry_points_check_their_arguments():
     assert cast(dt=3) == U and cast(rm=16, cm=16, cmd=3) == U
     assert cast(dst=17) == A and cast(ldd=40) == A and cast(dt_=16, ldt=8, sct=16) == A
 
-    def gemm(a=16, lda=32, sa=16, b=16, ldb=32, sb=16, bias=None, bd=0, out=16, od=0, ldo=8, M=4, N=8, K=32, acc=0, plan=0):
-        return lib.apa_block_gemm(a, lda, sa, b, ldb, sb, bias, bd, out, od, ldo, M, N, K, acc, plan, None)
+    def gemm(a=16, lda=32, sa=16, b=16, ldb=32, sb=16, bias=None, bd=0, out=16, od=0, ldo=8, M=4, N=8, K=32, acc=0, plan=0, ws=None, wb=0):
+        return lib.apa_block_gemm(a, lda, sa, b, ldb, sb, bias, bd, out, od, ldo, M, N, K, acc, plan, ws, wb, None)
 
     assert gemm(a=None) == I and gemm(sa=None) == I and gemm(out=None) == I and gemm(M=0) == I and gemm(K=0) == I
     assert gemm(lda=16) == I and gemm(ldo=7) == I and gemm(N=1 << 31, ldo=1 << 31) == I
     assert gemm(od=3) == U and gemm(bias=16, bd=3) == U and gemm(od=1, acc=1) == U
-    assert gemm(plan=3) == I and gemm(plan=128) == I and gemm(plan=128 | 2 << 8) == I and gemm(plan=1 << 17) == I
+    def split(bn, n, swap=0):
+        return bn | n << 7 | swap << 14
+
+    def pair(ew, n):
+        return n << 7 | ew << 15
+
+    for bad in (-1, 1, 3, split(16, 0), split(48, 1), split(64, 2), pair(4, 0), pair(5, 1), pair(4, 2), pair(0, 1),
+                pair(4, 1) | 1 << 14, split(64, 1) | 4 << 15, 1 << 19 | pair(4, 1)):
+        assert gemm(plan=bad) == I, bad
+    assert gemm(plan=split(64, 9), K=4096, lda=4096, ldb=4096) == I
     # tiles of 16 and 32 rows only for a side of one tile
-    assert gemm(plan=16 | 1 << 8, N=17, ldo=17) == I and gemm(plan=32 | 1 << 8, N=33, ldo=33) == I
-    assert gemm(plan=16 | 1 << 8 | 1 << 16, M=17) == I and gemm(plan=32 | 1 << 8 | 1 << 16, M=33) == I
+    assert gemm(plan=split(16, 1), N=17, ldo=17) == I and gemm(plan=split(32, 1), N=33, ldo=33) == I
+    assert gemm(plan=split(16, 1, 1), M=17) == I and gemm(plan=split(32, 1, 1), M=33) == I
+    # a forced split needs its workspace
+    big = dict(K=4096, lda=4096, ldb=4096, plan=pair(4, 2))
+    assert gemm(**big) == I and gemm(**big, ws=16, wb=2 * 256 * 8 * 4 - 1) == I
+    n = ctypes.c_int64(0)
+    at = ctypes.addressof(n)
+    assert lib.apa_block_gemm_workspace(4, 8, 4096, 0, pair(4, 2), at) == _lib.OK and n.value == 2 * 256 * 8 * 4
+    assert lib.apa_block_gemm_workspace(4, 8, 4096, 0, pair(4, 2), None) == I
+    assert lib.apa_block_gemm_workspace(4, 0, 4096, 0, 0, at) == I
+    assert lib.apa_block_gemm_workspace(4, 8, 4096, 3, 0, at) == U
+    assert gemm(ws=8, wb=64) == A
     assert gemm(a=8) == A and gemm(ldb=40) == A and gemm(sb=8) == A
 
     def fwd(x=16, res=None, g=16, gd=0, dt=0, rows=2, cols=32, st=None, y=16, q=None, sc=None, ldq=32):

@@ -243,13 +243,14 @@ def test_graph_capture():
     assert not torch.equal(ref, y)
 
 
-# plans of apa_block_gemm: the CTA pair with 4 or 8 epilogue warps, and the
-# split tile (columns, CTAs per tile, swapped)
-PAIRS = {"pair4": 1, "pair8": 2}
+# plans of apa_block_gemm: CTA pairs (epilogue warps, units per tile), and
+# the split tile (columns, CTAs per tile, swapped)
+def pair_plan(ew, split=1):
+    return split << 7 | ew << 15
 
 
 def split_plan(bn, split, swap):
-    return bn | split << 8 | swap << 16
+    return bn | split << 7 | swap << 14
 
 
 def exact_operands(m, n, k, seed):
@@ -264,52 +265,52 @@ def exact_operands(m, n, k, seed):
     return A, B, want
 
 
-@pytest.mark.parametrize("plan", sorted(PAIRS))
+@pytest.mark.parametrize("ew", [4, 8])
 @pytest.mark.parametrize("m,n,k", [
     (256, 256, 128), (257, 1, 1), (1, 257, 600), (300, 500, 1000), (1023, 777, 520),
     (2560, 2560, 256),      # 100 tiles: more than one on some CTA pairs
     (5000, 2600, 384),      # 220 tiles: both accumulators of a pair reused
     (4096, 4096, 128)])     # 256 tiles of one slab: the epilogue is the bound
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_pair_plan_exact(plan, m, n, k, dtype):
+def test_pair_plan_exact(ew, m, n, k, dtype):
     from apa import blockscale
     A, B, want = exact_operands(m, n, k, m + n)
     out = torch.empty(m, n, dtype=dtype, device="cuda")
-    blockscale._matmul(A, B, None, out, False, PAIRS[plan])
+    blockscale._matmul(A, B, None, out, False, pair_plan(ew))
     assert torch.equal(out, want.to(dtype))
     bias = torch.randint(-9, 9, (n,), device="cuda").float()
-    blockscale._matmul(A, B, bias, out, False, PAIRS[plan])
+    blockscale._matmul(A, B, bias, out, False, pair_plan(ew))
     assert torch.equal(out, (want + bias.double()).to(dtype))
 
 
-@pytest.mark.parametrize("plan", [*sorted(PAIRS), split_plan(128, 1, 0), split_plan(128, 4, 0), split_plan(64, 2, 1)])
+@pytest.mark.parametrize("plan", [pair_plan(4), pair_plan(8), pair_plan(4, 3), pair_plan(8, 9), split_plan(64, 1, 0),
+                                  split_plan(64, 4, 0), split_plan(64, 2, 1)])
 @pytest.mark.parametrize("pitch,off", [(0, 0), (1, 0), (8, 4), (5, 3)])
 def test_plans_write_inside_their_output(plan, pitch, off):
     """Aligned and unaligned rows, overwrite and accumulate: the bytes around stay."""
     from apa import blockscale
     m, n, k = 700, 333, 1100
     A, B, want = exact_operands(m, n, k, 5)
-    code = PAIRS.get(plan, plan)
     for dtype in DTYPES:
         buf = torch.full((m + 2, n + pitch + off + 3), 3.0, dtype=dtype, device="cuda")
         out = buf[1:m + 1, off:off + n]
-        blockscale._matmul(A, B, None, out, False, code)
+        blockscale._matmul(A, B, None, out, False, plan)
         assert torch.equal(out, want.to(dtype))
         if dtype == torch.float32:
-            blockscale._matmul(A, B, None, out, True, code)
+            blockscale._matmul(A, B, None, out, True, plan)
             assert torch.equal(out, (2 * want).float())
         out.fill_(3.0)
         assert bool((buf == 3.0).all())
 
 
-@pytest.mark.parametrize("bn", [16, 32, 64, 128])
-@pytest.mark.parametrize("split", [1, 2, 4, 8])
+@pytest.mark.parametrize("bn", [16, 32, 64])
+@pytest.mark.parametrize("split", [1, 2, 3, 4, 6, 8])
 @pytest.mark.parametrize("swap", [0, 1])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_split_plan_exact(bn, split, swap, dtype):
     """Every tile width, split and orientation, over ragged sizes and uneven splits of the slabs."""
     from apa import blockscale
-    small = {16: 13, 32: 29, 64: 139, 128: 300}[bn]
+    small = {16: 13, 32: 29, 64: 139}[bn]
     for big, k in ((200, 1024), (129, 1157)):
         m, n = (small, big) if swap else (big, small)
         A, B, want = exact_operands(m, n, k, bn + split)
@@ -325,14 +326,14 @@ def test_plans_agree_on_real_data():
     b = block_cast(rnd((900, 1300), 2).cuda(), square=True)
     av, bv = f64(a.dequantize()), f64(b.dequantize())
     want, tol = av @ bv.T, None
-    for plan in (1, 2, split_plan(128, 1, 0), split_plan(128, 8, 1), split_plan(64, 4, 0)):
+    for plan in (pair_plan(4), pair_plan(8), pair_plan(8, 5), split_plan(64, 1, 0), split_plan(64, 8, 1)):
         out = torch.empty(1500, 900, device="cuda")
         blockscale._matmul(a, b, None, out, False, plan)
         tol = matmul_bound(av, bv, 1300, want, torch.float32) if tol is None else tol
         assert np.all(np.abs(f64(out) - want) <= tol)
 
 
-@pytest.mark.parametrize("plan", [1, 2, split_plan(128, 2, 0), split_plan(32, 1, 1)])
+@pytest.mark.parametrize("plan", [pair_plan(4), pair_plan(8, 4), split_plan(64, 2, 0), split_plan(32, 1, 1)])
 def test_codes_past_the_last_column_do_not_count(plan):
     """The bytes between a row's last code and its pitch, and the scales of rows and blocks past the end, hold NaN."""
     from apa import blockscale
@@ -349,3 +350,41 @@ def test_codes_past_the_last_column_do_not_count(plan):
     out = torch.empty(m, n, device="cuda")
     blockscale._matmul(A, B, None, out, False, plan)
     assert torch.equal(out, want.float())
+
+
+@pytest.mark.parametrize("ew", [4, 8])
+@pytest.mark.parametrize("split", [2, 3, 7, 10])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 270, 1280), (513, 100, 1300), (2600, 1100, 1281)])
+def test_pair_split_exact(ew, split, dtype, m, n, k):
+    """Units of a tile on several pairs, slices added in order, with bias and accumulation."""
+    from apa import blockscale
+    A, B, want = exact_operands(m, n, k, m)
+    bias = torch.randint(-9, 9, (n,), device="cuda").float()
+    out = torch.empty(m, n, dtype=dtype, device="cuda")
+    blockscale._matmul(A, B, bias, out, False, pair_plan(ew, split))
+    assert torch.equal(out, (want + bias.double()).to(dtype))
+    if dtype == torch.float32:
+        blockscale._matmul(A, B, bias, out, True, pair_plan(ew, split))
+        assert torch.equal(out, (2 * (want + bias.double())).float())
+
+
+@pytest.mark.parametrize("plan", [0, pair_plan(4), pair_plan(8), pair_plan(8, 2)])
+@pytest.mark.parametrize("n", [300, 301])
+def test_long_reductions(plan, n):
+    """More than 64 slabs: an fp32 output is summed in rounded chunks (aligned rows by TMA reductions, others by
+    plain additions), each chunk's chain at most 8192 columns long; 16-bit outputs in one chain."""
+    from apa import blockscale
+    m, k = 270, 20000
+    A, B, want = exact_operands(m, n, k, 4)
+    for dtype in DTYPES:
+        out = torch.full((m, n), 5.0, dtype=dtype, device="cuda")
+        blockscale._matmul(A, B, None, out, False, plan)
+        assert torch.equal(out, want.to(dtype))
+    blockscale._matmul(A, B, None, out, True, plan)
+    assert torch.equal(out, (2 * want).float())
+    a, b = block_cast(rnd((m, k), 1, spread=0).cuda()), block_cast(rnd((n, k), 2, spread=0).cuda())
+    out = torch.empty(m, n, device="cuda")
+    blockscale._matmul(a, b, None, out, False, plan)
+    want = a.dequantize().double() @ b.dequantize().double().t()
+    assert float((out - want).norm() / want.norm()) < 1e-6
