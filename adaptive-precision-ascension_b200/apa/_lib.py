@@ -65,7 +65,7 @@ SIGNATURES = {
     "apa_rmsnorm_fwd": [_VP, _I64, _VP, _I64, _VP, _I, _I, _I64, _I64, _F, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP,
                         _VP],
     "apa_rmsnorm_bwd_workspace": [_I64, _I64, _VP],
-    "apa_rmsnorm_bwd": [_VP, _I64, _VP, _I64, _VP, _VP, _I, _VP, _I64, _VP, _I64, _I, _I64, _I64, _VP, _VP, _I64,
+    "apa_rmsnorm_bwd": [_VP, _I, _I64, _VP, _I64, _VP, _VP, _I, _VP, _I64, _VP, _I64, _I, _I64, _I64, _VP, _VP, _I64,
                         _VP],
     "apa_ladder_pack": [_I, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP],
     "apa_ladder_eval": [_I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _I64, _I64,

@@ -372,7 +372,7 @@ def _norm_backward(dh2, r2, rstd, g, dr2):
     n = ctypes.c_int64(0)
     _call(dev, "apa_rmsnorm_bwd_workspace", M, K, ctypes.addressof(n))
     ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
+    _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _REAL[dh2.dtype], _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
           _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K, _REAL[r2.dtype], M, K,
           dg.data_ptr(), ws.data_ptr(), n.value, _lib.stream_handle(dev))
     return dx, dg
@@ -534,7 +534,9 @@ class _BlockLinearFn(torch.autograd.Function):
             dw = torch.empty(N, K, dtype=ctx.weight_dtype, device=dev)
             _matmul(dyt, xt, None, dw, False)
         if need_in:
-            dh = torch.empty(M, K, dtype=ctx.dtype, device=dev)
+            # behind a norm the gradient of its output stays in fp32: rounding it
+            # would add to the rounding of dx and of dgamma's terms
+            dh = torch.empty(M, K, dtype=torch.float32 if ctx.has_norm else ctx.dtype, device=dev)
             _matmul(dyq, ctx.wt, None, dh, False)
             if ctx.has_norm:
                 dx, dg = _norm_backward(dh, r2, ctx.rstd, g, _grad_matrix(dr, ctx.dtype, K))

@@ -14,8 +14,11 @@
 // gradient), per 128 rows.
 //
 // Bound by HBM: every element is read once and written once per form. One
-// 128 x 128 tile per CTA of 256 threads; a thread holds an 8 x 8 piece in
-// registers, so both forms and all maxima come from one read.
+// 128 x 128 tile per CTA of 512 threads; a thread holds a 4 x 8 piece in
+// registers, so both forms and all maxima come from one read, and 64 registers
+// a thread leave room for two CTAs per SM (8 x 8 pieces on 256 threads, with
+// the loads of fewer warps to hide each phase's latency, ran at a third of
+// the speed).
 #include "block_scale.cuh"
 
 namespace apa {
@@ -27,199 +30,224 @@ struct CastArgs {
   uint8_t* dst; int64_t ld_dst; uint8_t* sc;
   uint8_t* dst_t; int64_t ld_dst_t; uint8_t* sc_t;
   float* colsum;
-  int vec_src;
+  int vec_src, vec_mul;
   int64_t tiles_c;
 };
 
-constexpr int kCastThreads = 256;
+constexpr int kCastThreads = 512;
 
 template <int SRC, bool SQUARE>
 __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p) {
-  __shared__ __align__(16) uint8_t s_t[128 * 128];
-  __shared__ uint32_t s_max[8][128];
-  __shared__ float s_sum[8][128];
-  __shared__ uint32_t s_byte[128];
+  __shared__ __align__(16) uint32_t s_t[128 * 32];       // transposed codes, 128 bytes per column
+  __shared__ __align__(16) float s_max[16][128];
+  __shared__ __align__(16) float s_sum[16][128];
+  __shared__ __align__(16) float s_inv[128];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane & 15;                              // columns 8 g .. 8 g + 7
-  const int lr0 = warp * 16 + (lane >> 4) * 8;          // rows lr0 .. lr0 + 7
-  const int64_t tile_r = blockIdx.x / p.tiles_c, tile_c = blockIdx.x % p.tiles_c;
+  const int g = lane & 15, half = lane >> 4;            // columns 8 g .. 8 g + 7
+  const int lr0 = warp * 8 + half * 4;                  // rows lr0 .. lr0 + 3
+  const int64_t tile_r = blockIdx.x / p.tiles_c, tile_c = blockIdx.x - tile_r * p.tiles_c;
   const int64_t row0 = tile_r * 128, col0 = tile_c * 128;
   const int64_t c0 = col0 + 8 * g;
   const int nc = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-  const bool vec = p.vec_src && nc == 8;
+  const int nr = (int)max((int64_t)0, min((int64_t)4, p.rows - row0 - lr0));
 
-  float v[8][8];
+  float v[4][8];
+  if (p.vec_src && row0 + 128 <= p.rows && col0 + 128 <= p.cols) {
+    const int64_t at = (row0 + lr0) * p.ld_src + c0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = row0 + lr0 + i;
-    const int n = r < p.rows ? nc : 0;
-    load8<SRC>(p.src, r * p.ld_src + c0, n, vec && n == 8, v[i]);
+    for (int i = 0; i < 4; ++i) load8<SRC>(p.src, at + i * p.ld_src, 8, true, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = i < nr ? nc : 0;
+      load8<SRC>(p.src, (row0 + lr0 + i) * p.ld_src + c0, n, p.vec_src && n == 8, v[i]);
+    }
   }
   if (p.row_mul != nullptr) {
     float gm[8];
+    load8(p.col_mul, p.col_mul_dt, c0, nc, p.vec_mul && nc == 8, gm);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) gm[j] = j < nc ? to_f32(p.col_mul, p.col_mul_dt, c0 + j) : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+      if (i < nr) {
+        const float rs = p.row_mul[row0 + lr0 + i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t r = row0 + lr0 + i;
-      const float rs = r < p.rows ? p.row_mul[r] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r < p.rows && j < nc) v[i][j] = normed(v[i][j], rs, gm[j]);
+        for (int j = 0; j < 8; ++j)
+          if (j < nc) v[i][j] = normed(v[i][j], rs, gm[j]);
+      }
     }
   }
   if (p.colsum != nullptr) {
-    // column sums in a fixed order: eight rows per thread, two half warps,
-    // eight warps
+    // column sums in a fixed order: four rows per thread, two half warps,
+    // sixteen warps
+    float t[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float t = v[0][j];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) t += v[i][j];
-      t += __shfl_xor_sync(0xFFFFFFFFu, t, 16);
-      if (lane < 16) s_sum[warp][8 * g + j] = t;
+      t[j] = (v[0][j] + v[1][j]) + (v[2][j] + v[3][j]);
+      t[j] += __shfl_xor_sync(0xFFFFFFFFu, t[j], 16);
+    }
+    if (half == 0) {
+      float4* d = reinterpret_cast<float4*>(&s_sum[warp][8 * g]);
+      d[0] = make_float4(t[0], t[1], t[2], t[3]);
+      d[1] = make_float4(t[4], t[5], t[6], t[7]);
     }
   }
 
-  uint32_t rm[8], cm[8], all = 0;
+  float rm[4], cm[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) rm[i] = 0;
+  for (int i = 0; i < 4; ++i) {
+    float a = fmaxf(fabsf(v[i][0]), fabsf(v[i][1])), b = fmaxf(fabsf(v[i][2]), fabsf(v[i][3]));
+    a = fmaxf(a, fmaxf(fabsf(v[i][4]), fabsf(v[i][5])));
+    b = fmaxf(b, fmaxf(fabsf(v[i][6]), fabsf(v[i][7])));
+    rm[i] = fmaxf(a, b);
+  }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cm[j] = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t a = mag_bits(v[i][j]);
-      rm[i] = max(rm[i], a);
-      cm[j] = max(cm[j], a);
-    }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) all = max(all, rm[i]);
-  const bool odd = bits_nonfinite(all);
+  for (int j = 0; j < 8; ++j)
+    cm[j] = fmaxf(fmaxf(fabsf(v[0][j]), fabsf(v[1][j])), fmaxf(fabsf(v[2][j]), fabsf(v[3][j])));
+  float all = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
+  const bool odd = is_inf(all);
   if (odd) {
-    // rare: scales come from the finite values alone
-    all = 0;
+    // rare: the scales come from the finite values alone
+    all = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rm[i] = 0;
+    for (int i = 0; i < 4; ++i) rm[i] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) cm[j] = 0;
+    for (int j = 0; j < 8; ++j) cm[j] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t a = finite_mag(v[i][j]);
-        rm[i] = max(rm[i], a);
-        cm[j] = max(cm[j], a);
-        all = max(all, a);
+        const float a = finite_mag(v[i][j]);
+        rm[i] = fmaxf(rm[i], a);
+        cm[j] = fmaxf(cm[j], a);
+        all = fmaxf(all, a);
       }
   }
+  // a thread of NaNs alone has NaN maxima
+  auto bits = [](float a) { return a == a ? __float_as_uint(a) : 0u; };
 
-  const int64_t kb_c = tile_c, kb_r = tile_r;
   const int64_t rows_pad = rows_padded(p.rows), cols_pad = rows_padded(p.cols);
   uint32_t byte_all = 0;
+  float inv_all = 0.0f;
   if constexpr (SQUARE) {
-    const uint32_t w = warp_max_u32(all);
-    if (lane == 0) s_max[0][warp] = w;
+    const uint32_t w = warp_max_u32(bits(all));
+    if (lane == 0) s_max[0][warp] = __uint_as_float(w);
     __syncthreads();
-    uint32_t m = 0;
+    uint32_t m = __float_as_uint(s_max[0][lane & 15]);
+    byte_all = scale_byte(warp_max_u32(m));
+    inv_all = inv_scale(byte_all);
+  } else if (p.dst_t != nullptr) {
+    uint32_t m[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, s_max[0][k]);
-    byte_all = scale_byte(m);
+    for (int j = 0; j < 8; ++j) {
+      m[j] = bits(cm[j]);
+      m[j] = max(m[j], __shfl_xor_sync(0xFFFFFFFFu, m[j], 16));
+    }
+    if (half == 0) {
+      uint4* d = reinterpret_cast<uint4*>(&s_max[warp][8 * g]);
+      d[0] = make_uint4(m[0], m[1], m[2], m[3]);
+      d[1] = make_uint4(m[4], m[5], m[6], m[7]);
+    }
   }
 
   if (p.dst != nullptr) {
+    float inv[4];
+    if constexpr (SQUARE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t b;
-      if constexpr (SQUARE) {
-        b = byte_all;
-      } else {
-        uint32_t m = rm[i];
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        b = scale_byte(m);
-      }
-      const float is = inv_scale(b);
-      const int64_t r = row0 + lr0 + i;
+      for (int i = 0; i < 4; ++i) inv[i] = inv_all;
       // rows past the end, up to the next multiple of 128, have a scale too
-      if (g == 0) p.sc[scale_offset(rows_pad, r, kb_c)] = (uint8_t)b;
-      if (r < p.rows && nc > 0) {
-        uint2 w;
-        w.x = codes2(v[i][0] * is, v[i][1] * is, odd) | (codes2(v[i][2] * is, v[i][3] * is, odd) << 16);
-        w.y = codes2(v[i][4] * is, v[i][5] * is, odd) | (codes2(v[i][6] * is, v[i][7] * is, odd) << 16);
-        store_codes8(p.dst + r * p.ld_dst + c0, w, nc);
-      }
+      if (g < 4) p.sc[scale_offset(rows_pad, row0 + lr0 + g, tile_c)] = (uint8_t)byte_all;
+    } else {
+      // maxima of four rows over sixteen lanes: each exchange halves the rows
+      // that a lane still follows, until it holds one, in four copies
+      const bool b3 = lane & 8, b2 = lane & 4;
+      uint32_t m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = bits(rm[i]);
+      const uint32_t a0 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[0] : m[2], 8);
+      const uint32_t a1 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[1] : m[3], 8);
+      const uint32_t k0 = max(b3 ? m[2] : m[0], a0), k1 = max(b3 ? m[3] : m[1], a1);
+      uint32_t k = max(b2 ? k1 : k0, __shfl_xor_sync(0xFFFFFFFFu, b2 ? k0 : k1, 4));
+      k = max(k, __shfl_xor_sync(0xFFFFFFFFu, k, 2));
+      k = max(k, __shfl_xor_sync(0xFFFFFFFFu, k, 1));
+      const uint32_t b = scale_byte(k);
+      const int mine = (b3 ? 2 : 0) + (b2 ? 1 : 0);
+      if ((lane & 3) == 0) p.sc[scale_offset(rows_pad, row0 + lr0 + mine, tile_c)] = (uint8_t)b;
+      const float is = inv_scale(b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        inv[i] = __shfl_sync(0xFFFFFFFFu, is, (lane & 16) | ((i >> 1) << 3) | ((i & 1) << 2));
     }
+    uint8_t* d = p.dst + (row0 + lr0) * p.ld_dst + c0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < nr && nc > 0) store_codes8(d + i * p.ld_dst, codes8(v[i], inv[i], odd), nc);
   }
 
-  if (p.dst_t != nullptr || p.colsum != nullptr) {
-    if (!SQUARE && p.dst_t != nullptr) {
+  if (p.dst_t == nullptr && p.colsum == nullptr) return;
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const int c = threadIdx.x;
+    if (p.dst_t != nullptr) {
+      uint32_t b = byte_all;
+      if constexpr (!SQUARE) {
+        uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t m = max(cm[j], __shfl_xor_sync(0xFFFFFFFFu, cm[j], 16));
-        if (lane < 16) s_max[warp][8 * g + j] = m;
+        for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(s_max[k][c]));
+        b = scale_byte(m);
+        s_inv[c] = inv_scale(b);
       }
+      p.sc_t[scale_offset(cols_pad, col0 + c, tile_r)] = (uint8_t)b;
     }
-    __syncthreads();
-    if (threadIdx.x < 128) {
-      const int c = threadIdx.x;
-      if (p.dst_t != nullptr) {
-        uint32_t b = byte_all;
-        if constexpr (!SQUARE) {
-          uint32_t m = 0;
+    if (p.colsum != nullptr && col0 + c < p.cols) {
+      float t = s_sum[0][c];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) m = max(m, s_max[k][c]);
-          b = scale_byte(m);
-        }
-        s_byte[c] = b;
-        p.sc_t[scale_offset(cols_pad, col0 + c, kb_r)] = (uint8_t)b;
-      }
-      if (p.colsum != nullptr && col0 + c < p.cols) {
-        float t = s_sum[0][c];
-#pragma unroll
-        for (int k = 1; k < 8; ++k) t += s_sum[k][c];
-        p.colsum[tile_r * p.cols + col0 + c] = t;
-      }
+      for (int k = 1; k < 16; ++k) t += s_sum[k][c];
+      p.colsum[tile_r * p.cols + col0 + c] = t;
     }
-    if (p.dst_t == nullptr) return;
-    __syncthreads();
-    // s_t[c][r]: row c in 16 chunks of 8 bytes, chunk k at k ^ (c / 8), so that
-    // the sixteen lanes of a half warp (one chunk, sixteen column groups)
-    // write to distinct banks
-    const int chunk = lr0 >> 3;
+  }
+  if (p.dst_t == nullptr) return;
+  float inv[8];
+  if constexpr (SQUARE) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float is = inv_scale(s_byte[8 * g + j]);
-      uint2 w;
-      w.x = codes2(v[0][j] * is, v[1][j] * is, odd) | (codes2(v[2][j] * is, v[3][j] * is, odd) << 16);
-      w.y = codes2(v[4][j] * is, v[5][j] * is, odd) | (codes2(v[6][j] * is, v[7][j] * is, odd) << 16);
-      *reinterpret_cast<uint2*>(s_t + (8 * g + j) * 128 + ((chunk ^ g) << 3)) = w;
+    for (int j = 0; j < 8; ++j) inv[j] = inv_all;
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 x = *reinterpret_cast<const float4*>(&s_inv[8 * g + 4 * h]);
+      inv[4 * h] = x.x; inv[4 * h + 1] = x.y; inv[4 * h + 2] = x.z; inv[4 * h + 3] = x.w;
     }
-    __syncthreads();
-    // eight threads per column, 16 bytes each; odd columns read their two
-    // chunks in the other order, which keeps the half warp's banks distinct
-    const int k2 = threadIdx.x & 7;
+  }
+  // Column c is 32 words of four rows; word u lies at u ^ 2 (c / 8). A warp's
+  // store (two words of sixteen columns) then covers all banks, and four
+  // neighbouring words stay together, at most with their halves exchanged.
+  const int u = warp * 2 + half;
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int c = it * 32 + (threadIdx.x >> 3);
-      const int64_t gc = col0 + c, gr = row0 + 16 * k2;
-      const int sw = c >> 3, first = c & 1;
-      const uint8_t* base = s_t + c * 128;
-      const uint2 a = *reinterpret_cast<const uint2*>(base + (((2 * k2 + first) ^ sw) << 3));
-      const uint2 b = *reinterpret_cast<const uint2*>(base + (((2 * k2 + (first ^ 1)) ^ sw) << 3));
-      const uint2 lo = first ? b : a, hi = first ? a : b;
-      if (gc < p.cols && gr < p.rows) {
-        uint8_t* d = p.dst_t + gc * p.ld_dst_t + gr;
-        const int64_t n = p.rows - gr;
-        if (n >= 16) {
-          *reinterpret_cast<uint4*>(d) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        } else {
-          store_codes8(d, lo, (int)min(n, (int64_t)8));
-          if (n > 8) store_codes8(d + 8, hi, (int)n - 8);
-        }
+  for (int j = 0; j < 8; ++j) {
+    const float x0 = v[0][j] * inv[j], x1 = v[1][j] * inv[j], x2 = v[2][j] * inv[j], x3 = v[3][j] * inv[j];
+    s_t[(8 * g + j) * 32 + (u ^ (2 * g))] =
+        odd ? e4m3x2_exact(x0, x1) | (e4m3x2_exact(x2, x3) << 16) : e4m3x2_sat(x0, x1) | (e4m3x2_sat(x2, x3) << 16);
+  }
+  __syncthreads();
+  const int k2 = threadIdx.x & 7;                        // sixteen rows
+  const int64_t gr = row0 + 16 * k2;
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int c = it * 64 + (threadIdx.x >> 3);
+    const int64_t gc = col0 + c;
+    const int cg = c >> 3;
+    const uint4 x = *reinterpret_cast<const uint4*>(s_t + c * 32 + 4 * (k2 ^ (cg >> 1)));
+    const uint4 w = (cg & 1) ? make_uint4(x.z, x.w, x.x, x.y) : x;
+    if (gc < p.cols && gr < p.rows) {
+      uint8_t* d = p.dst_t + gc * p.ld_dst_t + gr;
+      const int64_t n = p.rows - gr;
+      if (n >= 16) {
+        *reinterpret_cast<uint4*>(d) = w;
+      } else {
+        store_codes8(d, make_uint2(w.x, w.y), (int)min(n, (int64_t)8));
+        if (n > 8) store_codes8(d + 8, make_uint2(w.z, w.w), (int)n - 8);
       }
     }
   }
@@ -262,39 +290,51 @@ __global__ void __launch_bounds__(256) block_dequant_kernel(DequantArgs p) {
 }
 
 // Column sums of [parts, cols] fp32 partials in a fixed order, rounded once to
-// the output's type. 32 columns x 32 warps per CTA, warp w takes rows w, w+32, ..
+// the output's type. A CTA has 8 columns (one sector of every row) and 16, 64 or
+// 128 threads for each, so a few hundred to a thousand rows are one or two
+// rounds of loads.
 __global__ void __launch_bounds__(1024) block_colsum_kernel(const float* part, int64_t parts, int64_t cols, void* out,
                                                             int out_dt) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float s[32][33];
+  __shared__ float s[32][8];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = (int64_t)blockIdx.x * 8 + (lane & 7);
+  const int per = blockDim.x >> 3;
   float t = 0.0f;
   if (c < cols) {
-    int64_t r = w;
-    for (; r + 7 * 32 < parts; r += 8 * 32) {
+    int64_t r = threadIdx.x >> 3;
+    for (; r + 7 * per < parts; r += 8 * per) {
       float x[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = part[(r + 32 * k) * cols + c];
+      for (int k = 0; k < 8; ++k) x[k] = part[(r + per * k) * cols + c];
 #pragma unroll
       for (int k = 0; k < 8; ++k) t += x[k];
     }
-    for (; r < parts; r += 32) t += part[r * cols + c];
-  }
-  s[w][lane] = t;
-  __syncthreads();
-  // column `w` of the CTA is summed by warp w: lanes hold its 32 partials
-  float u = s[lane][w];
+    float x[7];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-  const int64_t oc = (int64_t)blockIdx.x * 32 + w;
-  if (lane == 0 && oc < cols) from_f32(out, out_dt, oc, u);
+    for (int k = 0; k < 7; ++k) x[k] = r + per * k < parts ? part[(r + per * k) * cols + c] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) t += x[k];
+  }
+  t += __shfl_xor_sync(0xFFFFFFFFu, t, 8);
+  t += __shfl_xor_sync(0xFFFFFFFFu, t, 16);
+  if (lane < 8) s[w][lane] = t;
+  __syncthreads();
+  if (w == 0) {
+    const int warps = blockDim.x >> 5;
+    float u = 0.0f;
+    for (int k = lane >> 3; k < warps; k += 4) u += s[k][lane & 7];
+    u += __shfl_xor_sync(0xFFFFFFFFu, u, 8);
+    u += __shfl_xor_sync(0xFFFFFFFFu, u, 16);
+    if (lane < 8 && c < cols) from_f32(out, out_dt, c, u);
+  }
 }
 
 int launch_colsum(const float* part, int64_t parts, int64_t cols, void* out, int out_dt, cudaStream_t s) {
-  const int64_t grid = (cols + 31) / 32;
-  return launch_kernel(block_colsum_kernel, dim3((unsigned)grid), dim3(1024), 0, s, 1, part, parts, cols, out,
+  const int64_t grid = (cols + 7) / 8;
+  const int threads = parts <= 32 ? 128 : parts <= 256 ? 512 : 1024;
+  return launch_kernel(block_colsum_kernel, dim3((unsigned)grid), dim3(threads), 0, s, 1, part, parts, cols, out,
                        out_dt) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }
 
@@ -320,7 +360,7 @@ extern "C" int apa_block_cast(const void* src, int src_dtype, int64_t rows, int6
   if (tr * tc > (1ll << 31) - 1) return APA_ERR_INVALID;
   CastArgs a{src, rows, cols, ld_src, row_mul, col_mul, col_mul_dtype, static_cast<uint8_t*>(dst), ld_dst,
              static_cast<uint8_t*>(scales), static_cast<uint8_t*>(dst_t), ld_dst_t, static_cast<uint8_t*>(scales_t),
-             colsum_partial, vec16(src, ld_src, es) ? 1 : 0, tc};
+             colsum_partial, vec16(src, ld_src, es) ? 1 : 0, vec16(col_mul, 8, 4) ? 1 : 0, tc};
   void (*k)(CastArgs);
   if (src_dtype == APA_DT_F32) k = square ? block_cast_kernel<APA_DT_F32, true> : block_cast_kernel<APA_DT_F32, false>;
   else if (src_dtype == APA_DT_F16) k = square ? block_cast_kernel<APA_DT_F16, true> : block_cast_kernel<APA_DT_F16, false>;

@@ -55,19 +55,19 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
   return __uint_as_float(b == 0u ? 0x00400000u : b << 23);
 }
 
-// max of magnitudes (fp32 bits) that skips NaN and Inf
-__device__ __forceinline__ uint32_t finite_mag(float v) {
-  const uint32_t a = mag_bits(v);
-  return a < 0x7F800000u ? a : 0u;
+// max of magnitudes (fp32 bits) that skips NaN and Inf. Kernels take the plain
+// maximum first (fmaxf skips NaN) and come here only when that is infinite.
+__device__ __forceinline__ float finite_mag(float v) {
+  const float a = fabsf(v);
+  return a < __uint_as_float(0x7F800000u) ? a : 0.0f;
 }
 
-// Two scaled values -> two codes. Finite values are at most 448 in magnitude
-// after scaling, where the saturating conversion rounds to nearest even like
-// the exact one; NaN and Inf become NaN (E4M3 has no infinity). odd: the
-// thread holds a NaN or Inf somewhere.
-__device__ __forceinline__ uint32_t codes2(float lo, float hi, bool odd) {
-  return odd ? e4m3x2_exact(lo, hi) : e4m3x2_sat(lo, hi);
-}
+__device__ __forceinline__ bool is_inf(float a) { return __float_as_uint(a) == 0x7F800000u; }
+
+// Scaled values -> codes. Finite values are at most 448 in magnitude after
+// scaling, where the saturating conversion rounds to nearest even like the
+// exact one, and it maps NaN to NaN. Only an infinity needs the exact rule (NaN;
+// E4M3 has no infinity): odd says that the thread holds one.
 
 // r * rstd * g with one rounding: the product r g is split into its rounded
 // value and the exact remainder, and the last product is a fused one. A value
@@ -111,6 +111,29 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   return r;
 }
 
+template <int DT>
+__device__ __forceinline__ float round_to(float v) {
+  if constexpr (DT == APA_DT_F16) return f16_to_f32(f16_from_f32(v));
+  else if constexpr (DT == APA_DT_BF16) return bf16_to_f32(bf16_from_f32(v));
+  else return v;
+}
+
+// Eight 16-bit elements -> fp32.
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint4& a, float (&v)[8]) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == APA_DT_BF16) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    } else {
+      v[2 * j] = f16lo_to_f32(w[j]);
+      v[2 * j + 1] = f16hi_to_f32(w[j]);
+    }
+  }
+}
+
 // Eight consecutive elements starting at i as fp32; n of them exist (the rest
 // read as 0). vec: i is 16-byte aligned and all eight exist.
 template <int DT>
@@ -122,23 +145,32 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, int n, bool vec,
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
       v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (DT == APA_DT_BF16) {
-          v[2 * j] = __uint_as_float(w[j] << 16);
-          v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        } else {
-          v[2 * j] = f16lo_to_f32(w[j]);
-          v[2 * j + 1] = f16hi_to_f32(w[j]);
-        }
-      }
+      unpack8<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i), v);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32<DT>(p, i + j) : 0.0f;
   }
+}
+
+// The same for an element type known at run time.
+__device__ __forceinline__ void load8(const void* p, int dt, int64_t i, int n, bool vec, float (&v)[8]) {
+  if (dt == APA_DT_F32) load8<APA_DT_F32>(p, i, n, vec, v);
+  else if (dt == APA_DT_F16) load8<APA_DT_F16>(p, i, n, vec, v);
+  else load8<APA_DT_BF16>(p, i, n, vec, v);
+}
+
+// Eight scaled values -> eight codes.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, bool odd) {
+  uint2 w;
+  if (!odd) {
+    w.x = e4m3x2_sat(v[0] * s, v[1] * s) | (e4m3x2_sat(v[2] * s, v[3] * s) << 16);
+    w.y = e4m3x2_sat(v[4] * s, v[5] * s) | (e4m3x2_sat(v[6] * s, v[7] * s) << 16);
+  } else {
+    w.x = e4m3x2_exact(v[0] * s, v[1] * s) | (e4m3x2_exact(v[2] * s, v[3] * s) << 16);
+    w.y = e4m3x2_exact(v[4] * s, v[5] * s) | (e4m3x2_exact(v[6] * s, v[7] * s) << 16);
+  }
+  return w;
 }
 
 template <int DT>

@@ -11,12 +11,15 @@
 // so the backward, which reads r back, differentiates the function the
 // forward computed. dx is the gradient of x and of the residual alike.
 //
-// Bound by HBM: a row is read once into registers (TPR threads per row, NV
-// chunks of eight elements per thread), reduced, and written once. A block of
-// 128 columns is sixteen neighbouring lanes, so its maximum is four shuffles.
-// The backward keeps the columns' dgamma sums in registers over all rows of a
-// CTA and writes them once, so a second kernel adds only a few hundred
-// partial rows, in a fixed order.
+// Bound by HBM. CTAs are persistent: TPR threads share a row, NV chunks of
+// eight elements each, and every thread copies its own chunks of the rows to
+// come into shared memory with cp.async, two rows ahead (no barrier: it reads
+// only what it copied). So loads are in flight while a row is reduced and
+// stored; without that the row's two block-wide barriers left HBM at half its
+// rate. A block of 128 columns is sixteen neighbouring lanes, so its maximum is
+// four shuffles. The backward keeps the columns' dgamma sums in registers over
+// all rows of a CTA and writes them once; a second kernel adds these few hundred
+// partial rows in a fixed order.
 #include "block_scale.cuh"
 
 namespace apa {
@@ -34,7 +37,7 @@ struct NormArgs {
   float* rstd;
   int64_t rows, cols;
   float eps;
-  int vec_x, vec_res, vec_r, vec_y;
+  int vec_x, vec_res, vec_r, vec_y, vec_g;
 };
 
 template <int TPR>
@@ -69,72 +72,167 @@ __device__ __forceinline__ float rsqrt_refined(float a) {
   return __fmaf_rn(0.5f * y, e, y);
 }
 
-template <int DT, int TPR, int NV, bool QUANT>
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int DT> constexpr int pieces() { return DT == APA_DT_F32 ? 2 : 1; }   // 16-byte pieces per chunk
+
+// The chunks of one thread in one row, in planes of 16 bytes per thread (so a
+// warp's accesses are conflict-free). at: this thread's bytes of plane 0.
+template <int DT, int TPR, int NV>
+__device__ __forceinline__ void fetch_row(uint32_t at, const void* p, int64_t row_at, int t, int64_t cols) {
+  constexpr int ES = DT == APA_DT_F32 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
+    if (c0 < cols) {
+      const char* g = static_cast<const char*>(p) + (row_at + c0) * ES;
+#pragma unroll
+      for (int k = 0; k < pieces<DT>(); ++k)
+        cp_async16(at + (uint32_t)((i * pieces<DT>() + k) * norm_threads<TPR>() * 16), g + 16 * k);
+    }
+  }
+}
+
+// Chunk i of the row: from shared memory (ASYNC, whole chunks only) or memory.
+template <int DT, int TPR, bool ASYNC>
+__device__ __forceinline__ void chunk8(const char* at, int i, const void* p, int64_t from, int n, bool vec,
+                                       float (&v)[8]) {
+  if constexpr (ASYNC) {
+    if (n > 0) {
+      const char* a = at + i * pieces<DT>() * norm_threads<TPR>() * 16;
+      const uint4 x = *reinterpret_cast<const uint4*>(a);
+      if constexpr (DT == APA_DT_F32) {
+        const uint4 y = *reinterpret_cast<const uint4*>(a + norm_threads<TPR>() * 16);
+        v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
+        v[4] = __uint_as_float(y.x); v[5] = __uint_as_float(y.y); v[6] = __uint_as_float(y.z); v[7] = __uint_as_float(y.w);
+      } else {
+        unpack8<DT>(x, v);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    }
+  } else {
+    load8<DT>(p, from, n, vec && n == 8, v);
+  }
+}
+
+// Rows in flight: three (or two) row buffers where they fit two CTAs (or one)
+// on an SM, else none.
+constexpr int norm_depth(int slot_bytes) {
+  return 3 * slot_bytes <= 75 * 1024 ? 3 : 2 * slot_bytes <= 200 * 1024 ? 2 : 0;
+}
+
+template <int DT, int TPR, int NV> struct NormCfg {
+  static constexpr int kThreads = norm_threads<TPR>();
+  static constexpr int kRows = kThreads / TPR;
+  static constexpr int kPlane = kThreads * 16;
+  static constexpr int kArray = NV * pieces<DT>() * kPlane;
+  static constexpr int kSlot = 2 * kArray;                       // x, residual
+  static constexpr int kDepth = norm_depth(kSlot);
+};
+
+template <int DT, int TPR, int NV, bool QUANT, bool ASYNC>
 __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p) {
-  constexpr int kRows = norm_threads<TPR>() / TPR;
+  using C = NormCfg<DT, TPR, NV>;
+  constexpr int kRows = C::kRows;
+  constexpr int D = ASYNC ? C::kDepth : 1;
   __shared__ float s_red[32];
+  extern __shared__ __align__(16) char s_rows[];
   pdl_launch_dependents();
   pdl_wait();
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
-  if (TPR == 32 && row >= p.rows) return;      // a whole warp
-  float v[NV][8];
-  float ss = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-    const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-    load8<DT>(p.x, row * p.ld_x + c0, n, p.vec_x && n == 8, v[i]);
-    if (p.res != nullptr) {
-      float u[8];
-      load8<DT>(p.res, row * p.ld_res + c0, n, p.vec_res && n == 8, u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[i][j] += u[j];
-        if constexpr (DT == APA_DT_F16) v[i][j] = f16_to_f32(f16_from_f32(v[i][j]));
-        if constexpr (DT == APA_DT_BF16) v[i][j] = bf16_to_f32(bf16_from_f32(v[i][j]));
-      }
-      if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, v[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) ss = __fmaf_rn(v[i][j], v[i][j], ss);
-  }
-  ss = row_sum<TPR>(ss, s_red);
-  const float rstd = rsqrt_refined(ss / (float)p.cols + p.eps);
-  if (t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+  const int64_t step = (int64_t)gridDim.x * kRows;
   const int64_t rows_pad = rows_padded(p.rows);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-    const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = j < n ? normed(v[i][j], rstd, to_f32(p.gamma, p.gamma_dt, c0 + j)) : 0.0f;
-    if constexpr (QUANT) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, mag_bits(y[j]));
-      const bool odd = bits_nonfinite(m);
-      if (odd) {
-        m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, finite_mag(y[j]));
+  char* mine = s_rows + threadIdx.x * 16;
+  auto fetch = [&](int64_t row, int slot) {
+    if constexpr (ASYNC) {
+      if (row < p.rows) {
+        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(mine + slot * C::kSlot));
+        fetch_row<DT, TPR, NV>(at, p.x, row * p.ld_x, t, p.cols);
+        if (p.res != nullptr) fetch_row<DT, TPR, NV>(at + C::kArray, p.res, row * p.ld_res, t, p.cols);
       }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      const uint32_t b = scale_byte(m);
-      const float is = inv_scale(b);
-      if (n > 0) {
-        uint2 w;
-        w.x = codes2(y[0] * is, y[1] * is, odd) | (codes2(y[2] * is, y[3] * is, odd) << 16);
-        w.y = codes2(y[4] * is, y[5] * is, odd) | (codes2(y[6] * is, y[7] * is, odd) << 16);
-        store_codes8(p.q + row * p.ld_q + c0, w, n);
-        if ((t & 15) == 0) p.sc[scale_offset(rows_pad, row, c0 >> 7)] = (uint8_t)b;
-      }
-    } else {
-      if (n > 0) store8<DT>(p.y, row * p.ld_y + c0, n, p.vec_y && n == 8, y);
+      cp_async_commit();
     }
+  };
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) fetch(row + d * step, d);
+  int slot = 0;
+  // TPR > 32: a CTA's threads share every row, so the loop is uniform
+  for (; row < p.rows; row += step) {
+    if constexpr (ASYNC) {
+      fetch(row + (D - 1) * step, slot == 0 ? D - 1 : slot - 1);
+      cp_async_wait<D - 1>();
+    }
+    const char* at = mine + slot * C::kSlot;
+    float v[NV][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
+      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
+      chunk8<DT, TPR, ASYNC>(at, i, p.x, row * p.ld_x + c0, n, p.vec_x, v[i]);
+      if (p.res != nullptr) {
+        float u[8];
+        chunk8<DT, TPR, ASYNC>(at + C::kArray, i, p.res, row * p.ld_res + c0, n, p.vec_res, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = round_to<DT>(v[i][j] + u[j]);
+        if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, v[i]);
+      }
+      // pairwise: eight squares, then the thread's chunks, then the threads
+      float q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = v[i][j] * v[i][j];
+      ss += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    }
+    ss = row_sum<TPR>(ss, s_red);
+    const float rstd = rsqrt_refined(ss / (float)p.cols + p.eps);
+    if (t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
+      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
+      float y[8], gm[8];
+      load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm);     // in L1 after the first row
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = normed(v[i][j], rstd, gm[j]);
+      if (n < 8) {
+        // columns past the end are 0 whatever the row's statistics
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j >= n) y[j] = 0.0f;
+      }
+      if constexpr (QUANT) {
+        float a = fabsf(y[0]);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) a = fmaxf(a, fabsf(y[j]));
+        const bool odd = is_inf(a);
+        if (odd) {
+          a = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_mag(y[j]));
+        }
+        uint32_t m = a == a ? __float_as_uint(a) : 0u;     // all NaN: no scale
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        const uint32_t b = scale_byte(m);
+        if (n > 0) {
+          store_codes8(p.q + row * p.ld_q + c0, codes8(y, inv_scale(b), odd), n);
+          if ((t & 15) == 0) p.sc[scale_offset(rows_pad, row, c0 >> 7)] = (uint8_t)b;
+        }
+      } else {
+        if (n > 0) store8<DT>(p.y, row * p.ld_y + c0, n, p.vec_y && n == 8, y);
+      }
+    }
+    if constexpr (ASYNC) slot = slot + 1 == D ? 0 : slot + 1;
   }
+  if constexpr (ASYNC) cp_async_wait<0>();
 }
 
 struct NormBwdArgs {
@@ -146,48 +244,78 @@ struct NormBwdArgs {
   void* dx; int64_t ld_dx;
   float* part;                       // [grid, cols] dgamma partials
   int64_t rows, cols;
-  int vec_dy, vec_r, vec_dr, vec_dx;
+  int vec_dy, vec_r, vec_dr, vec_dx, vec_g;
 };
 
-template <int DT, int TPR, int NV>
-__global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_bwd_kernel(NormBwdArgs p) {
-  constexpr int kRows = norm_threads<TPR>() / TPR;
+template <int DT, int DY, int TPR, int NV> struct NormBwdCfg {
+  static constexpr int kThreads = norm_threads<TPR>();
+  static constexpr int kRows = kThreads / TPR;
+  static constexpr int kPlane = kThreads * 16;
+  static constexpr int kArray = NV * pieces<DT>() * kPlane;
+  static constexpr int kArrayDy = NV * pieces<DY>() * kPlane;
+  static constexpr int kSlot = kArrayDy + 2 * kArray;            // dy; r, dr
+  static constexpr int kDepth = norm_depth(kSlot);
+  static constexpr int kSums = kRows > 1 ? kRows * NV * TPR * 8 * 4 : 0;
+};
+
+template <int DT, int DY, int TPR, int NV, bool ASYNC>
+__global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(NormBwdArgs p) {
+  using C = NormBwdCfg<DT, DY, TPR, NV>;
+  constexpr int kRows = C::kRows;
+  constexpr int D = ASYNC ? C::kDepth : 1;
   __shared__ float s_red[32];
-  extern __shared__ float s_dg[];    // kRows > 1: [kRows][NV * TPR * 8]
+  extern __shared__ __align__(16) char s_rows[];    // row buffers, then [kRows][NV * TPR * 8] sums
   pdl_launch_dependents();
   pdl_wait();
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  float dg[NV][8], gm[NV][8];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      dg[i][j] = 0.0f;
-      gm[i][j] = c0 + j < p.cols ? to_f32(p.gamma, p.gamma_dt, c0 + j) : 0.0f;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  char* mine = s_rows + threadIdx.x * 16;
+  auto fetch = [&](int64_t row, int slot) {
+    if constexpr (ASYNC) {
+      if (row < p.rows) {
+        const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(mine + slot * C::kSlot));
+        fetch_row<DY, TPR, NV>(at, p.dy, row * p.ld_dy, t, p.cols);
+        fetch_row<DT, TPR, NV>(at + C::kArrayDy, p.r, row * p.ld_r, t, p.cols);
+        if (p.dr != nullptr) fetch_row<DT, TPR, NV>(at + C::kArrayDy + C::kArray, p.dr, row * p.ld_dr, t, p.cols);
+      }
+      cp_async_commit();
     }
-  }
+  };
+  float dg[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[i][j] = 0.0f;
   const float inv_n = 1.0f / (float)p.cols;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < p.rows; row += (int64_t)gridDim.x * kRows) {
+  int64_t row = (int64_t)blockIdx.x * kRows + sub;
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) fetch(row + d * step, d);
+  int slot = 0;
+  for (; row < p.rows; row += step) {
     const float rstd = p.rstd[row];
-    float dy[NV][8], xh[NV][8];
+    if constexpr (ASYNC) {
+      fetch(row + (D - 1) * step, slot == 0 ? D - 1 : slot - 1);
+      cp_async_wait<D - 1>();
+    }
+    const char* at = mine + slot * C::kSlot;
+    float gdy[NV][8], xh[NV][8];
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
       const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-      load8<DT>(p.dy, row * p.ld_dy + c0, n, p.vec_dy && n == 8, dy[i]);
-      load8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, xh[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+      float gm[8];
+      load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm);     // in L1 after the first row
+      chunk8<DY, TPR, ASYNC>(at, i, p.dy, row * p.ld_dy + c0, n, p.vec_dy, gdy[i]);
+      chunk8<DT, TPR, ASYNC>(at + C::kArrayDy, i, p.r, row * p.ld_r + c0, n, p.vec_r, xh[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         xh[i][j] *= rstd;
-        dg[i][j] = __fmaf_rn(dy[i][j], xh[i][j], dg[i][j]);
-        dy[i][j] *= gm[i][j];
-        s = __fmaf_rn(dy[i][j], xh[i][j], s);
+        dg[i][j] = __fmaf_rn(gdy[i][j], xh[i][j], dg[i][j]);
+        gdy[i][j] *= gm[j];
+        s = __fmaf_rn(gdy[i][j], xh[i][j], s);
       }
+    }
     const float c = row_sum<TPR>(s, s_red) * inv_n;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -195,16 +323,19 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_bwd_kernel(NormBw
       const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
       float o[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = rstd * __fmaf_rn(-xh[i][j], c, dy[i][j]);
+      for (int j = 0; j < 8; ++j) o[j] = rstd * __fmaf_rn(-xh[i][j], c, gdy[i][j]);
       if (p.dr != nullptr) {
         float u[8];
-        load8<DT>(p.dr, row * p.ld_dr + c0, n, p.vec_dr && n == 8, u);
+        chunk8<DT, TPR, ASYNC>(at + C::kArrayDy + C::kArray, i, p.dr, row * p.ld_dr + c0, n, p.vec_dr, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] += u[j];
       }
       if (n > 0) store8<DT>(p.dx, row * p.ld_dx + c0, n, p.vec_dx && n == 8, o);
     }
+    if constexpr (ASYNC) slot = slot + 1 == D ? 0 : slot + 1;
   }
+  if constexpr (ASYNC) cp_async_wait<0>();
+  float* s_dg = reinterpret_cast<float*>(s_rows + (ASYNC ? D * C::kSlot : 0));
   float* out = p.part + (int64_t)blockIdx.x * p.cols;
   if constexpr (kRows > 1) {
     constexpr int kW = NV * TPR * 8;
@@ -232,55 +363,108 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_bwd_kernel(NormBw
 
 constexpr int64_t kMaxNormCols = 32768;   // 1024 threads x 4 chunks of eight
 
-// Threads per row and chunks per thread: a warp per row up to 1024 columns
-// (no block-wide sum), then 128, 512 and 1024 threads with at most four
-// chunks, which keeps a row in 32 registers per thread.
-template <template <int, int, int> class L, int DT, class A>
-int norm_dispatch(const A& a, cudaStream_t s) {
+// Kernels whose row buffers pass 48 KB need the limit raised, per device.
+template <class K>
+int norm_smem(K kernel, int bytes, unsigned long long* done) {
+  if (bytes <= 47 * 1024) return APA_OK;      // static shared memory counts too
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return APA_ERR_CUDA;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return APA_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return APA_ERR_CUDA;
+  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
+  return APA_OK;
+}
+
+// CTAs per SM: as many as the threads and the row buffers allow.
+int64_t norm_per_sm(int threads, int smem, int most) {
+  return std::max<int64_t>(1, std::min<int64_t>(std::min(2048 / threads, most), 220 * 1024 / (smem + 1024)));
+}
+
+template <int DT, int TPR, int NV, bool QUANT, bool ASYNC>
+int launch_norm_k(const NormArgs& a, cudaStream_t s) {
+  using C = NormCfg<DT, TPR, NV>;
+  constexpr int kSmem = ASYNC ? C::kDepth * C::kSlot : 0;
+  static unsigned long long attr = 0;
+  if (int st = norm_smem(rmsnorm_kernel<DT, TPR, NV, QUANT, ASYNC>, kSmem, &attr)) return st;
+  // at most 1024 threads' worth of registers (64 each)
+  const int64_t most = norm_per_sm(C::kThreads, kSmem, 1024 / C::kThreads) * num_sms();
+  const int64_t all = (a.rows + C::kRows - 1) / C::kRows;
+  const int64_t grid = ASYNC ? std::min<int64_t>(all, most) : all;
+  return launch_kernel(rmsnorm_kernel<DT, TPR, NV, QUANT, ASYNC>, dim3((unsigned)grid), dim3(C::kThreads), kSmem, s, 1,
+                       a) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
+}
+
+template <int DT, int TPR, int NV>
+int launch_norm(const NormArgs& a, cudaStream_t s) {
+  if constexpr (TPR > 32 && NormCfg<DT, TPR, NV>::kDepth >= 2) {
+    if (a.vec_x && (!a.res || a.vec_res) && a.cols % 8 == 0)
+      return a.q ? launch_norm_k<DT, TPR, NV, true, true>(a, s) : launch_norm_k<DT, TPR, NV, false, true>(a, s);
+  }
+  return a.q ? launch_norm_k<DT, TPR, NV, true, false>(a, s) : launch_norm_k<DT, TPR, NV, false, false>(a, s);
+}
+
+// Threads per row and chunks per thread: a warp per row up to 512 columns (no
+// block-wide sum), then 128 to 1024 threads with two chunks at most (four past
+// 16384 columns), so that a row and the backward's sums stay in registers.
+template <int DT>
+int norm_forward(const NormArgs& a, cudaStream_t s) {
   const int64_t chunks = (a.cols + 7) / 8;
-  if (chunks <= 32) return L<DT, 32, 1>::run(a, s);
-  if (chunks <= 64) return L<DT, 32, 2>::run(a, s);
-  if (chunks <= 128) return L<DT, 32, 4>::run(a, s);
-  if (chunks <= 256) return L<DT, 128, 2>::run(a, s);
-  if (chunks <= 512) return L<DT, 128, 4>::run(a, s);
-  if (chunks <= 1024) return L<DT, 512, 2>::run(a, s);
-  if (chunks <= 2048) return L<DT, 512, 4>::run(a, s);
-  return L<DT, 1024, 4>::run(a, s);
+  if (chunks <= 32) return launch_norm<DT, 32, 1>(a, s);
+  if (chunks <= 64) return launch_norm<DT, 32, 2>(a, s);
+  if (chunks <= 128) return launch_norm<DT, 32, 4>(a, s);
+  if (chunks <= 256) return launch_norm<DT, 128, 2>(a, s);
+  if (chunks <= 512) return launch_norm<DT, 256, 2>(a, s);
+  if (chunks <= 1024) return launch_norm<DT, 512, 2>(a, s);
+  if (chunks <= 2048) return launch_norm<DT, 1024, 2>(a, s);
+  return launch_norm<DT, 1024, 4>(a, s);
 }
 
-template <int DT, int TPR, int NV> struct NormFwd {
-  static int run(const NormArgs& a, cudaStream_t s) {
-    constexpr int kRows = norm_threads<TPR>() / TPR;
-    const int64_t grid = (a.rows + kRows - 1) / kRows;
-    void (*k)(NormArgs) = a.q ? rmsnorm_kernel<DT, TPR, NV, true> : rmsnorm_kernel<DT, TPR, NV, false>;
-    return launch_kernel(k, dim3((unsigned)grid), dim3(norm_threads<TPR>()), 0, s, 1, a) == cudaSuccess ? APA_OK
-                                                                                                        : APA_ERR_CUDA;
-  }
-};
-
-template <int TPR>
-int64_t norm_bwd_grid(int64_t rows) {
-  constexpr int kRows = norm_threads<TPR>() / TPR;
-  const int64_t per_sm = TPR >= 1024 ? 1 : TPR >= 512 ? 2 : 6;
-  return std::min<int64_t>((rows + kRows - 1) / kRows, per_sm * num_sms());
-}
-
-template <int DT, int TPR, int NV> struct NormBwd {
-  static int run(const NormBwdArgs& a, cudaStream_t s) {
-    constexpr int kRows = norm_threads<TPR>() / TPR;
-    const size_t smem = kRows > 1 ? (size_t)kRows * NV * TPR * 8 * 4 : 0;   // at most 16 KB
-    return launch_kernel(rmsnorm_bwd_kernel<DT, TPR, NV>, dim3((unsigned)norm_bwd_grid<TPR>(a.rows)),
-                         dim3(norm_threads<TPR>()), smem, s, 1, a) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
-  }
-};
-
-// CTAs (= dgamma partial rows) of the backward
+// CTAs (= dgamma partial rows) of the backward, as many as are resident at once
+// (a thread holds 64 to 116 registers).
 int64_t norm_bwd_parts(int64_t rows, int64_t cols) {
   const int64_t chunks = (cols + 7) / 8;
-  if (chunks <= 128) return norm_bwd_grid<32>(rows);
-  if (chunks <= 512) return norm_bwd_grid<128>(rows);
-  if (chunks <= 2048) return norm_bwd_grid<512>(rows);
-  return norm_bwd_grid<1024>(rows);
+  const int tpr = chunks <= 64 ? 32 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : 1024;
+  const int per_cta = tpr < 128 ? 128 / tpr : 1;
+  const int64_t per_sm = tpr >= 512 ? 1 : tpr >= 256 ? 2 : tpr == 128 && chunks <= 128 ? 8 : 4;
+  return std::min<int64_t>((rows + per_cta - 1) / per_cta, per_sm * num_sms());
+}
+
+template <int DT, int DY, int TPR, int NV, bool ASYNC>
+int launch_norm_bwd_k(const NormBwdArgs& a, int64_t parts, cudaStream_t s) {
+  using C = NormBwdCfg<DT, DY, TPR, NV>;
+  constexpr int kSmem = (ASYNC ? C::kDepth * C::kSlot : 0) + C::kSums;
+  static unsigned long long attr = 0;
+  if (int st = norm_smem(rmsnorm_bwd_kernel<DT, DY, TPR, NV, ASYNC>, kSmem, &attr)) return st;
+  return launch_kernel(rmsnorm_bwd_kernel<DT, DY, TPR, NV, ASYNC>, dim3((unsigned)parts), dim3(C::kThreads), kSmem, s,
+                       1, a) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
+}
+
+template <int DT, int DY, int TPR, int NV>
+int launch_norm_bwd(const NormBwdArgs& a, int64_t parts, cudaStream_t s) {
+  // Short rows need no buffers where enough warps fit an SM to hide their loads:
+  // 33280 x 512 fp32 41 us against 59 with buffers, 8192 x 1024 bf16 18 against
+  // 20; but 16384 x 384 bf16 15 with and 23 without, 8192 x 2048 33 and 41.
+  constexpr bool kBuffers = TPR >= 256 || (NV == 2 && (TPR == 128 || (DT != APA_DT_F32 && DY != APA_DT_F32)));
+  if constexpr (kBuffers && NormBwdCfg<DT, DY, TPR, NV>::kDepth >= 2) {
+    if (a.vec_dy && a.vec_r && (!a.dr || a.vec_dr) && a.cols % 8 == 0)
+      return launch_norm_bwd_k<DT, DY, TPR, NV, true>(a, parts, s);
+  }
+  return launch_norm_bwd_k<DT, DY, TPR, NV, false>(a, parts, s);
+}
+
+template <int DT, int DY>
+int norm_backward(const NormBwdArgs& a, int64_t parts, cudaStream_t s) {
+  const int64_t chunks = (a.cols + 7) / 8;
+  if (chunks <= 32) return launch_norm_bwd<DT, DY, 32, 1>(a, parts, s);
+  if (chunks <= 64) return launch_norm_bwd<DT, DY, 32, 2>(a, parts, s);
+  if (chunks <= 128) return launch_norm_bwd<DT, DY, 128, 1>(a, parts, s);
+  if (chunks <= 256) return launch_norm_bwd<DT, DY, 128, 2>(a, parts, s);
+  if (chunks <= 512) return launch_norm_bwd<DT, DY, 256, 2>(a, parts, s);
+  if (chunks <= 1024) return launch_norm_bwd<DT, DY, 512, 2>(a, parts, s);
+  if (chunks <= 2048) return launch_norm_bwd<DT, DY, 1024, 2>(a, parts, s);
+  return launch_norm_bwd<DT, DY, 1024, 4>(a, parts, s);
 }
 
 int norm_dims(int64_t rows, int64_t cols) {
@@ -308,11 +492,12 @@ extern "C" int apa_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual
   NormArgs a{x, ld_x, residual, ld_res, gamma, gamma_dtype, stream_out, ld_stream, y, ld_y,
              static_cast<uint8_t*>(q), ld_q, static_cast<uint8_t*>(scales), rstd, rows, cols, eps,
              vec16(x, ld_x, es) ? 1 : 0, residual && vec16(residual, ld_res, es) ? 1 : 0,
-             stream_out && vec16(stream_out, ld_stream, es) ? 1 : 0, y && vec16(y, ld_y, es) ? 1 : 0};
+             stream_out && vec16(stream_out, ld_stream, es) ? 1 : 0, y && vec16(y, ld_y, es) ? 1 : 0,
+             vec16(gamma, 8, 4) ? 1 : 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == APA_DT_F32) return norm_dispatch<NormFwd, APA_DT_F32>(a, s);
-  if (dtype == APA_DT_F16) return norm_dispatch<NormFwd, APA_DT_F16>(a, s);
-  return norm_dispatch<NormFwd, APA_DT_BF16>(a, s);
+  if (dtype == APA_DT_F32) return norm_forward<APA_DT_F32>(a, s);
+  if (dtype == APA_DT_F16) return norm_forward<APA_DT_F16>(a, s);
+  return norm_forward<APA_DT_BF16>(a, s);
 }
 
 extern "C" int apa_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int64_t* bytes_out) {
@@ -323,7 +508,7 @@ extern "C" int apa_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int64_t* by
   return APA_OK;
 }
 
-extern "C" int apa_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* r, int64_t ld_r, const float* rstd,
+extern "C" int apa_rmsnorm_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* r, int64_t ld_r, const float* rstd,
                                const void* gamma, int gamma_dtype, const void* dr, int64_t ld_dr, void* dx,
                                int64_t ld_dx, int dtype, int64_t rows, int64_t cols, void* dgamma, void* workspace,
                                int64_t workspace_bytes, void* stream) {
@@ -332,18 +517,21 @@ extern "C" int apa_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* r, int
   if (int st = norm_dims(rows, cols)) return st;
   const int es = elem_bytes(dtype);
   if (es == 0 || elem_bytes(gamma_dtype) == 0) return APA_ERR_UNSUPPORTED;
+  if (dy_dtype != dtype && dy_dtype != APA_DT_F32) return APA_ERR_UNSUPPORTED;
   if (ld_dy < cols || ld_r < cols || ld_dx < cols || (dr && ld_dr < cols)) return APA_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return APA_ERR_ALIGN;
   const int64_t parts = norm_bwd_parts(rows, cols);
   if (workspace_bytes < parts * cols * 4) return APA_ERR_INVALID;
   NormBwdArgs a{dy, ld_dy, r, ld_r, rstd, gamma, gamma_dtype, dr, ld_dr, dx, ld_dx, static_cast<float*>(workspace),
-                rows, cols, vec16(dy, ld_dy, es) ? 1 : 0, vec16(r, ld_r, es) ? 1 : 0,
-                dr && vec16(dr, ld_dr, es) ? 1 : 0, vec16(dx, ld_dx, es) ? 1 : 0};
+                rows, cols, vec16(dy, ld_dy, elem_bytes(dy_dtype)) ? 1 : 0, vec16(r, ld_r, es) ? 1 : 0,
+                dr && vec16(dr, ld_dr, es) ? 1 : 0, vec16(dx, ld_dx, es) ? 1 : 0, vec16(gamma, 8, 4) ? 1 : 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int st;
-  if (dtype == APA_DT_F32) st = norm_dispatch<NormBwd, APA_DT_F32>(a, s);
-  else if (dtype == APA_DT_F16) st = norm_dispatch<NormBwd, APA_DT_F16>(a, s);
-  else st = norm_dispatch<NormBwd, APA_DT_BF16>(a, s);
+  if (dtype == APA_DT_F32) st = norm_backward<APA_DT_F32, APA_DT_F32>(a, parts, s);
+  else if (dtype == APA_DT_F16 && dy_dtype == dtype) st = norm_backward<APA_DT_F16, APA_DT_F16>(a, parts, s);
+  else if (dtype == APA_DT_F16) st = norm_backward<APA_DT_F16, APA_DT_F32>(a, parts, s);
+  else if (dy_dtype == dtype) st = norm_backward<APA_DT_BF16, APA_DT_BF16>(a, parts, s);
+  else st = norm_backward<APA_DT_BF16, APA_DT_F32>(a, parts, s);
   if (st != APA_OK) return st;
   return launch_colsum(a.part, parts, cols, dgamma, gamma_dtype, s);
 }

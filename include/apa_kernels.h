@@ -450,12 +450,12 @@ int apa_rmsnorm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t l
 int apa_rmsnorm_bwd_workspace(int64_t rows, int64_t cols, int64_t* bytes_out);
 
 /*
- * Gradients of apa_rmsnorm_fwd from dy (of the output), r (the stream), rstd
+ * Gradients of apa_rmsnorm_fwd from dy (of the output; dtype or F32), r (the stream), rstd
  * and dr (nullable: the gradient of the stream itself): dx, of x and residual
  * alike (dtype), and dgamma (gamma_dtype). Deterministic. workspace: 16-byte
  * aligned, apa_rmsnorm_bwd_workspace bytes, used only during the call.
  */
-int apa_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* r, int64_t ld_r, const float* rstd,
+int apa_rmsnorm_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* r, int64_t ld_r, const float* rstd,
                     const void* gamma, int gamma_dtype, const void* dr, int64_t ld_dr, void* dx, int64_t ld_dx,
                     int dtype, int64_t rows, int64_t cols, void* dgamma, void* workspace, int64_t workspace_bytes,
                     void* stream);

@@ -146,10 +146,11 @@ def test_entry_points_check_their_arguments():
     assert lib.apa_rmsnorm_bwd_workspace(2, 32, None) == I
     assert lib.apa_rmsnorm_bwd_workspace(0, 32, ctypes.addressof(n)) == I
 
-    def bwd(dy=16, dx=16, dg=16, ws=16, wb=1 << 30, cols=32, dt=0, gd=0):
-        return lib.apa_rmsnorm_bwd(dy, 32, 16, 32, 16, 16, gd, None, 0, dx, 32, dt, 2, cols, dg, ws, wb, None)
+    def bwd(dy=16, dx=16, dg=16, ws=16, wb=1 << 30, cols=32, dt=0, gd=0, dyt=0):
+        return lib.apa_rmsnorm_bwd(dy, dyt, 32, 16, 32, 16, 16, gd, None, 0, dx, 32, dt, 2, cols, dg, ws, wb, None)
 
     assert bwd(dy=None) == I and bwd(dx=None) == I and bwd(dg=None) == I and bwd(ws=None) == I and bwd(cols=33) == I
+    assert bwd(dyt=2) == U and bwd(dt=2, dyt=1) == U
     assert bwd(dt=3) == U and bwd(gd=3) == U and bwd(ws=8) == A
     assert lib.apa_block_dequant(None, 32, 16, 2, 32, 16, 0, 32, None) == I
     assert lib.apa_block_dequant(16, 32, 16, 2, 32, 16, 3, 32, None) == U

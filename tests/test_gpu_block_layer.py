@@ -128,7 +128,7 @@ def test_norm_in_front(lead, k, n, dtype, with_res):
         wq, wt = block_cast(lin.weight_master, "both", square=True)
         assert torch.equal(block_matmul(q, wq, lin.bias_master, out_dtype=dtype), y.reshape(-1, n))
         dq, dt = block_cast(dy, "both")
-        dh = block_matmul(dq, wt, out_dtype=dtype)
+        dh = block_matmul(dq, wt, out_dtype=torch.float32)
         r2 = r.detach().reshape(-1, k)
         _, _, rstd = blockscale._norm_forward(r2, norm.weight, None, norm.eps, True, True)
         dx, dg = blockscale._norm_backward(dh, r2, rstd, norm.weight, dr.view(-1, k) if with_res else None)
