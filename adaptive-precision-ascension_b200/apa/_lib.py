@@ -62,6 +62,11 @@ SIGNATURES = {
     "apa_block_gemm": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _I, _I, _VP,
                        _I64, _VP],
     "apa_block_gemm_workspace": [_I64, _I64, _I64, _I, _I, _VP],
+    "apa_block_linear_fwd": [_VP, _I, _I64, _VP, _I64, _VP, _I, _F, _VP, _I64, _VP, _VP, _VP, _VP, _I, _I64, _VP, _VP,
+                             _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _VP, _I64, _VP],
+    "apa_block_linear_bwd_workspace": [_I64, _I64, _I64, _I, _I, _I, _VP],
+    "apa_block_linear_bwd": [_VP, _I, _I64, _VP, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I64, _VP, _I, _I64, _VP, _VP, _I,
+                             _I64, _VP, _I, _I64, _I64, _I64, _VP, _I64, _VP],
     "apa_rmsnorm_fwd": [_VP, _I64, _VP, _I64, _VP, _I, _I, _I64, _I64, _F, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP,
                         _VP],
     "apa_rmsnorm_bwd_workspace": [_I64, _I64, _VP],

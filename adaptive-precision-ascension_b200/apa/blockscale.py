@@ -54,9 +54,14 @@ _E4M3 = torch.float8_e4m3fn
 _REAL = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 
 
+_fns: dict = {}
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """One library call on the tensors' device, whichever is current."""
-    fn = getattr(_lib.lib(), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
     if device.index == torch.cuda.current_device():
         _lib.check(fn(*args), name)
     else:
@@ -75,13 +80,14 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     """x as a 2-D matrix with unit column stride, rows a positive distance apart."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(x).__name__}")
-    if x.dim() < 1:
+    d = x.dim()
+    if d < 1:
         raise ValueError(f"{what}: expected at least one dimension")
-    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    m = x if d == 2 else x.reshape(-1, x.shape[-1])
     n = m.shape[1]
     if n == 0:
         raise ValueError(f"{what}: has no columns")
-    if m.stride(1) != 1 and n > 1 or (m.shape[0] > 1 and m.stride(0) < n):
+    if not m.is_contiguous() and ((n > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < n)):
         m = m.contiguous()
     return m
 
@@ -105,15 +111,14 @@ def _vector(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.T
     return t if t.stride(0) == 1 else t.contiguous()
 
 
-def _codes(rows: int, cols: int, device) -> torch.Tensor:
-    """[rows, cols] E4M3 view whose row pitch is a multiple of 16 bytes."""
-    pitch = (cols + 15) & ~15
-    t = torch.empty(rows, pitch, dtype=_E4M3, device=device)
-    return t if pitch == cols else t[:, :cols]
+def _pitch(cols: int) -> int:
+    return (cols + 15) & ~15
 
 
-def _scale_bytes(rows: int, cols: int) -> int:
-    return ((cols + 511) >> 9) * ((rows + 127) & ~127) * 4
+def _packed_bytes(rows: int, cols: int) -> int:
+    """Codes with a row pitch of 16 bytes' multiple, then the scales: a 32-bit
+    word per row (rounded up to 128 rows) and 512 columns."""
+    return rows * _pitch(cols) + ((cols + 511) >> 9) * ((rows + 127) & ~127) * 4
 
 
 class APABlockTensor:
@@ -122,19 +127,34 @@ class APABlockTensor:
     in the order the tensor cores take, see ``exponents()`` for the plain one.
     """
 
-    __slots__ = ("data", "scales")
+    __slots__ = ("buffer", "rows", "cols")
 
-    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
-        self.data = data
-        self.scales = scales
+    def __init__(self, buffer: torch.Tensor, rows: int, cols: int):
+        self.buffer = buffer          # uint8: the codes, row by row with a pitch of _pitch(cols), then the scales
+        self.rows = rows
+        self.cols = cols
+
+    @property
+    def data(self) -> torch.Tensor:
+        pitch = _pitch(self.cols)
+        return self.buffer[:self.rows * pitch].view(_E4M3).view(self.rows, pitch)[:, :self.cols]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.buffer[self.rows * _pitch(self.cols):]
 
     @property
     def shape(self) -> torch.Size:
-        return self.data.shape
+        return torch.Size((self.rows, self.cols))
 
     @property
     def device(self) -> torch.device:
-        return self.data.device
+        return self.buffer.device
+
+    def _at(self) -> Tuple[int, int, int]:
+        """Addresses of codes and scales, and the codes' pitch."""
+        p, pitch = self.buffer.data_ptr(), _pitch(self.cols)
+        return p, pitch, p + self.rows * pitch
 
     def __repr__(self) -> str:
         return f"APABlockTensor({list(self.shape)}, device={self.device})"
@@ -168,10 +188,10 @@ class APABlockTensor:
         full = torch.full((rp, kp), 127, dtype=torch.uint8, device=data.device)
         full[:rows, :kb] = (e + 127).to(torch.uint8)
         # [row group, quarter, lane, word, byte] -> [word, row group, lane, quarter, byte]
-        scales = full.view(rp // 128, 4, 32, kp // 4, 4).permute(3, 0, 2, 1, 4).contiguous().view(-1)
-        q = _codes(rows, cols, data.device)
-        q.view(torch.uint8).copy_(data.view(torch.uint8))
-        return cls(q, scales)
+        t = _new_block(rows, cols, data.device)
+        t.scales.copy_(full.view(rp // 128, 4, 32, kp // 4, 4).permute(3, 0, 2, 1, 4).reshape(-1))
+        t.data.view(torch.uint8).copy_(data.view(torch.uint8))
+        return t
 
     def exponents(self) -> torch.Tensor:
         """int32 [rows, ceil(cols / 128)]: block b of row r has the scale 2^exponents[r, b]."""
@@ -185,23 +205,21 @@ class APABlockTensor:
         """The values code * scale, in ``dtype`` (exact in float32 and, within
         its range, bfloat16)."""
         code = _real(dtype, "APABlockTensor.dequantize")
-        _lib.require_cuda(self.data, "APABlockTensor.dequantize")
-        rows, cols = self.shape
+        _lib.require_cuda(self.buffer, "APABlockTensor.dequantize")
+        rows, cols = self.rows, self.cols
         out = torch.empty(rows, cols, dtype=dtype, device=self.device)
         if rows:
-            _call(self.device, "apa_block_dequant", self.data.data_ptr(), _ld(self.data) if rows > 1 else
-                  (cols + 15) & ~15, self.scales.data_ptr(), rows, cols, out.data_ptr(), code, cols,
+            p, pitch, sc = self._at()
+            _call(self.device, "apa_block_dequant", p, pitch, sc, rows, cols, out.data_ptr(), code, cols,
                   _lib.stream_handle(self.device))
         return out
 
 
 def _new_block(rows: int, cols: int, device) -> APABlockTensor:
-    return APABlockTensor(_codes(rows, cols, device),
-                          torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))
+    return APABlockTensor(torch.empty(_packed_bytes(rows, cols), dtype=torch.uint8, device=device), rows, cols)
 
 
-def _pitch(t: APABlockTensor) -> int:
-    return t.data.stride(0) if t.data.shape[0] > 1 else (t.data.shape[1] + 15) & ~15
+_NONE = (None, 0, None)
 
 
 def _cast(x2: torch.Tensor, rows_form: bool, cols_form: bool, square: bool = False, colsum=None, row_mul=None,
@@ -214,9 +232,7 @@ def _cast(x2: torch.Tensor, rows_form: bool, cols_form: bool, square: bool = Fal
         return q, qt
     _call(dev, "apa_block_cast", x2.data_ptr(), _REAL[x2.dtype], rows, cols, _ld(x2), _lib.ptr(row_mul),
           _lib.ptr(col_mul), _REAL[col_mul.dtype] if col_mul is not None else 0, int(square),
-          q.data.data_ptr() if q else None, _pitch(q) if q else 0, q.scales.data_ptr() if q else None,
-          qt.data.data_ptr() if qt else None, _pitch(qt) if qt else 0, qt.scales.data_ptr() if qt else None,
-          _lib.ptr(colsum), _lib.stream_handle(dev))
+          *(q._at() if q else _NONE), *(qt._at() if qt else _NONE), _lib.ptr(colsum), _lib.stream_handle(dev))
     return q, qt
 
 
@@ -250,14 +266,13 @@ def _matmul_workspace(M: int, N: int, K: int, dtype: int, plan: int, device: int
 
 
 def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool, plan: int = 0) -> None:
-    M, K = a.shape
-    N = b.shape[0]
+    M, K, N = a.rows, a.cols, b.rows
     dt = _REAL[out.dtype]
     n = _matmul_workspace(M, N, K, dt, plan, a.device.index)
     ws = torch.empty(n, dtype=torch.uint8, device=a.device) if n else None
-    _call(a.device, "apa_block_gemm", a.data.data_ptr(), _pitch(a), a.scales.data_ptr(), b.data.data_ptr(), _pitch(b),
-          b.scales.data_ptr(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, out.data_ptr(), dt,
-          _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n, _lib.stream_handle(a.device))
+    _call(a.device, "apa_block_gemm", *a._at(), *b._at(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0,
+          out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n,
+          _lib.stream_handle(a.device))
 
 
 def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,
@@ -270,12 +285,11 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
     ``accumulate`` the product is added to a float32 ``out``."""
     if not isinstance(a, APABlockTensor) or not isinstance(b, APABlockTensor):
         raise TypeError("block_matmul: both operands must be APABlockTensors")
-    _lib.require_cuda(a.data, "block_matmul")
-    _same_device("block_matmul", a.device, b.data)
-    M, K = a.shape
-    N = b.shape[0]
-    if b.shape[1] != K:
-        raise ValueError(f"block_matmul: operands reduce over {K} and {b.shape[1]} columns")
+    _lib.require_cuda(a.buffer, "block_matmul")
+    _same_device("block_matmul", a.device, b.buffer)
+    M, K, N = a.rows, a.cols, b.rows
+    if b.cols != K:
+        raise ValueError(f"block_matmul: operands reduce over {K} and {b.cols} columns")
     if N == 0:
         raise ValueError("block_matmul: the second operand has no rows")
     if bias is not None:
@@ -308,13 +322,40 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     if not isinstance(weight, APABlockTensor):
         raise TypeError("block_linear: the weight must be an APABlockTensor (block_cast(w, square=True))")
     x2 = _matrix(x, "block_linear")
-    _real(x2.dtype, "block_linear")
+    code = _real(x2.dtype, "block_linear")
     _lib.require_cuda(x2, "block_linear")
-    if x2.shape[1] != weight.shape[1]:
-        raise ValueError(f"block_linear: x has {x2.shape[1]} features, the weight {weight.shape[1]}")
-    q, _ = _cast(x2, True, False)
-    y = block_matmul(q, weight, bias, out_dtype or x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+    M, K = x2.shape
+    N = weight.rows
+    dev = x2.device
+    if K != weight.cols:
+        raise ValueError(f"block_linear: x has {K} features, the weight {weight.cols}")
+    _same_device("block_linear", dev, weight.buffer)
+    if bias is not None:
+        bias = _vector(bias, N, dev, "block_linear: bias")
+    out_code = code if out_dtype is None else _real(out_dtype, "block_linear: out_dtype")
+    y = torch.empty(M, N, dtype=out_dtype or x2.dtype, device=dev)
+    if M:
+        _linear_forward(x2, code, None, None, 0.0, None, None, None, None, weight.buffer.data_ptr(), None, bias, y,
+                        out_code, M, N, K)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bias, y, out_code, M, N, K) -> None:
+    """apa_block_linear_fwd with its temporaries in one buffer. xt, wq, wt:
+    addresses of packed block tensors; wq None: the weight w2 is cast into the
+    temporary buffer too."""
+    dev = x2.device
+    n = _matmul_workspace(M, N, K, out_code, 0, dev.index)
+    at_w = (_packed_bytes(M, K) + 255) & ~255
+    at_ws = at_w + ((_packed_bytes(N, K) + 255) & ~255 if wq is None else 0)
+    tmp = torch.empty(at_ws + n, dtype=torch.uint8, device=dev)
+    p = tmp.data_ptr()
+    _call(dev, "apa_block_linear_fwd", x2.data_ptr(), code, _ld(x2),
+          _lib.ptr(res2), _ld(res2) if res2 is not None else 0,
+          _lib.ptr(gamma), _REAL[gamma.dtype] if gamma is not None else 0, eps, _lib.ptr(stream), K, _lib.ptr(rstd),
+          p, xt, _lib.ptr(w2), _REAL[w2.dtype] if w2 is not None else 0, _ld(w2) if w2 is not None else 0,
+          p + at_w if wq is None else wq, wt, _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0,
+          y.data_ptr(), out_code, N, M, N, K, p + at_ws, n, _lib.stream_handle(dev))
 
 
 # ---------------------------------------------------------------------------
@@ -339,10 +380,9 @@ def _norm_args(x, weight, residual, what: str):
 
 
 def _check_eps(eps: float, what: str) -> float:
-    eps = float(eps)
-    if not (eps >= 0.0 and math.isfinite(eps)):
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f"{what}: eps must be finite and not negative")
-    return eps
+    return float(eps)
 
 
 def _norm_forward(x2, g, res2, eps: float, quantize: bool, want_rstd: bool):
@@ -356,9 +396,16 @@ def _norm_forward(x2, g, res2, eps: float, quantize: bool, want_rstd: bool):
     if M:
         _call(dev, "apa_rmsnorm_fwd", x2.data_ptr(), _ld(x2), _lib.ptr(res2), _ld(res2) if res2 is not None else 0,
               g.data_ptr(), _REAL[g.dtype], _REAL[x2.dtype], M, K, eps, _lib.ptr(stream), K, _lib.ptr(y), K,
-              q.data.data_ptr() if q else None, _pitch(q) if q else 0, q.scales.data_ptr() if q else None,
-              _lib.ptr(rstd), _lib.stream_handle(dev))
+              *(q._at() if q else _NONE), _lib.ptr(rstd), _lib.stream_handle(dev))
     return (q if quantize else y), stream, rstd
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(M: int, K: int, device: int) -> int:
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().apa_rmsnorm_bwd_workspace(M, K, ctypes.addressof(n)), "apa_rmsnorm_bwd_workspace")
+    return n.value
 
 
 def _norm_backward(dh2, r2, rstd, g, dr2):
@@ -369,12 +416,11 @@ def _norm_backward(dh2, r2, rstd, g, dr2):
     dg = torch.empty(K, dtype=g.dtype, device=dev)
     if M == 0:
         return dx, dg.zero_()
-    n = ctypes.c_int64(0)
-    _call(dev, "apa_rmsnorm_bwd_workspace", M, K, ctypes.addressof(n))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+    n = _norm_workspace(M, K, dev.index)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _REAL[dh2.dtype], _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
           _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K, _REAL[r2.dtype], M, K,
-          dg.data_ptr(), ws.data_ptr(), n.value, _lib.stream_handle(dev))
+          dg.data_ptr(), ws.data_ptr(), n, _lib.stream_handle(dev))
     return dx, dg
 
 
@@ -382,10 +428,9 @@ def _grad_matrix(g, dtype, K: int):
     """A gradient from autograd as a matrix of the operator's type (None stays None)."""
     if g is None:
         return None
-    g2 = g.reshape(-1, K)
-    if g2.dtype != dtype:
-        g2 = g2.to(dtype)
-    return _matrix(g2, "gradient")
+    if g.dtype != dtype:
+        g = g.to(dtype)
+    return _matrix(g if g.dim() == 2 else g.reshape(-1, K), "gradient")
 
 
 class _RMSNormFn(torch.autograd.Function):
@@ -396,14 +441,16 @@ class _RMSNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.has_res = residual is not None
         ctx.shape = x.shape
-        y = y.view(x.shape)
+        ctx.rstd = rstd
+        flat = x.dim() == 2
+        if not flat:
+            y = y.view(x.shape)
         if residual is None:
             ctx.save_for_backward(x, weight)
-            ctx.rstd = rstd
             return y
-        stream = stream.view(x.shape)
+        if not flat:
+            stream = stream.view(x.shape)
         ctx.save_for_backward(stream, weight)
-        ctx.rstd = rstd
         return y, stream
 
     @staticmethod
@@ -415,7 +462,8 @@ class _RMSNormFn(torch.autograd.Function):
             return dr, None, dr if ctx.has_res else None, None
         dx, dg = _norm_backward(_grad_matrix(dy, r.dtype, K), _matrix(r, "rms_norm"), ctx.rstd, weight.contiguous(),
                                 _grad_matrix(dr, r.dtype, K))
-        dx = dx.view(ctx.shape)
+        if dx.shape != ctx.shape:
+            dx = dx.view(ctx.shape)
         return dx, dg, dx if ctx.has_res else None, None
 
 
@@ -455,7 +503,8 @@ class APARMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(features, dtype=dtype, device=torch.device(config.device)))
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, quantize: bool = False):
-        return rms_norm(x, self.weight, residual, self.eps, quantize)
+        # nn.Module's attribute lookup takes a microsecond
+        return rms_norm(x, self._parameters["weight"], residual, self.eps, quantize)
 
     def extra_repr(self) -> str:
         return f"{self.features}, eps={self.eps}"
@@ -464,6 +513,15 @@ class APARMSNorm(nn.Module):
 # ---------------------------------------------------------------------------
 # linear layer
 # ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(M: int, N: int, K: int, flags: int, dtype: int, dw_dtype: int, device: int) -> int:
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().apa_block_linear_bwd_workspace(M, N, K, flags, dtype, dw_dtype, ctypes.addressof(n)),
+                   "apa_block_linear_bwd_workspace")
+    return n.value
+
+
 class _BlockLinearFn(torch.autograd.Function):
     """y = (norm of x + residual, or x) W^T + b with E4M3 operands; the casts
     pass gradients straight through."""
@@ -471,29 +529,37 @@ class _BlockLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, gamma, weight, bias, eps):
         ctx.set_materialize_grads(False)
-        need_in = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        need_dw = ctx.needs_input_grad[3]
+        need = ctx.needs_input_grad
+        need_in = need[0] or need[1] or need[2]
         N, K = weight.shape
-        ctx.shape, ctx.has_res, ctx.has_norm = x.shape, residual is not None, gamma is not None
-        ctx.bias_dtype = bias.dtype if bias is not None else None
-        ctx.weight_dtype = weight.dtype
-        stream = rstd = xt = None
-        if gamma is None:
-            x2 = _matrix(x, "APABlockLinear")
-            xq, xt = _cast(x2, True, need_dw and x2.shape[0] > 0)
-        else:
+        dev = x.device
+        has_norm = gamma is not None
+        if has_norm:
             x2, g, res2 = _norm_args(x, gamma, residual, "APABlockLinear")
-            xq, stream, rstd = _norm_forward(x2, g, res2, eps, True, True)
-        w2 = _matrix(weight, "APABlockLinear: weight")
-        wq, wt = _cast(w2, True, need_in, square=True)
+        else:
+            x2, g, res2 = _matrix(x, "APABlockLinear"), None, None
         M = x2.shape[0]
-        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        y = torch.empty(M, N, dtype=x.dtype, device=dev)
+        stream = torch.empty(M, K, dtype=x.dtype, device=dev) if res2 is not None else None
+        rstd = torch.empty(M, dtype=torch.float32, device=dev) if has_norm else None
+        # what the backward reads: the transposed cast of x (recomputed behind a
+        # norm) and of the weight, in one buffer
+        n_xt = (_packed_bytes(K, M) + 255) & ~255 if need[3] and not has_norm and M else 0
+        n_wt = _packed_bytes(K, N) if need_in and M else 0
+        keep = torch.empty(n_xt + n_wt, dtype=torch.uint8, device=dev) if n_xt + n_wt else None
         if M:
-            _matmul(xq, wq, bias, y, False)
-        ctx.xt, ctx.wt, ctx.rstd = xt, wt, rstd
-        ctx.M, ctx.N, ctx.K, ctx.dtype = M, N, K, x.dtype
-        y = y.view(*x.shape[:-1], N)
-        if gamma is None:
+            p = keep.data_ptr() if keep is not None else 0
+            code = _REAL[x.dtype]
+            _linear_forward(x2, code, res2, g, eps, stream, rstd, _matrix(weight, "APABlockLinear: weight"),
+                            p if n_xt else None, None, p + n_xt if n_wt else None,
+                            _vector(bias, N, dev, "APABlockLinear: bias") if bias is not None else None, y, code, M, N,
+                            K)
+        ctx.keep, ctx.n_xt, ctx.rstd = keep, n_xt, rstd
+        ctx.has_res, ctx.has_norm = residual is not None, has_norm
+        ctx.meta = (x.shape, M, N, K, x.dtype, weight.dtype, bias.dtype if bias is not None else None)
+        if y.shape[:-1] != x.shape[:-1]:
+            y = y.view(*x.shape[:-1], N)
+        if not has_norm:
             return y
         stream = x if stream is None else stream.view(x.shape)
         ctx.save_for_backward(stream, gamma)
@@ -503,48 +569,44 @@ class _BlockLinearFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dr=None):
         need = ctx.needs_input_grad
-        need_in = need[0] or need[1] or need[2]
-        M, N, K = ctx.M, ctx.N, ctx.K
+        has_norm, has_res = ctx.has_norm, ctx.has_res
         if dy is None:
-            return (dr if need[0] else None, dr if ctx.has_res and need[1] else None, None, None, None, None)
+            return (dr if need[0] else None, dr if has_res and need[1] else None, None, None, None, None)
+        shape, M, N, K, dtype, wdtype, bdtype = ctx.meta
+        need_in = need[0] or need[1] or need[2]
         dev = dy.device
-        dx = dg = dw = db = None
-        if M == 0:
-            dx = torch.zeros(ctx.shape, dtype=ctx.dtype, device=dev) if need[0] or need[1] else None
-            dg = torch.zeros(K, dtype=ctx.saved_tensors[1].dtype, device=dev) if need[2] else None
-            dw = torch.zeros(N, K, dtype=ctx.weight_dtype, device=dev) if need[3] else None
-            db = torch.zeros(N, dtype=ctx.bias_dtype, device=dev) if need[4] else None
-            return dx, dx if ctx.has_res else None, dg, dw, db, None
-        dy2 = _grad_matrix(dy, ctx.dtype, N)
-        parts = (M + 127) // 128
-        sums = torch.empty(parts, N, dtype=torch.float32, device=dev) if need[4] else None
-        dyq, dyt = _cast(dy2, need_in or not need[3], need[3], colsum=sums)
-        if need[4]:
-            db = torch.empty(N, dtype=ctx.bias_dtype, device=dev)
-            _call(dev, "apa_block_colsum", sums.data_ptr(), parts, N, db.data_ptr(), _REAL[ctx.bias_dtype],
-                  _lib.stream_handle(dev))
-        if ctx.has_norm:
+        dx = torch.empty(M, K, dtype=dtype, device=dev) if need_in else None
+        dw = torch.empty(N, K, dtype=wdtype, device=dev) if need[3] else None
+        db = torch.empty(N, dtype=bdtype, device=dev) if need[4] else None
+        dg = None
+        stream = gamma = None
+        if has_norm:
             stream, gamma = ctx.saved_tensors
-            r2, g = _matrix(stream, "APABlockLinear"), gamma.contiguous()
-        if need[3]:
-            xt = ctx.xt
-            if ctx.has_norm:
-                # the norm's output again, from the stream, with scales along the tokens
-                _, xt = _cast(r2, False, True, row_mul=ctx.rstd, col_mul=g)
-            dw = torch.empty(N, K, dtype=ctx.weight_dtype, device=dev)
-            _matmul(dyt, xt, None, dw, False)
-        if need_in:
-            # behind a norm the gradient of its output stays in fp32: rounding it
-            # would add to the rounding of dx and of dgamma's terms
-            dh = torch.empty(M, K, dtype=torch.float32 if ctx.has_norm else ctx.dtype, device=dev)
-            _matmul(dyq, ctx.wt, None, dh, False)
-            if ctx.has_norm:
-                dx, dg = _norm_backward(dh, r2, ctx.rstd, g, _grad_matrix(dr, ctx.dtype, K))
-            else:
-                dx = dh
-            dx = dx.view(ctx.shape)
-        return (dx if need[0] else None, dx if ctx.has_res and need[1] else None, dg if need[2] else None, dw, db,
-                None)
+            if need_in:
+                dg = torch.empty(K, dtype=gamma.dtype, device=dev)
+        if M:
+            dy2 = _grad_matrix(dy, dtype, N)
+            dr2 = _grad_matrix(dr, dtype, K) if has_norm and need_in else None
+            if has_norm:
+                stream, gamma = _matrix(stream, "APABlockLinear"), gamma.contiguous()
+            code, wcode = _REAL[dtype], _REAL[wdtype]
+            flags = (1 if need_in else 0) | (2 if need[3] else 0) | (4 if need[4] else 0) | (8 if has_norm else 0)
+            n = _linear_workspace(M, N, K, flags, code, wcode, dev.index)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            p = ctx.keep.data_ptr() if ctx.keep is not None else 0
+            _call(dev, "apa_block_linear_bwd", dy2.data_ptr(), code, _ld(dy2), p + ctx.n_xt if need_in else None,
+                  p if ctx.n_xt else None, _lib.ptr(stream), _ld(stream) if has_norm else 0, _lib.ptr(ctx.rstd),
+                  _lib.ptr(gamma), _REAL[gamma.dtype] if has_norm else 0, _lib.ptr(dr2),
+                  _ld(dr2) if dr2 is not None else 0, _lib.ptr(dx), code, K, _lib.ptr(dg), _lib.ptr(dw), wcode, K,
+                  _lib.ptr(db), _REAL[bdtype] if db is not None else 0, M, N, K, ws.data_ptr(), n,
+                  _lib.stream_handle(dev))
+        else:
+            for t in (dx, dw, db, dg):
+                if t is not None:
+                    t.zero_()
+        if dx is not None and dx.shape != shape:
+            dx = dx.view(shape)
+        return (dx if need[0] else None, dx if has_res and need[1] else None, dg if need[2] else None, dw, db, None)
 
 
 class APABlockLinear(nn.Module):
@@ -572,14 +634,11 @@ class APABlockLinear(nn.Module):
         self.in_features = in_features
         self.out_features = out_features
         dev = torch.device(config.device)
-        # initialised on the CPU generator and then moved, as APALinear does,
-        # so that a seed gives the same weights on every device
-        w = torch.empty(out_features, in_features)
-        nn.init.kaiming_uniform_(w, a=math.sqrt(5))
-        self.weight_master = nn.Parameter(w.to(device=dev, dtype=dtype))
+        self.weight_master = nn.Parameter(torch.empty(out_features, in_features, dtype=dtype, device=dev))
+        nn.init.kaiming_uniform_(self.weight_master, a=math.sqrt(5))
         if bias:
-            b = torch.empty(out_features).uniform_(-1 / math.sqrt(in_features), 1 / math.sqrt(in_features))
-            self.bias_master = nn.Parameter(b.to(device=dev, dtype=dtype))
+            bound = 1 / math.sqrt(in_features)
+            self.bias_master = nn.Parameter(torch.empty(out_features, dtype=dtype, device=dev).uniform_(-bound, bound))
         else:
             self.register_parameter("bias_master", None)
         self._wq: Optional[APABlockTensor] = None
@@ -593,35 +652,40 @@ class APABlockLinear(nn.Module):
         with torch.no_grad():
             q, _ = _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True)
             if self._wq is not None and self._wq.device == q.device:
-                self._wq.data.view(torch.uint8).copy_(q.data.view(torch.uint8))
-                self._wq.scales.copy_(q.scales)
+                self._wq.buffer.copy_(q.buffer)
             else:
                 self._wq = q
         self._wq_key = (W._version, W.device, W.dtype)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
-        W, b = self.weight_master, self.bias_master
+        # nn.Module's attribute lookup takes a microsecond
+        p = self._parameters
+        W, b = p["weight_master"], p["bias_master"]
         if not isinstance(x, torch.Tensor):
             raise TypeError(f"APABlockLinear: expected a tensor, got {type(x).__name__}")
-        if residual is not None and norm is None:
-            raise ValueError("APABlockLinear: residual needs norm")
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise ValueError(f"APABlockLinear: input of shape {list(x.shape)}, expected {self.in_features} features")
-        if norm is not None and norm.features != self.in_features:
-            raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
+        gamma, eps = None, 0.0
+        if norm is not None:
+            if norm.features != self.in_features:
+                raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
+            gamma, eps = norm._parameters["weight"], norm.eps
+        elif residual is not None:
+            raise ValueError("APABlockLinear: residual needs norm")
         _real(x.dtype, "APABlockLinear")
         _lib.require_cuda(x, "APABlockLinear")
         _same_device("APABlockLinear", x.device, W, residual)
-        gamma = norm.weight if norm is not None else None
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, gamma, W, b)):
-            return _BlockLinearFn.apply(x, residual, gamma, W, b, norm.eps if norm is not None else 0.0)
+        if torch.is_grad_enabled() and (W.requires_grad or x.requires_grad or (b is not None and b.requires_grad)
+                                        or (gamma is not None and gamma.requires_grad)
+                                        or (residual is not None and residual.requires_grad)):
+            return _BlockLinearFn.apply(x, residual, gamma, W, b, eps)
         if self._wq is None or self._wq_key != (W._version, W.device, W.dtype):
             self.refresh_working_copy()
         if norm is None:
             return block_linear(x, self._wq, b)
-        out = rms_norm(x.detach(), gamma.detach(), residual.detach() if residual is not None else None, norm.eps, True)
+        out = rms_norm(x.detach(), gamma.detach(), residual.detach() if residual is not None else None, eps, True)
         q = out if residual is None else out[0]
-        y = block_linear(q, self._wq, b, x.dtype).view(*x.shape[:-1], self.out_features)
+        y = block_matmul(q, self._wq, b, x.dtype).view(*x.shape[:-1], self.out_features)
         return y if residual is None else (y, out[1])
 
     def extra_repr(self) -> str:

@@ -12,3 +12,4 @@
 #include "block_cast.cu"
 #include "rmsnorm.cu"
 #include "block_gemm.cu"
+#include "block_layer.cu"

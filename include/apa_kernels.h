@@ -460,6 +460,40 @@ int apa_rmsnorm_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* r, 
                     int dtype, int64_t rows, int64_t cols, void* dgamma, void* workspace, int64_t workspace_bytes,
                     void* stream);
 
+/*
+ * Forward of a block-scaled linear layer, y[M, N] = z . w[N, K]^T + bias, in
+ * one call, where z is x, or with gamma the norm of r = x + residual
+ * (apa_rmsnorm_fwd: residual, stream_out, rstd as there). xq, xt, wq, wt are
+ * packed block tensors: codes with the row pitch cols rounded up to 16, then
+ * the scale bytes (16-byte aligned buffers). xq [M, K] receives z; xt
+ * (nullable, without gamma only) its transpose [K, M] for the weight gradient.
+ * w (F32, F16, BF16) is cast here, 128 x 128 scales, to wq [N, K] and wt
+ * (nullable) [K, N]; with w null, wq holds the cast weight already. workspace:
+ * as for apa_block_gemm.
+ */
+int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, const void* residual, int64_t ld_res,
+                         const void* gamma, int gamma_dtype, float eps, void* stream_out, int64_t ld_stream,
+                         float* rstd, void* xq, void* xt, const void* w, int w_dtype, int64_t ld_w, void* wq,
+                         void* wt, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ld_y,
+                         int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its backward: dx[M, K] (dtype), dw[N, K], db[N] from dy[M, N]; each nullable.
+ * wt: needed for dx; xt: for dw without a norm. With gamma the layer had a
+ * norm in front: r is its stream (dtype), rstd its statistics; dx is then the
+ * gradient of x and residual, dgamma (gamma_dtype, given with dx) that of
+ * gamma, and dr (nullable) the stream's own gradient, added to dx. workspace:
+ * apa_block_linear_bwd_workspace bytes, 16-byte aligned, used only during the
+ * call; flags 1 dx, 2 dw, 4 db, 8 norm in front.
+ */
+int apa_block_linear_bwd_workspace(int64_t M, int64_t N, int64_t K, int flags, int dtype, int dw_dtype,
+                                   int64_t* bytes_out);
+int apa_block_linear_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* wt, const void* xt, const void* r,
+                         int64_t ld_r, const float* rstd, const void* gamma, int gamma_dtype, const void* dr,
+                         int64_t ld_dr, void* dx, int dtype, int64_t ld_dx, void* dgamma, void* dw, int dw_dtype,
+                         int64_t ld_dw, void* db, int db_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 int apa_ladder_pack(int L, const float* const* amax_ptr, const float* const* ratio_ptr,
                     const int32_t* const* flag_ptr, int O, const float* const* oamax_ptr,
                     const int32_t* const* oflag_ptr, int32_t* packed, void* stream);
