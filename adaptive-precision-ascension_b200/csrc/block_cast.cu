@@ -13,12 +13,13 @@
 // residual stream), and the column sums of the source come along (the bias
 // gradient), per 128 rows.
 //
-// Bound by HBM: every element is read once and written once per form. One
+// Bound by HBM for fp32 sources, by the instructions of the conversion for
+// 16-bit ones: every element is read once and written once per form. One
 // 128 x 128 tile per CTA of 512 threads; a thread holds a 4 x 8 piece in
 // registers, so both forms and all maxima come from one read, and 64 registers
-// a thread leave room for two CTAs per SM (8 x 8 pieces on 256 threads, with
-// the loads of fewer warps to hide each phase's latency, ran at a third of
-// the speed).
+// a thread leave room for two CTAs per SM. (8 x 8 pieces on 256 threads ran at
+// a third of the speed; persistent CTAs with the next tile fetched ahead by
+// cp.async gained nothing in bf16 and lost a third in fp32.)
 #include "block_scale.cuh"
 
 namespace apa {
@@ -53,8 +54,10 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
   const int nc = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
   const int nr = (int)max((int64_t)0, min((int64_t)4, p.rows - row0 - lr0));
 
+  // a whole tile of aligned rows (the same for every thread)
+  const bool whole = row0 + 128 <= p.rows && col0 + 128 <= p.cols;
   float v[4][8];
-  if (p.vec_src && row0 + 128 <= p.rows && col0 + 128 <= p.cols) {
+  if (p.vec_src && whole) {
     const int64_t at = (row0 + lr0) * p.ld_src + c0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) load8<SRC>(p.src, at + i * p.ld_src, 8, true, v[i]);
@@ -70,11 +73,13 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     load8(p.col_mul, p.col_mul_dt, c0, nc, p.vec_mul && nc == 8, gm);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (i < nr) {
-        const float rs = p.row_mul[row0 + lr0 + i];
+      // elements past the edges are 0 whatever the row's statistics
+      const bool in = i < nr;
+      normed8(v[i], in ? p.row_mul[row0 + lr0 + i] : 0.0f, gm);
+      if (!whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (j < nc) v[i][j] = normed(v[i][j], rs, gm[j]);
+          if (!in || j >= nc) v[i][j] = 0.0f;
       }
     }
   }
@@ -94,44 +99,33 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     }
   }
 
-  float rm[4], cm[8];
+  float rm[4], cm[8], all;
+  auto maxima = [&]() {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float a = fmaxf(fabsf(v[i][0]), fabsf(v[i][1])), b = fmaxf(fabsf(v[i][2]), fabsf(v[i][3]));
-    a = fmaxf(a, fmaxf(fabsf(v[i][4]), fabsf(v[i][5])));
-    b = fmaxf(b, fmaxf(fabsf(v[i][6]), fabsf(v[i][7])));
-    rm[i] = fmaxf(a, b);
-  }
+    for (int i = 0; i < 4; ++i) {
+      rm[i] = max_abs(v[i][0], v[i][1], 0.0f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    cm[j] = fmaxf(fmaxf(fabsf(v[0][j]), fabsf(v[1][j])), fmaxf(fabsf(v[2][j]), fabsf(v[3][j])));
-  float all = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
-  const bool odd = is_inf(all);
-  if (odd) {
+      for (int j = 2; j < 8; j += 2) rm[i] = max_abs(v[i][j], v[i][j + 1], rm[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cm[j] = max_abs(v[2][j], v[3][j], max_abs(v[0][j], v[1][j], 0.0f));
+    all = max_abs(rm[2], rm[3], max_abs(rm[0], rm[1], 0.0f));
+  };
+  maxima();
+  if (is_inf(all)) {
     // rare: the scales come from the finite values alone
-    all = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rm[i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) cm[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float a = finite_mag(v[i][j]);
-        rm[i] = fmaxf(rm[i], a);
-        cm[j] = fmaxf(cm[j], a);
-        all = fmaxf(all, a);
-      }
+      for (int j = 0; j < 8; ++j) v[i][j] = inf_to_nan(v[i][j]);
+    maxima();
   }
-  // a thread of NaNs alone has NaN maxima
-  auto bits = [](float a) { return a == a ? __float_as_uint(a) : 0u; };
 
   const int64_t rows_pad = rows_padded(p.rows), cols_pad = rows_padded(p.cols);
   uint32_t byte_all = 0;
   float inv_all = 0.0f;
   if constexpr (SQUARE) {
-    const uint32_t w = warp_max_u32(bits(all));
+    const uint32_t w = warp_max_u32(__float_as_uint(all));
     if (lane == 0) s_max[0][warp] = __uint_as_float(w);
     __syncthreads();
     uint32_t m = __float_as_uint(s_max[0][lane & 15]);
@@ -141,7 +135,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     uint32_t m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      m[j] = bits(cm[j]);
+      m[j] = __float_as_uint(cm[j]);
       m[j] = max(m[j], __shfl_xor_sync(0xFFFFFFFFu, m[j], 16));
     }
     if (half == 0) {
@@ -164,7 +158,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       const bool b3 = lane & 8, b2 = lane & 4;
       uint32_t m[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = bits(rm[i]);
+      for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(rm[i]);
       const uint32_t a0 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[0] : m[2], 8);
       const uint32_t a1 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[1] : m[3], 8);
       const uint32_t k0 = max(b3 ? m[2] : m[0], a0), k1 = max(b3 ? m[3] : m[1], a1);
@@ -181,8 +175,11 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     }
     uint8_t* d = p.dst + (row0 + lr0) * p.ld_dst + c0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < nr && nc > 0) store_codes8(d + i * p.ld_dst, codes8(v[i], inv[i], odd), nc);
+    for (int i = 0; i < 4; ++i) {
+      const uint2 w = codes8(v[i], inv[i]);
+      if (whole) *reinterpret_cast<uint2*>(d + i * p.ld_dst) = w;
+      else if (i < nr && nc > 0) store_codes8(d + i * p.ld_dst, w, nc);
+    }
   }
 
   if (p.dst_t == nullptr && p.colsum == nullptr) return;
@@ -225,11 +222,12 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
   // neighbouring words stay together, at most with their halves exchanged.
   const int u = warp * 2 + half;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x0 = v[0][j] * inv[j], x1 = v[1][j] * inv[j], x2 = v[2][j] * inv[j], x3 = v[3][j] * inv[j];
-    s_t[(8 * g + j) * 32 + (u ^ (2 * g))] =
-        odd ? e4m3x2_exact(x0, x1) | (e4m3x2_exact(x2, x3) << 16) : e4m3x2_sat(x0, x1) | (e4m3x2_sat(x2, x3) << 16);
-  }
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) mul2(v[i][j], v[i][j + 1], inv[j], inv[j + 1], v[i][j], v[i][j + 1]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    s_t[(8 * g + j) * 32 + (u ^ (2 * g))] = e4m3x2_sat(v[0][j], v[1][j]) | (e4m3x2_sat(v[2][j], v[3][j]) << 16);
   __syncthreads();
   const int k2 = threadIdx.x & 7;                        // sixteen rows
   const int64_t gr = row0 + 16 * k2;
@@ -240,8 +238,10 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     const int cg = c >> 3;
     const uint4 x = *reinterpret_cast<const uint4*>(s_t + c * 32 + 4 * (k2 ^ (cg >> 1)));
     const uint4 w = (cg & 1) ? make_uint4(x.z, x.w, x.x, x.y) : x;
-    if (gc < p.cols && gr < p.rows) {
-      uint8_t* d = p.dst_t + gc * p.ld_dst_t + gr;
+    uint8_t* d = p.dst_t + gc * p.ld_dst_t + gr;
+    if (whole) {
+      *reinterpret_cast<uint4*>(d) = w;
+    } else if (gc < p.cols && gr < p.rows) {
       const int64_t n = p.rows - gr;
       if (n >= 16) {
         *reinterpret_cast<uint4*>(d) = w;

@@ -19,7 +19,9 @@
 //   holds the weight's rows) it is bound by reading the weight, and S CTAs per
 //   tile keep every SM's loads in flight; for a small weight gradient over
 //   many tokens the split is what fills the SMs. No workspace, no atomics: the
-//   result does not depend on timing.
+//   result does not depend on timing. For up to 16 tokens it can cast them
+//   itself (QX): every CTA casts its slabs of the few rows again, which costs
+//   less than a kernel of its own before it.
 //
 // pair_kernel  256 x 256 tiles on CTA pairs (tcgen05 cta_group::2), persistent,
 //   for everything large: bound by the tensor cores. Two accumulators of 256
@@ -162,16 +164,20 @@ template <int BN> struct SplitCfg {
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 
+// Rows of the BN side as they come, to be cast by the kernel (QX).
+struct RowArgs { const void* x; int64_t ld; int dt, vec; int64_t K; };
+
 struct SplitArgs {
   int rows_a, rows_b;       // rows of the 128 side and of the BN side
   int tiles_b;
   int kb_count;             // 128-column slabs
   int split;                // CTAs per tile (cluster size)
   int swap;                 // the 128 side is D's N
+  RowArgs rows;             // QX
   OutArgs o;
 };
 
-template <int BN>
+template <int BN, bool QX>
 __global__ void __launch_bounds__(192, 2)
     split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, SplitArgs p) {
@@ -186,7 +192,8 @@ __global__ void __launch_bounds__(192, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smS + kStages * C::kScaleBytes);
   uint64_t* empty = full + kStages;
   uint64_t* done = empty + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* cast = done + 1;               // QX: the stage's rows are cast
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cast + kStages);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / p.split, rank = blockIdx.x - tile * p.split;
   const int a0 = (tile / p.tiles_b) * BM, b0 = (tile % p.tiles_b) * BN;
@@ -198,6 +205,7 @@ __global__ void __launch_bounds__(192, 2)
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&cast[s], 128);
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -229,13 +237,14 @@ __global__ void __launch_bounds__(192, 2)
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty)) { ok = false; break; }
         const bool scales = kb == kb0 || (kb & 3) == 0;
-        mbar_expect_tx(&full[stage], C::kStageBytes + (scales ? C::kScaleBytes : 0));
+        mbar_expect_tx(&full[stage], QX ? C::kABytes + (scales ? 512 : 0)
+                                        : C::kStageBytes + (scales ? C::kScaleBytes : 0));
         tma_load_2d(smA + stage * C::kABytes, &tmA, kb * kSlab, a0, &full[stage]);
-        tma_load_2d(smB + stage * C::kBBytes, &tmB, kb * kSlab, b0, &full[stage]);
+        if constexpr (!QX) tma_load_2d(smB + stage * C::kBBytes, &tmB, kb * kSlab, b0, &full[stage]);
         if (scales) {
           uint8_t* s = smS + stage * C::kScaleBytes;
           tma_load_2d(s, &tmSA, a0, kb >> 2, &full[stage]);
-          tma_load_2d(s + 512, &tmSB, b0 & ~127, kb >> 2, &full[stage]);
+          if constexpr (!QX) tma_load_2d(s + 512, &tmSB, b0 & ~127, kb >> 2, &full[stage]);
         }
         if (++stage == kStages) { stage = 0; phase ^= 1u; }
       }
@@ -252,14 +261,15 @@ __global__ void __launch_bounds__(192, 2)
       const uint32_t sfb0 = sfb + (uint32_t)((b0 & 127) >> 5);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(&full[stage], phase, kStatusTimeoutFull)) { ok = false; break; }
+        if (QX && !mbar_wait(&cast[stage], phase, kStatusTimeoutFull)) { ok = false; break; }
         fence_after();
-        if (kb == kb0 || (kb & 3) == 0) {
-          const uint32_t s = smem_u32(smS + stage * C::kScaleBytes);
-          scale_copy<false>(sfa, s);
-          scale_copy<false>(sfb, s + 512);
-        }
+        const uint32_t s = smem_u32(smS + stage * C::kScaleBytes);
+        const bool scales = kb == kb0 || (kb & 3) == 0;
+        if (scales) scale_copy<false>(sfa, s);
+        if (QX || scales) scale_copy<false>(sfb, s + 512);
         const uint32_t j = (uint32_t)(kb & 3);
-        const uint32_t id = mx_idesc<BN, BM>() | (j << 4) | (j << 29);
+        // rows cast here have their slab's scale in byte 0
+        const uint32_t id = mx_idesc<BN, BM>() | ((QX ? 0u : j) << 4) | (j << 29);
         const uint32_t a = smem_u32(smA + stage * C::kABytes), b = smem_u32(smB + stage * C::kBBytes);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -270,6 +280,69 @@ __global__ void __launch_bounds__(192, 2)
       if (ok) gemm::mma_commit<false>(done);
     }
     __syncwarp();
+  }
+
+  if constexpr (QX) {
+    // warps 2 .. 5 cast the rows, slab by slab, into the swizzled layout that
+    // TMA would have written: sixteen threads a row, eight columns each, rows
+    // rr and rr + 8; the loads of four slabs are under way together. Rows past
+    // the last stay as they are: they make columns that nothing reads.
+    static_assert(BN == 16, "two rows per thread");
+    if (warp >= 2) {
+      const int t = threadIdx.x - 64, g = t & 15, rr = t >> 4;
+      const RowArgs& x = p.rows;
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int base = kb0; ok && base < kb1; base += 4) {
+        float v[4][2][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t c0 = (int64_t)(base + i) * kSlab + 8 * g;
+            const int n = base + i < kb1 && rr + 8 * h < p.rows_b ? (int)max((int64_t)0, min((int64_t)8, x.K - c0)) : 0;
+            load8(x.x, x.dt, (rr + 8 * h) * x.ld + c0, n, x.vec && n == 8, v[i][h]);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (base + i >= kb1) break;
+          // one lane's verdict for the warp: shuffles follow
+          bool free = true;
+          if (lane == 0) free = mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty);
+          ok = __shfl_sync(0xFFFFFFFFu, free ? 1 : 0, 0) != 0;
+          if (!ok) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (8 * h >= p.rows_b) break;             // no second row anywhere
+            float (&y)[8] = v[i][h];
+            auto top = [&]() {
+              float a = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 8; j += 2) a = max_abs(y[j], y[j + 1], a);
+              return a;
+            };
+            float a = top();
+            if (is_inf(a)) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) y[j] = inf_to_nan(y[j]);
+              a = top();
+            }
+            uint32_t m = __float_as_uint(a);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            const uint32_t b = scale_byte(m);
+            uint8_t* row = smB + stage * C::kBBytes + h * 1024 + rr * 128;
+            *reinterpret_cast<uint2*>(row + (((g >> 1) ^ rr) << 4) + (g & 1) * 8) = codes8(y, inv_scale(b));
+            if (g == 0) *reinterpret_cast<uint32_t*>(smS + stage * C::kScaleBytes + 512 + (rr + 8 * h) * 16) = b;
+          }
+          gemm::fence_async_smem();
+          gemm::mbar_arrive(&cast[stage]);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      __syncwarp();
+    }
   }
 
   // epilogue: warps 2 .. 5 read the accumulator's lane quarter warp % 4
@@ -747,39 +820,31 @@ int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Operand { const void* q; int64_t ld; const void* sc; int64_t rows; };
 
-// The dynamic shared memory limit is a property of a kernel on a device.
-template <class K>
-int allow_smem(K kernel, int bytes, unsigned long long* done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return APA_ERR_CUDA;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return APA_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return APA_ERR_CUDA;
-  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
-  return APA_OK;
-}
-
-template <int BN>
+// B's codes and scales are not read with `rows` (QX).
+template <int BN, bool QX = false>
 int launch_split(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, bool swap, int split,
-                 cudaStream_t s) {
+                 cudaStream_t s, const RowArgs& rows = RowArgs{}) {
   using C = SplitCfg<BN>;
   static unsigned long long attr = 0;
-  if (int st = allow_smem(split_kernel<BN>, C::kSmemBytes, &attr)) return st;
+  if (int st = allow_smem(split_kernel<BN, QX>, C::kSmemBytes, &attr)) return st;
   const int64_t kb = (K + kSlab - 1) / kSlab;
   CUtensorMap ta, tb, tsa, tsb;
   if (int st = code_map(&ta, A.q, A.rows, K, A.ld, BM)) return st;
-  if (int st = code_map(&tb, B.q, B.rows, K, B.ld, BN)) return st;
   if (int st = scale_map(&tsa, A.sc, A.rows, kb, 128)) return st;
-  if (int st = scale_map(&tsb, B.sc, B.rows, kb, 128)) return st;
+  tb = ta;
+  tsb = tsa;
+  if constexpr (!QX) {
+    if (int st = code_map(&tb, B.q, B.rows, K, B.ld, BN)) return st;
+    if (int st = scale_map(&tsb, B.sc, B.rows, kb, 128)) return st;
+  }
   SplitArgs p;
   p.rows_a = (int)A.rows; p.rows_b = (int)B.rows;
   p.tiles_b = (int)((B.rows + BN - 1) / BN);
-  p.kb_count = (int)kb; p.split = split; p.swap = swap ? 1 : 0; p.o = o;
+  p.kb_count = (int)kb; p.split = split; p.swap = swap ? 1 : 0; p.rows = rows; p.o = o;
   const int64_t grid = (A.rows + BM - 1) / BM * p.tiles_b * split;
   if (grid > (1ll << 31) - 1) return APA_ERR_INVALID;
-  return launch_kernel(split_kernel<BN>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmemBytes, s, split, ta, tb, tsa,
-                       tsb, p) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
+  return launch_kernel(split_kernel<BN, QX>, dim3((unsigned)grid), dim3(C::kThreads), C::kSmemBytes, s, split, ta, tb,
+                       tsa, tsb, p) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }
 
 // Output: dims {N, M}, box {128 bytes, 32 rows}, 128-byte swizzle.
@@ -995,6 +1060,18 @@ int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, 
     case 32: return launch_split<32>(x, y, K, o, p.swap, p.split, s);
     default: return launch_split<64>(x, y, K, o, p.swap, p.split, s);
   }
+}
+
+// y = x W^T for up to 16 rows that the product casts itself; false where the
+// plan is another kernel's.
+bool small_linear(const void* x, int x_dt, int64_t ld_x, const Operand& W, int64_t K, const OutArgs& o, cudaStream_t s,
+                  int* status) {
+  if (o.M > 16 || o.M > o.N) return false;
+  const BlockPlan p = block_plan(o.M, o.N, K, o.vec && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0);
+  if (p.kind != 0 || p.bn != 16 || !p.swap) return false;
+  const RowArgs rows{x, ld_x, x_dt, vec16(x, ld_x, elem_bytes(x_dt)) ? 1 : 0, K};
+  *status = launch_split<16, true>(W, Operand{nullptr, 0, nullptr, o.M}, K, o, true, p.split, s, rows);
+  return true;
 }
 
 }  // namespace blk

@@ -90,6 +90,12 @@ extern "C" int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, co
   if (ld_x < K || (w && ld_w < K) || ld_y < N) return APA_ERR_INVALID;
   const Packed X(xq, M, K), XT(xt, K, M), W(wq, N, K), WT(wt, K, N);
   int st;
+  if (!gamma && !xt && !w && M <= 16) {
+    // a few tokens through a kept weight: the product casts them itself
+    const OutArgs o{y, ld_y, y_dtype, bias, bias_dtype, 0, vec16(y, ld_y, elem_bytes(y_dtype)) ? 1 : 0, (int)M, (int)N};
+    if (small_linear(x, x_dtype, ld_x, Operand{W.q, W.ld, W.sc, N}, K, o, static_cast<cudaStream_t>(stream), &st))
+      return st;
+  }
   if (gamma)
     st = apa_rmsnorm_fwd(x, ld_x, residual, ld_res, gamma, gamma_dtype, x_dtype, M, K, eps, stream_out, ld_stream,
                          nullptr, 0, X.q, X.ld, X.sc, rstd, stream);

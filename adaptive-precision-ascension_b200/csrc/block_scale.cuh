@@ -55,28 +55,51 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
   return __uint_as_float(b == 0u ? 0x00400000u : b << 23);
 }
 
-// max of magnitudes (fp32 bits) that skips NaN and Inf. Kernels take the plain
-// maximum first (fmaxf skips NaN) and come here only when that is infinite.
-__device__ __forceinline__ float finite_mag(float v) {
-  const float a = fabsf(v);
-  return a < __uint_as_float(0x7F800000u) ? a : 0.0f;
+// m = max(m, |a|, |b|). NaN operands are skipped, so a maximum that starts at 0
+// is a number; an infinity shows in it.
+__device__ __forceinline__ float max_abs(float a, float b, float m) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(m));
+  return r;
 }
 
 __device__ __forceinline__ bool is_inf(float a) { return __float_as_uint(a) == 0x7F800000u; }
 
-// Scaled values -> codes. Finite values are at most 448 in magnitude after
-// scaling, where the saturating conversion rounds to nearest even like the
-// exact one, and it maps NaN to NaN. Only an infinity needs the exact rule (NaN;
-// E4M3 has no infinity): odd says that the thread holds one.
+// Infinities become NaN: E4M3 has no infinity, and the scale comes from the
+// finite values. After this the saturating conversion gives the right codes:
+// finite values are at most 448 in magnitude after scaling, where it rounds to
+// nearest even, and it maps NaN to NaN.
+__device__ __forceinline__ float inf_to_nan(float v) {
+  return is_inf(fabsf(v)) ? __uint_as_float(0x7FC00000u) : v;
+}
+
+// Two products (or sums) per instruction, each rounded as the scalar one is.
+__device__ __forceinline__ void mul2(float a0, float a1, float b0, float b1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2(float a0, float a1, float b0, float b1, float c0, float c1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
 
 // r * rstd * g with one rounding: the product r g is split into its rounded
 // value and the exact remainder, and the last product is a fused one. A value
 // next to a border of the E4M3 grid then lands on the side the exact product
 // is on unless rstd's own rounding moves it.
-__device__ __forceinline__ float normed(float r, float rstd, float g) {
-  const float t = __fmul_rn(r, g);
-  const float e = __fmaf_rn(r, g, -t);
-  return __fmaf_rn(t, rstd, __fmul_rn(e, rstd));
+__device__ __forceinline__ void normed8(float (&v)[8], float rstd, const float (&g)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    float t0, t1, e0, e1;
+    mul2(v[j], v[j + 1], g[j], g[j + 1], t0, t1);
+    fma2(v[j], v[j + 1], g[j], g[j + 1], -t0, -t1, e0, e1);
+    mul2(e0, e1, rstd, rstd, e0, e1);
+    fma2(t0, t1, rstd, rstd, e0, e1, v[j], v[j + 1]);
+  }
 }
 
 template <int DT>
@@ -109,13 +132,6 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-
-template <int DT>
-__device__ __forceinline__ float round_to(float v) {
-  if constexpr (DT == APA_DT_F16) return f16_to_f32(f16_from_f32(v));
-  else if constexpr (DT == APA_DT_BF16) return bf16_to_f32(bf16_from_f32(v));
-  else return v;
 }
 
 // Eight 16-bit elements -> fp32.
@@ -160,17 +176,23 @@ __device__ __forceinline__ void load8(const void* p, int dt, int64_t i, int n, b
   else load8<APA_DT_BF16>(p, i, n, vec, v);
 }
 
-// Eight scaled values -> eight codes.
-__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s, bool odd) {
-  uint2 w;
-  if (!odd) {
-    w.x = e4m3x2_sat(v[0] * s, v[1] * s) | (e4m3x2_sat(v[2] * s, v[3] * s) << 16);
-    w.y = e4m3x2_sat(v[4] * s, v[5] * s) | (e4m3x2_sat(v[6] * s, v[7] * s) << 16);
-  } else {
-    w.x = e4m3x2_exact(v[0] * s, v[1] * s) | (e4m3x2_exact(v[2] * s, v[3] * s) << 16);
-    w.y = e4m3x2_exact(v[4] * s, v[5] * s) | (e4m3x2_exact(v[6] * s, v[7] * s) << 16);
-  }
-  return w;
+// Eight values times s -> eight codes (inf_to_nan first where there may be one).
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float s) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) mul2(v[j], v[j + 1], s, s, a[j], a[j + 1]);
+  return make_uint2(e4m3x2_sat(a[0], a[1]) | (e4m3x2_sat(a[2], a[3]) << 16),
+                    e4m3x2_sat(a[4], a[5]) | (e4m3x2_sat(a[6], a[7]) << 16));
+}
+
+// Eight fp32 values -> eight 16-bit elements.
+template <int DT>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    w[j] = DT == APA_DT_BF16 ? bf16x2(v[2 * j], v[2 * j + 1]) : f16x2_from_f32(v[2 * j], v[2 * j + 1]);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <int DT>
@@ -181,11 +203,7 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int n, bool vec, cons
       d[0] = make_float4(v[0], v[1], v[2], v[3]);
       d[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = DT == APA_DT_BF16 ? bf16x2(v[2 * j], v[2 * j + 1]) : f16x2_from_f32(v[2 * j], v[2 * j + 1]);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = pack8<DT>(v);
     }
   } else {
 #pragma unroll
@@ -202,6 +220,27 @@ __device__ __forceinline__ void store_codes8(uint8_t* d, uint2 w, int n) {
     const uint64_t b = ((uint64_t)w.y << 32) | w.x;
     for (int j = 0; j < n; ++j) d[j] = (uint8_t)(b >> (8 * j));
   }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Raises a kernel's dynamic shared memory limit, which is a property of the
+// kernel on a device: `done` holds a bit per device.
+template <class K>
+int allow_smem(K kernel, int bytes, unsigned long long* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return APA_ERR_CUDA;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return APA_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return APA_ERR_CUDA;
+  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
+  return APA_OK;
 }
 
 inline int elem_bytes(int dt) { return dt == APA_DT_F32 ? 4 : dt == APA_DT_F16 || dt == APA_DT_BF16 ? 2 : 0; }

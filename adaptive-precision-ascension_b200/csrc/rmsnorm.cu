@@ -72,13 +72,6 @@ __device__ __forceinline__ float rsqrt_refined(float a) {
   return __fmaf_rn(0.5f * y, e, y);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <int DT> constexpr int pieces() { return DT == APA_DT_F32 ? 2 : 1; }   // 16-byte pieces per chunk
 
 // The chunks of one thread in one row, in planes of 16 bytes per thread (so a
@@ -182,14 +175,21 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
         float u[8];
         chunk8<DT, TPR, ASYNC>(at + C::kArray, i, p.res, row * p.ld_res + c0, n, p.vec_res, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = round_to<DT>(v[i][j] + u[j]);
-        if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, v[i]);
+        for (int j = 0; j < 8; ++j) v[i][j] += u[j];
+        if constexpr (DT == APA_DT_F32) {
+          if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, v[i]);
+        } else {
+          const uint4 w = pack8<DT>(v[i]);
+          unpack8<DT>(w, v[i]);
+          if (p.vec_r && n == 8) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.r) + row * p.ld_r + c0) = w;
+          else if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, false, v[i]);
+        }
       }
-      // pairwise: eight squares, then the thread's chunks, then the threads
-      float q[8];
+      // squares in two chains per chunk, then the chunks, then the threads
+      float q0 = 0.0f, q1 = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = v[i][j] * v[i][j];
-      ss += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+      for (int j = 0; j < 8; j += 2) fma2(v[i][j], v[i][j + 1], v[i][j], v[i][j + 1], q0, q1, q0, q1);
+      ss += q0 + q1;
     }
     ss = row_sum<TPR>(ss, s_red);
     const float rstd = rsqrt_refined(ss / (float)p.cols + p.eps);
@@ -198,10 +198,10 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
     for (int i = 0; i < NV; ++i) {
       const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
       const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-      float y[8], gm[8];
+      float gm[8];
       load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm);     // in L1 after the first row
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = normed(v[i][j], rstd, gm[j]);
+      float (&y)[8] = v[i];
+      normed8(y, rstd, gm);
       if (n < 8) {
         // columns past the end are 0 whatever the row's statistics
 #pragma unroll
@@ -209,21 +209,24 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
           if (j >= n) y[j] = 0.0f;
       }
       if constexpr (QUANT) {
-        float a = fabsf(y[0]);
+        auto top = [&]() {
+          float a = 0.0f;
 #pragma unroll
-        for (int j = 1; j < 8; ++j) a = fmaxf(a, fabsf(y[j]));
-        const bool odd = is_inf(a);
-        if (odd) {
-          a = 0.0f;
+          for (int j = 0; j < 8; j += 2) a = max_abs(y[j], y[j + 1], a);
+          return a;
+        };
+        float a = top();
+        if (is_inf(a)) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a = fmaxf(a, finite_mag(y[j]));
+          for (int j = 0; j < 8; ++j) y[j] = inf_to_nan(y[j]);
+          a = top();
         }
-        uint32_t m = a == a ? __float_as_uint(a) : 0u;     // all NaN: no scale
+        uint32_t m = __float_as_uint(a);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         const uint32_t b = scale_byte(m);
         if (n > 0) {
-          store_codes8(p.q + row * p.ld_q + c0, codes8(y, inv_scale(b), odd), n);
+          store_codes8(p.q + row * p.ld_q + c0, codes8(y, inv_scale(b)), n);
           if ((t & 15) == 0) p.sc[scale_offset(rows_pad, row, c0 >> 7)] = (uint8_t)b;
         }
       } else {
@@ -363,20 +366,6 @@ __global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(Nor
 
 constexpr int64_t kMaxNormCols = 32768;   // 1024 threads x 4 chunks of eight
 
-// Kernels whose row buffers pass 48 KB need the limit raised, per device.
-template <class K>
-int norm_smem(K kernel, int bytes, unsigned long long* done) {
-  if (bytes <= 47 * 1024) return APA_OK;      // static shared memory counts too
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return APA_ERR_CUDA;
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (__atomic_load_n(done, __ATOMIC_ACQUIRE) & bit) return APA_OK;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return APA_ERR_CUDA;
-  __atomic_fetch_or(done, bit, __ATOMIC_RELEASE);
-  return APA_OK;
-}
-
 // CTAs per SM: as many as the threads and the row buffers allow.
 int64_t norm_per_sm(int threads, int smem, int most) {
   return std::max<int64_t>(1, std::min<int64_t>(std::min(2048 / threads, most), 220 * 1024 / (smem + 1024)));
@@ -387,7 +376,7 @@ int launch_norm_k(const NormArgs& a, cudaStream_t s) {
   using C = NormCfg<DT, TPR, NV>;
   constexpr int kSmem = ASYNC ? C::kDepth * C::kSlot : 0;
   static unsigned long long attr = 0;
-  if (int st = norm_smem(rmsnorm_kernel<DT, TPR, NV, QUANT, ASYNC>, kSmem, &attr)) return st;
+  if (int st = allow_smem(rmsnorm_kernel<DT, TPR, NV, QUANT, ASYNC>, kSmem, &attr)) return st;
   // at most 1024 threads' worth of registers (64 each)
   const int64_t most = norm_per_sm(C::kThreads, kSmem, 1024 / C::kThreads) * num_sms();
   const int64_t all = (a.rows + C::kRows - 1) / C::kRows;
@@ -436,7 +425,7 @@ int launch_norm_bwd_k(const NormBwdArgs& a, int64_t parts, cudaStream_t s) {
   using C = NormBwdCfg<DT, DY, TPR, NV>;
   constexpr int kSmem = (ASYNC ? C::kDepth * C::kSlot : 0) + C::kSums;
   static unsigned long long attr = 0;
-  if (int st = norm_smem(rmsnorm_bwd_kernel<DT, DY, TPR, NV, ASYNC>, kSmem, &attr)) return st;
+  if (int st = allow_smem(rmsnorm_bwd_kernel<DT, DY, TPR, NV, ASYNC>, kSmem, &attr)) return st;
   return launch_kernel(rmsnorm_bwd_kernel<DT, DY, TPR, NV, ASYNC>, dim3((unsigned)parts), dim3(C::kThreads), kSmem, s,
                        1, a) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }

@@ -465,7 +465,7 @@ int apa_rmsnorm_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* r, 
  * one call, where z is x, or with gamma the norm of r = x + residual
  * (apa_rmsnorm_fwd: residual, stream_out, rstd as there). xq, xt, wq, wt are
  * packed block tensors: codes with the row pitch cols rounded up to 16, then
- * the scale bytes (16-byte aligned buffers). xq [M, K] receives z; xt
+ * the scale bytes (16-byte aligned buffers). xq [M, K] is room for z; xt
  * (nullable, without gamma only) its transpose [K, M] for the weight gradient.
  * w (F32, F16, BF16) is cast here, 128 x 128 scales, to wq [N, K] and wt
  * (nullable) [K, N]; with w null, wq holds the cast weight already. workspace:

@@ -389,3 +389,20 @@ def test_long_reductions(plan, n):
     blockscale._matmul(a, b, None, out, False, plan)
     want = a.dequantize().double() @ b.dequantize().double().t()
     assert float((out - want).norm() / want.norm()) < 1e-6
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("n,k", [(64, 100), (300, 128), (513, 1157), (4096, 1024), (260, 4096)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens(m, n, k, dtype):
+    """Up to 16 tokens are cast inside the product: the same bits as cast and product apart."""
+    x, w, b = rnd((m, k), m + k, dtype).cuda(), rnd((n, k), 2).cuda(), rnd((n, 1), 3)[:, 0].cuda()
+    wq = block_cast(w, square=True)
+    y = block_linear(x, wq, b, out_dtype=torch.float32)
+    assert torch.equal(y, block_matmul(block_cast(x), wq, b, out_dtype=torch.float32))
+    wide = torch.full((m, k + 9), 3.0, dtype=dtype, device="cuda")
+    wide[:, 5:5 + k] = x
+    assert torch.equal(block_linear(wide[:, 5:5 + k], wq, b, out_dtype=torch.float32), y)
+    x[0, k // 2] = float("inf")
+    z = block_linear(x, wq, b, out_dtype=torch.float32)
+    assert bool(torch.isnan(z[0]).all()) and torch.equal(z[1:], y[1:])
