@@ -62,8 +62,9 @@ SIGNATURES = {
     "apa_block_gemm": [_VP, _I64, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _I, _I, _VP,
                        _I64, _VP],
     "apa_block_gemm_workspace": [_I64, _I64, _I64, _I, _I, _VP],
-    "apa_block_linear_fwd": [_VP, _I, _I64, _VP, _I64, _VP, _I, _F, _VP, _I64, _VP, _VP, _VP, _VP, _I, _I64, _VP, _VP,
-                             _VP, _I, _VP, _I, _I64, _I64, _I64, _I64, _VP, _I64, _VP],
+    "apa_block_linear_fwd_workspace": [_I64, _I64, _I64, _I, _I, _VP],
+    "apa_block_linear_fwd": [_VP, _I, _I64, _VP, _I64, _VP, _I, _F, _VP, _I64, _VP, _VP, _VP, _I, _I64, _VP, _VP, _VP,
+                             _I, _VP, _I, _I64, _I64, _I64, _I64, _VP, _I64, _VP],
     "apa_block_linear_bwd_workspace": [_I64, _I64, _I64, _I, _I, _I, _VP],
     "apa_block_linear_bwd": [_VP, _I, _I64, _VP, _VP, _VP, _I64, _VP, _VP, _I, _VP, _I64, _VP, _I, _I64, _VP, _VP, _I,
                              _I64, _VP, _I, _I64, _I64, _I64, _VP, _I64, _VP],

@@ -340,22 +340,29 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
+@functools.lru_cache(maxsize=4096)
+def _forward_workspace(M: int, N: int, K: int, flags: int, dtype: int, device: int) -> int:
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().apa_block_linear_fwd_workspace(M, N, K, flags, dtype, ctypes.addressof(n)),
+                   "apa_block_linear_fwd_workspace")
+    return n.value
+
+
 def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bias, y, out_code, M, N, K) -> None:
-    """apa_block_linear_fwd with its temporaries in one buffer. xt, wq, wt:
-    addresses of packed block tensors; wq None: the weight w2 is cast into the
-    temporary buffer too."""
+    """apa_block_linear_fwd with its temporaries in one buffer. The weight is
+    w2, or wq, the address of its packed cast; xt, wt: addresses for the
+    transposed casts."""
     dev = x2.device
-    n = _matmul_workspace(M, N, K, out_code, 0, dev.index)
-    at_w = (_packed_bytes(M, K) + 255) & ~255
-    at_ws = at_w + ((_packed_bytes(N, K) + 255) & ~255 if wq is None else 0)
-    tmp = torch.empty(at_ws + n, dtype=torch.uint8, device=dev)
-    p = tmp.data_ptr()
+    flags = (0 if w2 is None else 1) | (0 if gamma is None else 2) | (0 if xt is None else 4)
+    n = _forward_workspace(M, N, K, flags, out_code, dev.index)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     _call(dev, "apa_block_linear_fwd", x2.data_ptr(), code, _ld(x2),
           _lib.ptr(res2), _ld(res2) if res2 is not None else 0,
           _lib.ptr(gamma), _REAL[gamma.dtype] if gamma is not None else 0, eps, _lib.ptr(stream), K, _lib.ptr(rstd),
-          p, xt, _lib.ptr(w2), _REAL[w2.dtype] if w2 is not None else 0, _ld(w2) if w2 is not None else 0,
-          p + at_w if wq is None else wq, wt, _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0,
-          y.data_ptr(), out_code, N, M, N, K, p + at_ws, n, _lib.stream_handle(dev))
+          xt, _lib.ptr(w2), _REAL[w2.dtype] if w2 is not None else 0, _ld(w2) if w2 is not None else 0, wq, wt,
+          _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, y.data_ptr(), out_code, N, M, N, K,
+          _lib.ptr(ws), n, _lib.stream_handle(dev))
 
 
 # ---------------------------------------------------------------------------
@@ -433,6 +440,19 @@ def _grad_matrix(g, dtype, K: int):
     return _matrix(g if g.dim() == 2 else g.reshape(-1, K), "gradient")
 
 
+def _first_order(fn):
+    """A backward without a second derivative. torch's decorator costs two
+    microseconds a call, so it is used only where a graph of the gradient is
+    being built."""
+    graphed = once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def backward(ctx, *grads):
+        return graphed(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return backward
+
+
 class _RMSNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
@@ -454,7 +474,7 @@ class _RMSNormFn(torch.autograd.Function):
         return y, stream
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dr=None):
         r, weight = ctx.saved_tensors
         K = weight.shape[0]
@@ -566,7 +586,7 @@ class _BlockLinearFn(torch.autograd.Function):
         return (y, stream) if residual is not None else y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dr=None):
         need = ctx.needs_input_grad
         has_norm, has_res = ctx.has_norm, ctx.has_res

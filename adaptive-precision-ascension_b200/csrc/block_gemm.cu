@@ -1062,16 +1062,11 @@ int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, 
   }
 }
 
-// y = x W^T for up to 16 rows that the product casts itself; false where the
-// plan is another kernel's.
-bool small_linear(const void* x, int x_dt, int64_t ld_x, const Operand& W, int64_t K, const OutArgs& o, cudaStream_t s,
-                  int* status) {
-  if (o.M > 16 || o.M > o.N) return false;
+// y = x W^T for up to 16 rows that the product casts itself.
+int small_linear(const void* x, int x_dt, int64_t ld_x, const Operand& W, int64_t K, const OutArgs& o, cudaStream_t s) {
   const BlockPlan p = block_plan(o.M, o.N, K, o.vec && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0);
-  if (p.kind != 0 || p.bn != 16 || !p.swap) return false;
   const RowArgs rows{x, ld_x, x_dt, vec16(x, ld_x, elem_bytes(x_dt)) ? 1 : 0, K};
-  *status = launch_split<16, true>(W, Operand{nullptr, 0, nullptr, o.M}, K, o, true, p.split, s, rows);
-  return true;
+  return launch_split<16, true>(W, Operand{nullptr, 0, nullptr, o.M}, K, o, true, p.split, s, rows);
 }
 
 }  // namespace blk

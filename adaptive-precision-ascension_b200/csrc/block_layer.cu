@@ -26,10 +26,38 @@ struct Packed {
       : q(static_cast<uint8_t*>(const_cast<void*>(base))), ld(pitch16(cols)), sc(q ? q + rows * ld : nullptr) {}
 };
 
-// Workspace of the backward, in the order it is used.
+// Workspaces, in the order they are used.
+struct FwdSpace { int64_t xq, wq, gemm, gemm_bytes, total; };
 struct BwdSpace {
   int64_t dyq, dyt, xt, sums, dh, norm, gemm, norm_bytes, gemm_bytes, total;
 };
+
+// A few tokens through a kept weight: the product casts them itself.
+bool casts_itself(int64_t M, int64_t N, int64_t K, int flags, bool aligned) {
+  if (flags != 0 || M > 16) return false;
+  const BlockPlan p = block_plan(M, N, K, aligned);
+  return p.kind == 0 && p.bn == 16 && p.swap;
+}
+
+// flags: 1 the weight is cast, 2 a norm in front, 4 the transposed cast of x too
+int fwd_space(int64_t M, int64_t N, int64_t K, int flags, int y_dtype, FwdSpace* s) {
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += round256(bytes);
+    return here;
+  };
+  // whether y's rows are aligned is known only in the call: room for both
+  const bool itself = casts_itself(M, N, K, flags, true) && casts_itself(M, N, K, flags, false);
+  s->xq = take(itself ? 0 : packed_bytes(M, K));
+  s->wq = take((flags & 1) ? packed_bytes(N, K) : 0);
+  s->gemm_bytes = 0;
+  if (!itself)
+    if (int st = apa_block_gemm_workspace(M, N, K, y_dtype, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
+  s->gemm = take(s->gemm_bytes);
+  s->total = at;
+  return APA_OK;
+}
 
 enum { kWantDx = 1, kWantDw = 2, kWantDb = 4, kNorm = 8 };
 
@@ -71,31 +99,48 @@ bool aligned_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) =
 }  // namespace blk
 }  // namespace apa
 
+extern "C" int apa_block_linear_fwd_workspace(int64_t M, int64_t N, int64_t K, int flags, int y_dtype,
+                                              int64_t* bytes_out) {
+  using namespace apa::blk;
+  if (!bytes_out || (flags & ~7) != 0) return APA_ERR_INVALID;
+  if (int st = layer_dims(M, N, K)) return st;
+  if (elem_bytes(y_dtype) == 0) return APA_ERR_UNSUPPORTED;
+  FwdSpace s;
+  if (int st = fwd_space(M, N, K, flags, y_dtype, &s)) return st;
+  *bytes_out = s.total;
+  return APA_OK;
+}
+
 extern "C" int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, const void* residual, int64_t ld_res,
                                     const void* gamma, int gamma_dtype, float eps, void* stream_out, int64_t ld_stream,
-                                    float* rstd, void* xq, void* xt, const void* w, int w_dtype, int64_t ld_w, void* wq,
+                                    float* rstd, void* xt, const void* w, int w_dtype, int64_t ld_w, const void* wq,
                                     void* wt, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ld_y,
                                     int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                                     void* stream) {
   using namespace apa::blk;
   if (int st = layer_dims(M, N, K)) return st;
-  if (!x || !xq || !wq || !y) return APA_ERR_INVALID;
+  if (!x || !y || (w == nullptr) == (wq == nullptr)) return APA_ERR_INVALID;
   if (!gamma && (residual || stream_out || rstd)) return APA_ERR_INVALID;
   if ((gamma && xt) || (!w && wt)) return APA_ERR_INVALID;
-  if (!aligned_16(xq) || !aligned_16(xt) || !aligned_16(wq) || !aligned_16(wt)) return APA_ERR_ALIGN;
+  if (!aligned_16(workspace) || !aligned_16(xt) || !aligned_16(wq) || !aligned_16(wt)) return APA_ERR_ALIGN;
   // all refusals come before the first launch
-  if (elem_bytes(x_dtype) == 0 || elem_bytes(y_dtype) == 0 || (w && elem_bytes(w_dtype) == 0) ||
-      (bias && elem_bytes(bias_dtype) == 0) || (gamma && elem_bytes(gamma_dtype) == 0))
+  const int es = elem_bytes(y_dtype);
+  if (elem_bytes(x_dtype) == 0 || es == 0 || (w && elem_bytes(w_dtype) == 0) || (bias && elem_bytes(bias_dtype) == 0) ||
+      (gamma && elem_bytes(gamma_dtype) == 0))
     return APA_ERR_UNSUPPORTED;
   if (ld_x < K || (w && ld_w < K) || ld_y < N) return APA_ERR_INVALID;
-  const Packed X(xq, M, K), XT(xt, K, M), W(wq, N, K), WT(wt, K, N);
-  int st;
-  if (!gamma && !xt && !w && M <= 16) {
-    // a few tokens through a kept weight: the product casts them itself
-    const OutArgs o{y, ld_y, y_dtype, bias, bias_dtype, 0, vec16(y, ld_y, elem_bytes(y_dtype)) ? 1 : 0, (int)M, (int)N};
-    if (small_linear(x, x_dtype, ld_x, Operand{W.q, W.ld, W.sc, N}, K, o, static_cast<cudaStream_t>(stream), &st))
-      return st;
+  const int flags = (w ? 1 : 0) | (gamma ? 2 : 0) | (xt ? 4 : 0);
+  FwdSpace f;
+  if (int st = fwd_space(M, N, K, flags, y_dtype, &f)) return st;
+  if (workspace_bytes < f.total || (f.total > 0 && !workspace)) return APA_ERR_INVALID;
+  char* ws = static_cast<char*>(workspace);
+  const OutArgs o{y, ld_y, y_dtype, bias, bias_dtype, 0, vec16(y, ld_y, es) ? 1 : 0, (int)M, (int)N};
+  if (casts_itself(M, N, K, flags, o.vec && (N * es) % 16 == 0)) {
+    const Packed W(wq, N, K);
+    return small_linear(x, x_dtype, ld_x, Operand{W.q, W.ld, W.sc, N}, K, o, static_cast<cudaStream_t>(stream));
   }
+  const Packed X(ws + f.xq, M, K), XT(xt, K, M), W(w ? ws + f.wq : wq, N, K), WT(wt, K, N);
+  int st;
   if (gamma)
     st = apa_rmsnorm_fwd(x, ld_x, residual, ld_res, gamma, gamma_dtype, x_dtype, M, K, eps, stream_out, ld_stream,
                          nullptr, 0, X.q, X.ld, X.sc, rstd, stream);
@@ -109,7 +154,7 @@ extern "C" int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, co
     if (st) return st;
   }
   return apa_block_gemm(X.q, X.ld, X.sc, W.q, W.ld, W.sc, bias, bias_dtype, y, y_dtype, ld_y, M, N, K, 0,
-                        APA_BLOCK_AUTO, workspace, workspace_bytes, stream);
+                        APA_BLOCK_AUTO, ws + f.gemm, f.gemm_bytes, stream);
 }
 
 extern "C" int apa_block_linear_bwd_workspace(int64_t M, int64_t N, int64_t K, int flags, int dtype, int dw_dtype,

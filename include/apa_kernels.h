@@ -463,19 +463,21 @@ int apa_rmsnorm_bwd(const void* dy, int dy_dtype, int64_t ld_dy, const void* r, 
 /*
  * Forward of a block-scaled linear layer, y[M, N] = z . w[N, K]^T + bias, in
  * one call, where z is x, or with gamma the norm of r = x + residual
- * (apa_rmsnorm_fwd: residual, stream_out, rstd as there). xq, xt, wq, wt are
- * packed block tensors: codes with the row pitch cols rounded up to 16, then
- * the scale bytes (16-byte aligned buffers). xq [M, K] is room for z; xt
- * (nullable, without gamma only) its transpose [K, M] for the weight gradient.
- * w (F32, F16, BF16) is cast here, 128 x 128 scales, to wq [N, K] and wt
- * (nullable) [K, N]; with w null, wq holds the cast weight already. workspace:
- * as for apa_block_gemm.
+ * (apa_rmsnorm_fwd: residual, stream_out, rstd as there). xt, wq, wt are packed
+ * block tensors: codes with the row pitch cols rounded up to 16, then the scale
+ * bytes, in 16-byte aligned buffers. The weight is w (F32, F16, BF16), cast
+ * here with 128 x 128 scales, or wq [N, K], cast before. xt (nullable, without
+ * gamma only) and wt (nullable, with w) receive the transposed casts [K, M] and
+ * [K, N], which the backward reads. workspace: apa_block_linear_fwd_workspace
+ * bytes (may be 0), 16-byte aligned, used only during the call; flags 1 the
+ * weight is w, 2 gamma, 4 xt.
  */
+int apa_block_linear_fwd_workspace(int64_t M, int64_t N, int64_t K, int flags, int y_dtype, int64_t* bytes_out);
 int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, const void* residual, int64_t ld_res,
                          const void* gamma, int gamma_dtype, float eps, void* stream_out, int64_t ld_stream,
-                         float* rstd, void* xq, void* xt, const void* w, int w_dtype, int64_t ld_w, void* wq,
-                         void* wt, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ld_y,
-                         int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+                         float* rstd, void* xt, const void* w, int w_dtype, int64_t ld_w, const void* wq, void* wt,
+                         const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ld_y, int64_t M, int64_t N,
+                         int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Its backward: dx[M, K] (dtype), dw[N, K], db[N] from dy[M, N]; each nullable.

@@ -281,3 +281,13 @@ def test_chain_serving_equals_modules():
         u = apa.block_linear(apa.block_linear(q, w1), w2)
         v, s2 = rms_norm(u, n2.weight.detach(), s1)
         assert torch.equal(v, z) and torch.equal(s1, r1) and torch.equal(s2, r2)
+
+
+def test_second_derivatives_are_refused():
+    lin = layer(rnd((40, 64), 1))
+    x = rnd((9, 64), 3).cuda().requires_grad_(True)
+    norm = APARMSNorm(64, config=APAConfig(device="cuda"))
+    for out in (lin(x), norm(x), lin(x, norm=norm)):
+        (g,) = torch.autograd.grad(out.sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError):          # no gradient of it, or none a second time
+            g.sum().backward()
