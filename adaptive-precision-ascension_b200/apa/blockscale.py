@@ -662,7 +662,7 @@ class APABlockLinear(nn.Module):
         else:
             self.register_parameter("bias_master", None)
         self._wq: Optional[APABlockTensor] = None
-        self._wq_key: Optional[Tuple] = None
+        self._wq_key: Optional[Tuple] = None       # the parameter that _wq was cast from, and its state then
 
     def refresh_working_copy(self) -> None:
         """Cast the weight for calls without gradients (buffers are kept, so a
@@ -675,7 +675,12 @@ class APABlockLinear(nn.Module):
                 self._wq.buffer.copy_(q.buffer)
             else:
                 self._wq = q
-        self._wq_key = (W._version, W.device, W.dtype)
+        self._wq_key = (W, self._state(W))
+
+    @staticmethod
+    def _state(W: torch.Tensor) -> Tuple:
+        # tensors made in inference mode have no version; they cannot change in place outside it
+        return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
         # nn.Module's attribute lookup takes a microsecond
@@ -699,7 +704,8 @@ class APABlockLinear(nn.Module):
                                         or (gamma is not None and gamma.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
             return _BlockLinearFn.apply(x, residual, gamma, W, b, eps)
-        if self._wq is None or self._wq_key != (W._version, W.device, W.dtype):
+        key = self._wq_key
+        if key is None or key[0] is not W or key[1] != self._state(W):
             self.refresh_working_copy()
         if norm is None:
             return block_linear(x, self._wq, b)

@@ -13,7 +13,7 @@
 // residual stream), and the column sums of the source come along (the bias
 // gradient), per 128 rows.
 //
-// Bound by HBM for fp32 sources, by the instructions of the conversion for
+// Bound by HBM for fp32 sources, by the conversion's instructions (ALU pipe) for
 // 16-bit ones: every element is read once and written once per form. One
 // 128 x 128 tile per CTA of 512 threads; a thread holds a 4 x 8 piece in
 // registers, so both forms and all maxima come from one read, and 64 registers
@@ -37,18 +37,21 @@ struct CastArgs {
 
 constexpr int kCastThreads = 512;
 
-template <int SRC, bool SQUARE>
-__global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p) {
-  __shared__ __align__(16) uint32_t s_t[128 * 32];       // transposed codes, 128 bytes per column
-  __shared__ __align__(16) float s_max[16][128];
-  __shared__ __align__(16) float s_sum[16][128];
-  __shared__ __align__(16) float s_inv[128];
-  pdl_launch_dependents();
-  pdl_wait();
+struct CastShared {
+  uint32_t t[128 * 32];          // transposed codes, 128 bytes per column
+  float max[16][128];            // column maxima per warp
+  float sum[16][128];
+  float inv[128];
+};
+
+// One 128 x 128 tile. NORM: the source is src * row_mul * col_mul. (Maxima of
+// 16-bit sources on packed pairs, half the instructions, were no faster.)
+template <int SRC, bool SQUARE, bool NORM>
+__device__ __forceinline__ void cast_tile(const CastArgs& p, int64_t tile, CastShared& sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane & 15, half = lane >> 4;            // columns 8 g .. 8 g + 7
   const int lr0 = warp * 8 + half * 4;                  // rows lr0 .. lr0 + 3
-  const int64_t tile_r = blockIdx.x / p.tiles_c, tile_c = blockIdx.x - tile_r * p.tiles_c;
+  const int64_t tile_r = tile / p.tiles_c, tile_c = tile - tile_r * p.tiles_c;
   const int64_t row0 = tile_r * 128, col0 = tile_c * 128;
   const int64_t c0 = col0 + 8 * g;
   const int nc = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       load8<SRC>(p.src, (row0 + lr0 + i) * p.ld_src + c0, n, p.vec_src && n == 8, v[i]);
     }
   }
-  if (p.row_mul != nullptr) {
+  if constexpr (NORM) {
     float gm[8];
     load8(p.col_mul, p.col_mul_dt, c0, nc, p.vec_mul && nc == 8, gm);
 #pragma unroll
@@ -83,6 +86,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       }
     }
   }
+
   if (p.colsum != nullptr) {
     // column sums in a fixed order: four rows per thread, two half warps,
     // sixteen warps
@@ -93,12 +97,14 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       t[j] += __shfl_xor_sync(0xFFFFFFFFu, t[j], 16);
     }
     if (half == 0) {
-      float4* d = reinterpret_cast<float4*>(&s_sum[warp][8 * g]);
+      float4* d = reinterpret_cast<float4*>(&sm.sum[warp][8 * g]);
       d[0] = make_float4(t[0], t[1], t[2], t[3]);
       d[1] = make_float4(t[4], t[5], t[6], t[7]);
     }
   }
 
+  // maxima of the thread's rows, columns and whole piece; infinities (rare)
+  // become NaN, which maxima skip, so that the finite values set the scales
   float rm[4], cm[8], all;
   auto maxima = [&]() {
 #pragma unroll
@@ -113,7 +119,6 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
   };
   maxima();
   if (is_inf(all)) {
-    // rare: the scales come from the finite values alone
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -125,11 +130,10 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
   uint32_t byte_all = 0;
   float inv_all = 0.0f;
   if constexpr (SQUARE) {
-    const uint32_t w = warp_max_u32(__float_as_uint(all));
-    if (lane == 0) s_max[0][warp] = __uint_as_float(w);
+    const uint32_t m = warp_max_u32(__float_as_uint(all));
+    if (lane == 0) sm.max[0][warp] = __uint_as_float(m);
     __syncthreads();
-    uint32_t m = __float_as_uint(s_max[0][lane & 15]);
-    byte_all = scale_byte(warp_max_u32(m));
+    byte_all = scale_byte(warp_max_u32(__float_as_uint(sm.max[0][lane & 15])));
     inv_all = inv_scale(byte_all);
   } else if (p.dst_t != nullptr) {
     uint32_t m[8];
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       m[j] = max(m[j], __shfl_xor_sync(0xFFFFFFFFu, m[j], 16));
     }
     if (half == 0) {
-      uint4* d = reinterpret_cast<uint4*>(&s_max[warp][8 * g]);
+      uint4* d = reinterpret_cast<uint4*>(&sm.max[warp][8 * g]);
       d[0] = make_uint4(m[0], m[1], m[2], m[3]);
       d[1] = make_uint4(m[4], m[5], m[6], m[7]);
     }
@@ -176,9 +180,9 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     uint8_t* d = p.dst + (row0 + lr0) * p.ld_dst + c0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint2 w = codes8(v[i], inv[i]);
-      if (whole) *reinterpret_cast<uint2*>(d + i * p.ld_dst) = w;
-      else if (i < nr && nc > 0) store_codes8(d + i * p.ld_dst, w, nc);
+      const uint2 c = codes8(v[i], inv[i]);
+      if (whole) *reinterpret_cast<uint2*>(d + i * p.ld_dst) = c;
+      else if (i < nr && nc > 0) store_codes8(d + i * p.ld_dst, c, nc);
     }
   }
 
@@ -191,16 +195,16 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
       if constexpr (!SQUARE) {
         uint32_t m = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(s_max[k][c]));
+        for (int k = 0; k < 16; ++k) m = max(m, __float_as_uint(sm.max[k][c]));
         b = scale_byte(m);
-        s_inv[c] = inv_scale(b);
+        sm.inv[c] = inv_scale(b);
       }
       p.sc_t[scale_offset(cols_pad, col0 + c, tile_r)] = (uint8_t)b;
     }
     if (p.colsum != nullptr && col0 + c < p.cols) {
-      float t = s_sum[0][c];
+      float t = sm.sum[0][c];
 #pragma unroll
-      for (int k = 1; k < 16; ++k) t += s_sum[k][c];
+      for (int k = 1; k < 16; ++k) t += sm.sum[k][c];
       p.colsum[tile_r * p.cols + col0 + c] = t;
     }
   }
@@ -213,7 +217,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4 x = *reinterpret_cast<const float4*>(&s_inv[8 * g + 4 * h]);
+      const float4 x = *reinterpret_cast<const float4*>(&sm.inv[8 * g + 4 * h]);
       inv[4 * h] = x.x; inv[4 * h + 1] = x.y; inv[4 * h + 2] = x.z; inv[4 * h + 3] = x.w;
     }
   }
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     for (int j = 0; j < 8; j += 2) mul2(v[i][j], v[i][j + 1], inv[j], inv[j + 1], v[i][j], v[i][j + 1]);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    s_t[(8 * g + j) * 32 + (u ^ (2 * g))] = e4m3x2_sat(v[0][j], v[1][j]) | (e4m3x2_sat(v[2][j], v[3][j]) << 16);
+    sm.t[(8 * g + j) * 32 + (u ^ (2 * g))] = e4m3x2_sat(v[0][j], v[1][j]) | (e4m3x2_sat(v[2][j], v[3][j]) << 16);
   __syncthreads();
   const int k2 = threadIdx.x & 7;                        // sixteen rows
   const int64_t gr = row0 + 16 * k2;
@@ -236,21 +240,40 @@ __global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p)
     const int c = it * 64 + (threadIdx.x >> 3);
     const int64_t gc = col0 + c;
     const int cg = c >> 3;
-    const uint4 x = *reinterpret_cast<const uint4*>(s_t + c * 32 + 4 * (k2 ^ (cg >> 1)));
-    const uint4 w = (cg & 1) ? make_uint4(x.z, x.w, x.x, x.y) : x;
+    const uint4 x = *reinterpret_cast<const uint4*>(sm.t + c * 32 + 4 * (k2 ^ (cg >> 1)));
+    const uint4 q = (cg & 1) ? make_uint4(x.z, x.w, x.x, x.y) : x;
     uint8_t* d = p.dst_t + gc * p.ld_dst_t + gr;
     if (whole) {
-      *reinterpret_cast<uint4*>(d) = w;
+      *reinterpret_cast<uint4*>(d) = q;
     } else if (gc < p.cols && gr < p.rows) {
       const int64_t n = p.rows - gr;
       if (n >= 16) {
-        *reinterpret_cast<uint4*>(d) = w;
+        *reinterpret_cast<uint4*>(d) = q;
       } else {
-        store_codes8(d, make_uint2(w.x, w.y), (int)min(n, (int64_t)8));
-        if (n > 8) store_codes8(d + 8, make_uint2(w.z, w.w), (int)n - 8);
+        store_codes8(d, make_uint2(q.x, q.y), (int)min(n, (int64_t)8));
+        if (n > 8) store_codes8(d + 8, make_uint2(q.z, q.w), (int)n - 8);
       }
     }
   }
+}
+
+template <int SRC, bool SQUARE, bool NORM>
+__global__ void __launch_bounds__(kCastThreads, 2) block_cast_kernel(CastArgs p) {
+  __shared__ __align__(16) CastShared sm;
+  pdl_launch_dependents();
+  pdl_wait();
+  cast_tile<SRC, SQUARE, NORM>(p, blockIdx.x, sm);
+}
+
+// A layer's weight and activations in one launch: the weight's tiles come
+// first, so a small weight's cast hides behind the activations'.
+template <int SRC_W, int SRC_X>
+__global__ void __launch_bounds__(kCastThreads, 2) block_cast2_kernel(CastArgs w, CastArgs x, int w_tiles) {
+  __shared__ __align__(16) CastShared sm;
+  pdl_launch_dependents();
+  pdl_wait();
+  if ((int)blockIdx.x < w_tiles) cast_tile<SRC_W, true, false>(w, blockIdx.x, sm);
+  else cast_tile<SRC_X, false, false>(x, (int64_t)blockIdx.x - w_tiles, sm);
 }
 
 struct DequantArgs {
@@ -287,6 +310,33 @@ __global__ void __launch_bounds__(256) block_dequant_kernel(DequantArgs p) {
       if (nn > 0) store8<DST>(p.dst, r * p.ld_dst + c0 + 8 * h, nn, p.vec_dst && nn == 8, v);
     }
   }
+}
+
+CastArgs cast_args(const void* src, int es, int64_t rows, int64_t cols, int64_t ld_src, const float* row_mul,
+                   const void* col_mul, int col_mul_dt, void* dst, int64_t ld_dst, void* sc, void* dst_t,
+                   int64_t ld_dst_t, void* sc_t, float* colsum) {
+  return CastArgs{src, rows, cols, ld_src, row_mul, col_mul, col_mul_dt, static_cast<uint8_t*>(dst), ld_dst,
+                  static_cast<uint8_t*>(sc), static_cast<uint8_t*>(dst_t), ld_dst_t, static_cast<uint8_t*>(sc_t), colsum,
+                  vec16(src, ld_src, es) ? 1 : 0, vec16(col_mul, 8, 4) ? 1 : 0, (cols + 127) / 128};
+}
+
+int64_t cast_tiles(int64_t rows, int64_t cols) { return ((rows + 127) / 128) * ((cols + 127) / 128); }
+
+// The weight (square scales) and the activations of a layer, both checked.
+int cast_pair(const CastArgs& w, int w_dt, const CastArgs& x, int x_dt, cudaStream_t s) {
+  const int64_t tw = cast_tiles(w.rows, w.cols), tx = cast_tiles(x.rows, x.cols);
+  if (tw + tx > (1ll << 31) - 1) return APA_ERR_INVALID;
+  void (*k)(CastArgs, CastArgs, int) = nullptr;
+#define APA_CAST2_CASE(W)                                                       \
+  k = x_dt == APA_DT_F32   ? block_cast2_kernel<W, APA_DT_F32>                  \
+      : x_dt == APA_DT_F16 ? block_cast2_kernel<W, APA_DT_F16>                  \
+                           : block_cast2_kernel<W, APA_DT_BF16>
+  if (w_dt == APA_DT_F32) APA_CAST2_CASE(APA_DT_F32);
+  else if (w_dt == APA_DT_F16) APA_CAST2_CASE(APA_DT_F16);
+  else APA_CAST2_CASE(APA_DT_BF16);
+#undef APA_CAST2_CASE
+  return launch_kernel(k, dim3((unsigned)(tw + tx)), dim3(kCastThreads), 0, s, 1, w, x, (int)tw) == cudaSuccess
+             ? APA_OK : APA_ERR_CUDA;
 }
 
 // Column sums of [parts, cols] fp32 partials in a fixed order, rounded once to
@@ -358,13 +408,17 @@ extern "C" int apa_block_cast(const void* src, int src_dtype, int64_t rows, int6
   if (dst_t && !vec16(dst_t, ld_dst_t, 1)) return APA_ERR_ALIGN;
   const int64_t tr = (rows + 127) / 128, tc = (cols + 127) / 128;
   if (tr * tc > (1ll << 31) - 1) return APA_ERR_INVALID;
-  CastArgs a{src, rows, cols, ld_src, row_mul, col_mul, col_mul_dtype, static_cast<uint8_t*>(dst), ld_dst,
-             static_cast<uint8_t*>(scales), static_cast<uint8_t*>(dst_t), ld_dst_t, static_cast<uint8_t*>(scales_t),
-             colsum_partial, vec16(src, ld_src, es) ? 1 : 0, vec16(col_mul, 8, 4) ? 1 : 0, tc};
+  const CastArgs a = cast_args(src, es, rows, cols, ld_src, row_mul, col_mul, col_mul_dtype, dst, ld_dst, scales, dst_t,
+                               ld_dst_t, scales_t, colsum_partial);
   void (*k)(CastArgs);
-  if (src_dtype == APA_DT_F32) k = square ? block_cast_kernel<APA_DT_F32, true> : block_cast_kernel<APA_DT_F32, false>;
-  else if (src_dtype == APA_DT_F16) k = square ? block_cast_kernel<APA_DT_F16, true> : block_cast_kernel<APA_DT_F16, false>;
-  else k = square ? block_cast_kernel<APA_DT_BF16, true> : block_cast_kernel<APA_DT_BF16, false>;
+  const bool norm = row_mul != nullptr;
+#define APA_CAST_CASE(SRC)                                                                        \
+  k = square ? (norm ? block_cast_kernel<SRC, true, true> : block_cast_kernel<SRC, true, false>)  \
+             : (norm ? block_cast_kernel<SRC, false, true> : block_cast_kernel<SRC, false, false>)
+  if (src_dtype == APA_DT_F32) APA_CAST_CASE(APA_DT_F32);
+  else if (src_dtype == APA_DT_F16) APA_CAST_CASE(APA_DT_F16);
+  else APA_CAST_CASE(APA_DT_BF16);
+#undef APA_CAST_CASE
   return apa::launch_kernel(k, dim3((unsigned)(tr * tc)), dim3(kCastThreads), 0, static_cast<cudaStream_t>(stream), 1,
                             a) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }

@@ -141,18 +141,23 @@ extern "C" int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, co
   }
   const Packed X(ws + f.xq, M, K), XT(xt, K, M), W(w ? ws + f.wq : wq, N, K), WT(wt, K, N);
   int st;
-  if (gamma)
-    st = apa_rmsnorm_fwd(x, ld_x, residual, ld_res, gamma, gamma_dtype, x_dtype, M, K, eps, stream_out, ld_stream,
-                         nullptr, 0, X.q, X.ld, X.sc, rstd, stream);
-  else
-    st = apa_block_cast(x, x_dtype, M, K, ld_x, nullptr, nullptr, 0, 0, X.q, X.ld, X.sc, XT.q, XT.ld, XT.sc, nullptr,
-                        stream);
-  if (st) return st;
-  if (w) {
-    st = apa_block_cast(w, w_dtype, N, K, ld_w, nullptr, nullptr, 0, 1, W.q, W.ld, W.sc, WT.q, WT.ld, WT.sc, nullptr,
-                        stream);
-    if (st) return st;
+  if (gamma || !w) {
+    if (gamma)
+      st = apa_rmsnorm_fwd(x, ld_x, residual, ld_res, gamma, gamma_dtype, x_dtype, M, K, eps, stream_out, ld_stream,
+                           nullptr, 0, X.q, X.ld, X.sc, rstd, stream);
+    else
+      st = apa_block_cast(x, x_dtype, M, K, ld_x, nullptr, nullptr, 0, 0, X.q, X.ld, X.sc, nullptr, 0, nullptr, nullptr,
+                          stream);
+    if (!st && w)
+      st = apa_block_cast(w, w_dtype, N, K, ld_w, nullptr, nullptr, 0, 1, W.q, W.ld, W.sc, WT.q, WT.ld, WT.sc, nullptr,
+                          stream);
+  } else {
+    st = cast_pair(cast_args(w, elem_bytes(w_dtype), N, K, ld_w, nullptr, nullptr, 0, W.q, W.ld, W.sc, WT.q, WT.ld, WT.sc,
+                             nullptr), w_dtype,
+                   cast_args(x, elem_bytes(x_dtype), M, K, ld_x, nullptr, nullptr, 0, X.q, X.ld, X.sc, XT.q, XT.ld, XT.sc,
+                             nullptr), x_dtype, static_cast<cudaStream_t>(stream));
   }
+  if (st) return st;
   return apa_block_gemm(X.q, X.ld, X.sc, W.q, W.ld, W.sc, bias, bias_dtype, y, y_dtype, ld_y, M, N, K, 0,
                         APA_BLOCK_AUTO, ws + f.gemm, f.gemm_bytes, stream);
 }

@@ -161,6 +161,31 @@ def test_kept_weight_follows_the_parameter():
         assert torch.equal(other(x), 4 * a)
 
 
+def test_kept_weight_of_another_parameter():
+    import copy
+    lin = layer(rnd((40, 64), 1))
+    x, w = rnd((3, 64), 2).cuda(), rnd((40, 64), 3).cuda()
+    with torch.no_grad():
+        lin(x)
+        want = layer(w)(x)
+        v = lin.weight_master._version
+        fresh = w.clone()
+        for _ in range(v - fresh._version):
+            fresh.add_(0.0)
+        lin.weight_master = nn.Parameter(fresh)            # as many changes as the one before it
+        assert lin.weight_master._version == v and torch.equal(lin(x), want)
+        other = copy.deepcopy(lin)
+        other.weight_master.mul_(2.0)
+        assert torch.equal(other(x), 2 * want) and torch.equal(lin(x), want)
+        lin.weight_master.data = 4 * w
+        assert torch.equal(lin(x), 4 * want)
+        assert torch.equal(lin.to(torch.bfloat16)(x), layer((4 * w).bfloat16().float())(x))
+    with torch.inference_mode():
+        assert torch.equal(other(x), 2 * want)
+        made = layer(w)
+        assert torch.equal(made(x), want)
+
+
 def test_empty_batch_and_frozen_parts():
     lin = layer(rnd((40, 64), 1), rnd((40,), 2))
     x = torch.zeros(0, 64, device="cuda", requires_grad=True)

@@ -406,3 +406,31 @@ def test_few_tokens(m, n, k, dtype):
     x[0, k // 2] = float("inf")
     z = block_linear(x, wq, b, out_dtype=torch.float32)
     assert bool(torch.isnan(z[0]).all()) and torch.equal(z[1:], y[1:])
+
+
+@pytest.mark.parametrize("plan", [pair_plan(4), pair_plan(8, 2), split_plan(64, 1, 0), split_plan(16, 2, 1)])
+def test_extreme_scales(plan):
+    """Scales from 2^-127 to 2^127: the exponents of the two sides add."""
+    from apa import blockscale
+    m, n, k = 16, 200, 512
+    g = torch.Generator().manual_seed(1)
+    a = torch.randint(1, 5, (m, k), generator=g).float()
+    b = torch.randint(1, 5, (n, k), generator=g).float()
+    for ea in (-127, -126, -1, 0, 126, 127):
+        A = APABlockTensor.from_parts(a.to(torch.float8_e4m3fn).cuda(), torch.full((m, 4), ea).cuda())
+        B = APABlockTensor.from_parts(b.to(torch.float8_e4m3fn).cuda(), torch.full((n, 4), -ea).cuda())
+        out = torch.empty(m, n, device="cuda")
+        blockscale._matmul(A, B, None, out, False, plan)
+        assert torch.equal(out.cpu(), a @ b.t()), ea
+
+
+def test_column_sums_of_infinite_gradients():
+    """A bias gradient sums the gradient as it comes: an infinity stays one."""
+    from apa import blockscale
+    x = torch.ones(300, 40)
+    x[5, 3] = float("inf")
+    x[200, 4] = float("nan")
+    sums = torch.empty(3, 40, device="cuda")
+    blockscale._cast(x.cuda(), True, True, colsum=sums)
+    got = sums.sum(0).cpu()
+    assert got[3] == float("inf") and torch.isnan(got[4]) and bool((got[5:] == 300).all())
