@@ -55,18 +55,28 @@ _REAL = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16:
 
 
 _fns: dict = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
-    """One library call on the tensors' device, whichever is current."""
+    """One library call on the current stream of the tensors' device, which
+    need not be the current device. The stream is the call's last argument."""
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args), name)
+    if device.index == _current_device():
+        _lib.check(fn(*args, _lib.stream_handle(device)), name)
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args), name)
+            _lib.check(fn(*args, _lib.stream_handle(device)), name)
+
+
+def _sizes(device: int, name: str, *args) -> int:
+    """A size that the library computes for a device."""
+    n = ctypes.c_int64(0)
+    with torch.cuda.device(device):
+        _lib.check(getattr(_lib.lib(), name)(*args, ctypes.addressof(n)), name)
+    return n.value
 
 
 def _real(dtype: torch.dtype, what: str) -> int:
@@ -210,8 +220,7 @@ class APABlockTensor:
         out = torch.empty(rows, cols, dtype=dtype, device=self.device)
         if rows:
             p, pitch, sc = self._at()
-            _call(self.device, "apa_block_dequant", p, pitch, sc, rows, cols, out.data_ptr(), code, cols,
-                  _lib.stream_handle(self.device))
+            _call(self.device, "apa_block_dequant", p, pitch, sc, rows, cols, out.data_ptr(), code, cols)
         return out
 
 
@@ -232,7 +241,7 @@ def _cast(x2: torch.Tensor, rows_form: bool, cols_form: bool, square: bool = Fal
         return q, qt
     _call(dev, "apa_block_cast", x2.data_ptr(), _REAL[x2.dtype], rows, cols, _ld(x2), _lib.ptr(row_mul),
           _lib.ptr(col_mul), _REAL[col_mul.dtype] if col_mul is not None else 0, int(square),
-          *(q._at() if q else _NONE), *(qt._at() if qt else _NONE), _lib.ptr(colsum), _lib.stream_handle(dev))
+          *(q._at() if q else _NONE), *(qt._at() if qt else _NONE), _lib.ptr(colsum))
     return q, qt
 
 
@@ -258,11 +267,7 @@ def block_cast(x: torch.Tensor, form: str = "rows", square: bool = False):
 
 @functools.lru_cache(maxsize=1024)
 def _matmul_workspace(M: int, N: int, K: int, dtype: int, plan: int, device: int) -> int:
-    n = ctypes.c_int64(0)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().apa_block_gemm_workspace(M, N, K, dtype, plan, ctypes.addressof(n)),
-                   "apa_block_gemm_workspace")
-    return n.value
+    return _sizes(device, "apa_block_gemm_workspace", M, N, K, dtype, plan)
 
 
 def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accumulate: bool, plan: int = 0) -> None:
@@ -271,8 +276,7 @@ def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accum
     n = _matmul_workspace(M, N, K, dt, plan, a.device.index)
     ws = torch.empty(n, dtype=torch.uint8, device=a.device) if n else None
     _call(a.device, "apa_block_gemm", *a._at(), *b._at(), _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0,
-          out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n,
-          _lib.stream_handle(a.device))
+          out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n)
 
 
 def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,
@@ -342,11 +346,7 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
 
 @functools.lru_cache(maxsize=4096)
 def _forward_workspace(M: int, N: int, K: int, flags: int, dtype: int, device: int) -> int:
-    n = ctypes.c_int64(0)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().apa_block_linear_fwd_workspace(M, N, K, flags, dtype, ctypes.addressof(n)),
-                   "apa_block_linear_fwd_workspace")
-    return n.value
+    return _sizes(device, "apa_block_linear_fwd_workspace", M, N, K, flags, dtype)
 
 
 def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bias, y, out_code, M, N, K) -> None:
@@ -362,7 +362,7 @@ def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bi
           _lib.ptr(gamma), _REAL[gamma.dtype] if gamma is not None else 0, eps, _lib.ptr(stream), K, _lib.ptr(rstd),
           xt, _lib.ptr(w2), _REAL[w2.dtype] if w2 is not None else 0, _ld(w2) if w2 is not None else 0, wq, wt,
           _lib.ptr(bias), _REAL[bias.dtype] if bias is not None else 0, y.data_ptr(), out_code, N, M, N, K,
-          _lib.ptr(ws), n, _lib.stream_handle(dev))
+          _lib.ptr(ws), n)
 
 
 # ---------------------------------------------------------------------------
@@ -403,16 +403,13 @@ def _norm_forward(x2, g, res2, eps: float, quantize: bool, want_rstd: bool):
     if M:
         _call(dev, "apa_rmsnorm_fwd", x2.data_ptr(), _ld(x2), _lib.ptr(res2), _ld(res2) if res2 is not None else 0,
               g.data_ptr(), _REAL[g.dtype], _REAL[x2.dtype], M, K, eps, _lib.ptr(stream), K, _lib.ptr(y), K,
-              *(q._at() if q else _NONE), _lib.ptr(rstd), _lib.stream_handle(dev))
+              *(q._at() if q else _NONE), _lib.ptr(rstd))
     return (q if quantize else y), stream, rstd
 
 
 @functools.lru_cache(maxsize=1024)
 def _norm_workspace(M: int, K: int, device: int) -> int:
-    n = ctypes.c_int64(0)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().apa_rmsnorm_bwd_workspace(M, K, ctypes.addressof(n)), "apa_rmsnorm_bwd_workspace")
-    return n.value
+    return _sizes(device, "apa_rmsnorm_bwd_workspace", M, K)
 
 
 def _norm_backward(dh2, r2, rstd, g, dr2):
@@ -427,7 +424,7 @@ def _norm_backward(dh2, r2, rstd, g, dr2):
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _REAL[dh2.dtype], _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
           _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K, _REAL[r2.dtype], M, K,
-          dg.data_ptr(), ws.data_ptr(), n, _lib.stream_handle(dev))
+          dg.data_ptr(), ws.data_ptr(), n)
     return dx, dg
 
 
@@ -535,11 +532,7 @@ class APARMSNorm(nn.Module):
 # ---------------------------------------------------------------------------
 @functools.lru_cache(maxsize=1024)
 def _linear_workspace(M: int, N: int, K: int, flags: int, dtype: int, dw_dtype: int, device: int) -> int:
-    n = ctypes.c_int64(0)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().apa_block_linear_bwd_workspace(M, N, K, flags, dtype, dw_dtype, ctypes.addressof(n)),
-                   "apa_block_linear_bwd_workspace")
-    return n.value
+    return _sizes(device, "apa_block_linear_bwd_workspace", M, N, K, flags, dtype, dw_dtype)
 
 
 class _BlockLinearFn(torch.autograd.Function):
@@ -618,8 +611,7 @@ class _BlockLinearFn(torch.autograd.Function):
                   p if ctx.n_xt else None, _lib.ptr(stream), _ld(stream) if has_norm else 0, _lib.ptr(ctx.rstd),
                   _lib.ptr(gamma), _REAL[gamma.dtype] if has_norm else 0, _lib.ptr(dr2),
                   _ld(dr2) if dr2 is not None else 0, _lib.ptr(dx), code, K, _lib.ptr(dg), _lib.ptr(dw), wcode, K,
-                  _lib.ptr(db), _REAL[bdtype] if db is not None else 0, M, N, K, ws.data_ptr(), n,
-                  _lib.stream_handle(dev))
+                  _lib.ptr(db), _REAL[bdtype] if db is not None else 0, M, N, K, ws.data_ptr(), n)
         else:
             for t in (dx, dw, db, dg):
                 if t is not None:
