@@ -280,34 +280,47 @@ struct DequantArgs {
   const uint8_t* src; int64_t ld; const uint8_t* sc;
   int64_t rows, cols; void* dst; int64_t ld_dst;
   int vec_dst;
-  int64_t chunks;   // 16-element chunks per row
+  uint32_t chunks;   // 8-element chunks per row
 };
 
-// One thread per 16 codes (one 16-byte load).
-template <int DST>
+// Eight codes per thread and step, so a warp's stores cover whole lines; four
+// steps under way together. I: the type that counts chunks (64-bit division
+// costs as much as the conversion).
+template <int DST, class I>
 __global__ void __launch_bounds__(256) block_dequant_kernel(DequantArgs p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t total = p.rows * p.chunks;
+  const I total = (I)p.rows * p.chunks;
   const int64_t rows_pad = rows_padded(p.rows);
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-    const int64_t r = e / p.chunks, c0 = (e - r * p.chunks) * 16;
-    const uint4 q = *reinterpret_cast<const uint4*>(p.src + r * p.ld + c0);   // rows are padded to 16 codes
-    const float s = scale_value(p.sc[scale_offset(rows_pad, r, c0 >> 7)]);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    const int n = (int)min((int64_t)16, p.cols - c0);
+  const I first = (I)blockIdx.x * 1024 + threadIdx.x;
+  uint2 q[4];
+  uint32_t b[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+  for (int k = 0; k < 4; ++k) {
+    const I e = first + 256 * k;
+    if (e < total) {
+      const I r = e / p.chunks;
+      const int c0 = (int)(e - r * p.chunks) * 8;
+      q[k] = *reinterpret_cast<const uint2*>(p.src + (int64_t)r * p.ld + c0);     // rows are padded to 16 codes
+      b[k] = p.sc[scale_offset(rows_pad, (int64_t)r, c0 >> 7)];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const I e = first + 256 * k;
+    if (e < total) {
+      const I r = e / p.chunks;
+      const int c0 = (int)(e - r * p.chunks) * 8;
+      const float s = scale_value(b[k]);
+      const uint32_t w[2] = {q[k].x, q[k].y};
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t two = (w[2 * h + (k >> 1)] >> (16 * (k & 1))) & 0xFFFFu;
-        const uint32_t f = f16x2_from_e4m3x2(two);
-        v[2 * k] = f16lo_to_f32(f) * s;
-        v[2 * k + 1] = f16hi_to_f32(f) * s;
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t f = f16x2_from_e4m3x2((w[h >> 1] >> (16 * (h & 1))) & 0xFFFFu);
+        mul2(f16lo_to_f32(f), f16hi_to_f32(f), s, s, v[2 * h], v[2 * h + 1]);
       }
-      const int nn = min(8, n - 8 * h);
-      if (nn > 0) store8<DST>(p.dst, r * p.ld_dst + c0 + 8 * h, nn, p.vec_dst && nn == 8, v);
+      const int n = (int)min((int64_t)8, p.cols - c0);
+      store8<DST>(p.dst, (int64_t)r * p.ld_dst + c0, n, p.vec_dst && n == 8, v);
     }
   }
 }
@@ -432,11 +445,16 @@ extern "C" int apa_block_dequant(const void* src, int64_t ld, const void* scales
   if (es == 0) return APA_ERR_UNSUPPORTED;
   if (!vec16(src, ld, 1)) return APA_ERR_ALIGN;
   DequantArgs a{static_cast<const uint8_t*>(src), ld, static_cast<const uint8_t*>(scales), rows, cols, dst, ld_dst,
-                vec16(dst, ld_dst, es) ? 1 : 0, (cols + 15) / 16};
-  const int64_t grid = std::min<int64_t>((rows * a.chunks + 255) / 256, (int64_t)apa::num_sms() * 16);
-  void (*k)(DequantArgs) = dst_dtype == APA_DT_F32 ? block_dequant_kernel<APA_DT_F32>
-                           : dst_dtype == APA_DT_F16 ? block_dequant_kernel<APA_DT_F16>
-                                                     : block_dequant_kernel<APA_DT_BF16>;
+                vec16(dst, ld_dst, es) ? 1 : 0, (uint32_t)((cols + 7) / 8)};
+  const int64_t total = rows * (int64_t)a.chunks, grid = (total + 1023) / 1024;
+  if (grid > (1ll << 31) - 1) return APA_ERR_INVALID;
+  const bool wide = total > (1ll << 31) - 2048;
+  void (*k)(DequantArgs);
+#define APA_DEQUANT_CASE(DST) k = wide ? block_dequant_kernel<DST, uint64_t> : block_dequant_kernel<DST, uint32_t>
+  if (dst_dtype == APA_DT_F32) APA_DEQUANT_CASE(APA_DT_F32);
+  else if (dst_dtype == APA_DT_F16) APA_DEQUANT_CASE(APA_DT_F16);
+  else APA_DEQUANT_CASE(APA_DT_BF16);
+#undef APA_DEQUANT_CASE
   return apa::launch_kernel(k, dim3((unsigned)grid), dim3(256), 0, static_cast<cudaStream_t>(stream), 1, a) ==
                  cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }

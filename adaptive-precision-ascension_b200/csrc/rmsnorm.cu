@@ -77,13 +77,14 @@ template <int DT> constexpr int pieces() { return DT == APA_DT_F32 ? 2 : 1; }   
 // The chunks of one thread in one row, in planes of 16 bytes per thread (so a
 // warp's accesses are conflict-free). at: this thread's bytes of plane 0.
 template <int DT, int TPR, int NV>
-__device__ __forceinline__ void fetch_row(uint32_t at, const void* p, int64_t row_at, int t, int64_t cols) {
+__device__ __forceinline__ void fetch_row(uint32_t at, const void* p, int64_t row_at, int t, int cols) {
   constexpr int ES = DT == APA_DT_F32 ? 4 : 2;
+  const char* row = static_cast<const char*>(p) + row_at * ES;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
+    const int c0 = (t + TPR * i) * 8;
     if (c0 < cols) {
-      const char* g = static_cast<const char*>(p) + (row_at + c0) * ES;
+      const char* g = row + c0 * ES;
 #pragma unroll
       for (int k = 0; k < pieces<DT>(); ++k)
         cp_async16(at + (uint32_t)((i * pieces<DT>() + k) * norm_threads<TPR>() * 16), g + 16 * k);
@@ -135,11 +136,13 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
   using C = NormCfg<DT, TPR, NV>;
   constexpr int kRows = C::kRows;
   constexpr int D = ASYNC ? C::kDepth : 1;
+  constexpr int ES = DT == APA_DT_F32 ? 4 : 2;
   __shared__ float s_red[32];
   extern __shared__ __align__(16) char s_rows[];
   pdl_launch_dependents();
   pdl_wait();
   const int t = threadIdx.x % TPR;
+  const int cols = (int)p.cols;
   const int64_t step = (int64_t)gridDim.x * kRows;
   const int64_t rows_pad = rows_padded(p.rows);
   char* mine = s_rows + threadIdx.x * 16;
@@ -147,12 +150,23 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
     if constexpr (ASYNC) {
       if (row < p.rows) {
         const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(mine + slot * C::kSlot));
-        fetch_row<DT, TPR, NV>(at, p.x, row * p.ld_x, t, p.cols);
-        if (p.res != nullptr) fetch_row<DT, TPR, NV>(at + C::kArray, p.res, row * p.ld_res, t, p.cols);
+        fetch_row<DT, TPR, NV>(at, p.x, row * p.ld_x, t, cols);
+        if (p.res != nullptr) fetch_row<DT, TPR, NV>(at + C::kArray, p.res, row * p.ld_res, t, cols);
       }
       cp_async_commit();
     }
   };
+  // this thread's elements in chunk i (whole chunks or none with ASYNC)
+  auto count = [&](int i) {
+    const int left = cols - (t + TPR * i) * 8;
+    return ASYNC ? (left > 0 ? 8 : 0) : max(0, min(8, left));
+  };
+  // a persistent CTA keeps the weight in registers
+  float gm[NV][8];
+  if constexpr (ASYNC) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load8(p.gamma, p.gamma_dt, (t + TPR * i) * 8, count(i), p.vec_g && count(i) == 8, gm[i]);
+  }
   int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
 #pragma unroll
   for (int d = 0; d < D - 1; ++d) fetch(row + d * step, d);
@@ -164,25 +178,28 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
       cp_async_wait<D - 1>();
     }
     const char* at = mine + slot * C::kSlot;
+    const char* x_row = static_cast<const char*>(p.x) + row * p.ld_x * ES;
+    const char* res_row = static_cast<const char*>(p.res) + row * p.ld_res * ES;
+    char* r_row = static_cast<char*>(p.r) + row * p.ld_r * ES;
     float v[NV][8];
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-      chunk8<DT, TPR, ASYNC>(at, i, p.x, row * p.ld_x + c0, n, p.vec_x, v[i]);
+      const int c0 = (t + TPR * i) * 8;
+      const int n = count(i);
+      chunk8<DT, TPR, ASYNC>(at, i, x_row, c0, n, p.vec_x, v[i]);
       if (p.res != nullptr) {
         float u[8];
-        chunk8<DT, TPR, ASYNC>(at + C::kArray, i, p.res, row * p.ld_res + c0, n, p.vec_res, u);
+        chunk8<DT, TPR, ASYNC>(at + C::kArray, i, res_row, c0, n, p.vec_res, u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] += u[j];
         if constexpr (DT == APA_DT_F32) {
-          if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, p.vec_r && n == 8, v[i]);
+          if (n > 0) store8<DT>(r_row, c0, n, p.vec_r && n == 8, v[i]);
         } else {
           const uint4 w = pack8<DT>(v[i]);
           unpack8<DT>(w, v[i]);
-          if (p.vec_r && n == 8) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.r) + row * p.ld_r + c0) = w;
-          else if (n > 0) store8<DT>(p.r, row * p.ld_r + c0, n, false, v[i]);
+          if (p.vec_r && n == 8) *reinterpret_cast<uint4*>(r_row + c0 * ES) = w;
+          else if (n > 0) store8<DT>(r_row, c0, n, false, v[i]);
         }
       }
       // squares in two chains per chunk, then the chunks, then the threads
@@ -192,16 +209,22 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
       ss += q0 + q1;
     }
     ss = row_sum<TPR>(ss, s_red);
-    const float rstd = rsqrt_refined(ss / (float)p.cols + p.eps);
+    const float rstd = rsqrt_refined(ss / (float)cols + p.eps);
     if (t == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+    uint8_t* q_row = p.q + row * p.ld_q;
+    char* y_row = static_cast<char*>(p.y) + row * p.ld_y * ES;
+    uint8_t* sc_row = p.sc + scale_offset(rows_pad, row, 0);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
-      float gm[8];
-      load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm);     // in L1 after the first row
+      const int c0 = (t + TPR * i) * 8;
+      const int n = count(i);
       float (&y)[8] = v[i];
-      normed8(y, rstd, gm);
+      if constexpr (ASYNC) {
+        normed8(y, rstd, gm[i]);
+      } else {
+        load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm[i]);
+        normed8(y, rstd, gm[i]);
+      }
       if (n < 8) {
         // columns past the end are 0 whatever the row's statistics
 #pragma unroll
@@ -226,11 +249,14 @@ __global__ void __launch_bounds__(norm_threads<TPR>()) rmsnorm_kernel(NormArgs p
         for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         const uint32_t b = scale_byte(m);
         if (n > 0) {
-          store_codes8(p.q + row * p.ld_q + c0, codes8(y, inv_scale(b)), n);
-          if ((t & 15) == 0) p.sc[scale_offset(rows_pad, row, c0 >> 7)] = (uint8_t)b;
+          const uint2 w = codes8(y, inv_scale(b));
+          if (ASYNC || n == 8) *reinterpret_cast<uint2*>(q_row + c0) = w;
+          else store_codes8(q_row + c0, w, n);
+          // byte kb % 4 of the word of group kb / 4
+          if ((t & 15) == 0) sc_row[(int64_t)(c0 >> 9) * rows_pad * 4 + ((c0 >> 7) & 3)] = (uint8_t)b;
         }
       } else {
-        if (n > 0) store8<DT>(p.y, row * p.ld_y + c0, n, p.vec_y && n == 8, y);
+        if (n > 0) store8<DT>(y_row, c0, n, p.vec_y && n == 8, y);
       }
     }
     if constexpr (ASYNC) slot = slot + 1 == D ? 0 : slot + 1;
@@ -250,6 +276,11 @@ struct NormBwdArgs {
   int vec_dy, vec_r, vec_dr, vec_dx, vec_g;
 };
 
+// CTAs of the backward per SM, which is what bounds a thread's registers.
+constexpr int norm_bwd_resident(int tpr, int nv) {
+  return tpr >= 512 ? 1 : tpr == 256 ? 3 : tpr == 128 && nv == 1 ? 8 : 4;
+}
+
 template <int DT, int DY, int TPR, int NV> struct NormBwdCfg {
   static constexpr int kThreads = norm_threads<TPR>();
   static constexpr int kRows = kThreads / TPR;
@@ -262,10 +293,12 @@ template <int DT, int DY, int TPR, int NV> struct NormBwdCfg {
 };
 
 template <int DT, int DY, int TPR, int NV, bool ASYNC>
-__global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(NormBwdArgs p) {
+__global__ void __launch_bounds__(norm_threads<TPR>(), norm_bwd_resident(TPR, NV)) rmsnorm_bwd_kernel(NormBwdArgs p) {
   using C = NormBwdCfg<DT, DY, TPR, NV>;
   constexpr int kRows = C::kRows;
   constexpr int D = ASYNC ? C::kDepth : 1;
+  constexpr int ES = DT == APA_DT_F32 ? 4 : 2, EY = DY == APA_DT_F32 ? 4 : 2;
+  const int cols = (int)p.cols;
   __shared__ float s_red[32];
   extern __shared__ __align__(16) char s_rows[];    // row buffers, then [kRows][NV * TPR * 8] sums
   pdl_launch_dependents();
@@ -277,9 +310,9 @@ __global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(Nor
     if constexpr (ASYNC) {
       if (row < p.rows) {
         const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(mine + slot * C::kSlot));
-        fetch_row<DY, TPR, NV>(at, p.dy, row * p.ld_dy, t, p.cols);
-        fetch_row<DT, TPR, NV>(at + C::kArrayDy, p.r, row * p.ld_r, t, p.cols);
-        if (p.dr != nullptr) fetch_row<DT, TPR, NV>(at + C::kArrayDy + C::kArray, p.dr, row * p.ld_dr, t, p.cols);
+        fetch_row<DY, TPR, NV>(at, p.dy, row * p.ld_dy, t, cols);
+        fetch_row<DT, TPR, NV>(at + C::kArrayDy, p.r, row * p.ld_r, t, cols);
+        if (p.dr != nullptr) fetch_row<DT, TPR, NV>(at + C::kArrayDy + C::kArray, p.dr, row * p.ld_dr, t, cols);
       }
       cp_async_commit();
     }
@@ -289,7 +322,11 @@ __global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(Nor
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) dg[i][j] = 0.0f;
-  const float inv_n = 1.0f / (float)p.cols;
+  const float inv_n = 1.0f / (float)cols;
+  auto count = [&](int i) {
+    const int left = cols - (t + TPR * i) * 8;
+    return ASYNC ? (left > 0 ? 8 : 0) : max(0, min(8, left));
+  };
   int64_t row = (int64_t)blockIdx.x * kRows + sub;
 #pragma unroll
   for (int d = 0; d < D - 1; ++d) fetch(row + d * step, d);
@@ -301,39 +338,49 @@ __global__ void __launch_bounds__(norm_threads<TPR>(), 1) rmsnorm_bwd_kernel(Nor
       cp_async_wait<D - 1>();
     }
     const char* at = mine + slot * C::kSlot;
-    float gdy[NV][8], xh[NV][8];
+    const char* dy_row = static_cast<const char*>(p.dy) + row * p.ld_dy * EY;
+    const char* r_row = static_cast<const char*>(p.r) + row * p.ld_r * ES;
+    const char* dr_row = static_cast<const char*>(p.dr) + row * p.ld_dr * ES;
+    char* dx_row = static_cast<char*>(p.dx) + row * p.ld_dx * ES;
+    float gdy[NV][8], xh[NV][8], u[NV][8];
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
+      const int c0 = (t + TPR * i) * 8;
+      const int n = count(i);
       float gm[8];
       load8(p.gamma, p.gamma_dt, c0, n, p.vec_g && n == 8, gm);     // in L1 after the first row
-      chunk8<DY, TPR, ASYNC>(at, i, p.dy, row * p.ld_dy + c0, n, p.vec_dy, gdy[i]);
-      chunk8<DT, TPR, ASYNC>(at + C::kArrayDy, i, p.r, row * p.ld_r + c0, n, p.vec_r, xh[i]);
+      chunk8<DY, TPR, ASYNC>(at, i, dy_row, c0, n, p.vec_dy, gdy[i]);
+      chunk8<DT, TPR, ASYNC>(at + C::kArrayDy, i, r_row, c0, n, p.vec_r, xh[i]);
+      // without buffers the stream's gradient is loaded ahead of the row's sum
+      if (!ASYNC && p.dr != nullptr) load8<DT>(dr_row, c0, n, p.vec_dr && n == 8, u[i]);
+      float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        xh[i][j] *= rstd;
-        dg[i][j] = __fmaf_rn(gdy[i][j], xh[i][j], dg[i][j]);
-        gdy[i][j] *= gm[j];
-        s = __fmaf_rn(gdy[i][j], xh[i][j], s);
+      for (int j = 0; j < 8; j += 2) {
+        mul2(xh[i][j], xh[i][j + 1], rstd, rstd, xh[i][j], xh[i][j + 1]);
+        fma2(gdy[i][j], gdy[i][j + 1], xh[i][j], xh[i][j + 1], dg[i][j], dg[i][j + 1], dg[i][j], dg[i][j + 1]);
+        mul2(gdy[i][j], gdy[i][j + 1], gm[j], gm[j + 1], gdy[i][j], gdy[i][j + 1]);
+        fma2(gdy[i][j], gdy[i][j + 1], xh[i][j], xh[i][j + 1], s0, s1, s0, s1);
       }
+      s += s0 + s1;
     }
-    const float c = row_sum<TPR>(s, s_red) * inv_n;
+    const float c = -row_sum<TPR>(s, s_red) * inv_n;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c0 = ((int64_t)t + (int64_t)TPR * i) * 8;
-      const int n = (int)max((int64_t)0, min((int64_t)8, p.cols - c0));
+      const int c0 = (t + TPR * i) * 8;
+      const int n = count(i);
       float o[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = rstd * __fmaf_rn(-xh[i][j], c, gdy[i][j]);
-      if (p.dr != nullptr) {
-        float u[8];
-        chunk8<DT, TPR, ASYNC>(at + C::kArrayDy + C::kArray, i, p.dr, row * p.ld_dr + c0, n, p.vec_dr, u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += u[j];
+      for (int j = 0; j < 8; j += 2) {
+        fma2(xh[i][j], xh[i][j + 1], c, c, gdy[i][j], gdy[i][j + 1], o[j], o[j + 1]);
+        mul2(o[j], o[j + 1], rstd, rstd, o[j], o[j + 1]);
       }
-      if (n > 0) store8<DT>(p.dx, row * p.ld_dx + c0, n, p.vec_dx && n == 8, o);
+      if (p.dr != nullptr) {
+        if constexpr (ASYNC) chunk8<DT, TPR, ASYNC>(at + C::kArrayDy + C::kArray, i, dr_row, c0, n, p.vec_dr, u[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += u[i][j];
+      }
+      if (n > 0) store8<DT>(dx_row, c0, n, p.vec_dx && n == 8, o);
     }
     if constexpr (ASYNC) slot = slot + 1 == D ? 0 : slot + 1;
   }
@@ -410,13 +457,12 @@ int norm_forward(const NormArgs& a, cudaStream_t s) {
   return launch_norm<DT, 1024, 4>(a, s);
 }
 
-// CTAs (= dgamma partial rows) of the backward, as many as are resident at once
-// (a thread holds 64 to 116 registers).
+// CTAs (= dgamma partial rows) of the backward: as many as are resident.
 int64_t norm_bwd_parts(int64_t rows, int64_t cols) {
   const int64_t chunks = (cols + 7) / 8;
   const int tpr = chunks <= 64 ? 32 : chunks <= 256 ? 128 : chunks <= 512 ? 256 : chunks <= 1024 ? 512 : 1024;
   const int per_cta = tpr < 128 ? 128 / tpr : 1;
-  const int64_t per_sm = tpr >= 512 ? 1 : tpr >= 256 ? 2 : tpr == 128 && chunks <= 128 ? 8 : 4;
+  const int64_t per_sm = norm_bwd_resident(tpr, chunks <= 32 || (chunks > 64 && chunks <= 128) ? 1 : 2);
   return std::min<int64_t>((rows + per_cta - 1) / per_cta, per_sm * num_sms());
 }
 
