@@ -460,7 +460,8 @@ template <int EW> struct PairCfg {
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
-struct PairArgs {
+// One product of a launch.
+struct Problem {
   int kb_count;
   int splits;           // the reduction is split over this many units per tile
   int slice_rows;       // rows of one split's slice of the workspace (out is the workspace when splits > 1)
@@ -469,36 +470,82 @@ struct PairArgs {
   OutArgs o;
 };
 
-// One pass of the persistent schedule: slabs kb0 .. kb1 of an output tile.
-// Units (tile, split) go round the CTA pairs; a unit's chunks follow each
-// other on the same pair.
+struct ProblemMaps { CUtensorMap a, b, sa, sb, o; };
+
+// NP products in one launch. Units (tile, split) go round the CTA pairs. With
+// two products, `units0` units of the first, the longer ones, are dealt first;
+// they may end in the middle of a round, so the pairs from `late` on, which
+// have one unit less, take `extra` units of the second product each before
+// all go on with what is left.
+template <int NP> struct PairArgs {
+  Problem q[NP];
+  int units0, units1, late, extra;
+};
+template <int NP> struct PairMaps { ProblemMaps m[NP]; };
+
+// One pass of the schedule: slabs kb0 .. kb1 of an output tile. A unit's
+// chunks follow each other on the same pair.
 struct Pass {
-  int unit, tile, split, first, kb0, kb1, end;
+  int prob, unit, phase;            // phase 0, 1, 2: first product, extra units, the rest; 3: done
+  int tile, split, first, kb0, kb1, end;
 };
 
-__device__ __forceinline__ void pass_unit(const PairArgs& p, int unit, Pass& a) {
-  a.unit = a.tile = unit;
+template <int NP>
+__device__ __forceinline__ void pass_unit(const PairArgs<NP>& p, Pass& a) {
+  const Problem& q = p.q[NP == 1 ? 0 : a.prob];
+  a.tile = a.unit;
   a.split = 0;
   a.first = 0;
-  a.end = p.kb_count;
-  if (p.splits > 1) {
+  a.end = q.kb_count;
+  if (q.splits > 1) {
     // kb_count < 2^24 and splits < 2^7: 32 bits hold the products
-    a.tile = unit / p.splits;
-    a.split = unit - a.tile * p.splits;
-    a.first = (int)((uint32_t)p.kb_count * (uint32_t)a.split / (uint32_t)p.splits);
-    a.end = (int)((uint32_t)p.kb_count * (uint32_t)(a.split + 1) / (uint32_t)p.splits);
+    a.tile = a.unit / q.splits;
+    a.split = a.unit - a.tile * q.splits;
+    a.first = (int)((uint32_t)q.kb_count * (uint32_t)a.split / (uint32_t)q.splits);
+    a.end = (int)((uint32_t)q.kb_count * (uint32_t)(a.split + 1) / (uint32_t)q.splits);
   }
   a.kb0 = a.first;
-  a.kb1 = min(a.kb0 + p.chunk, a.end);
+  a.kb1 = min(a.kb0 + q.chunk, a.end);
 }
 
-__device__ __forceinline__ void pass_next(const PairArgs& p, int step, Pass& a) {
+// The unit at a.unit of the current phase, or of the first phase after it that
+// has one for this pair.
+template <int NP>
+__device__ __forceinline__ void pass_settle(const PairArgs<NP>& p, int pair, int step, Pass& a) {
+  if (a.phase == 0) {
+    if (a.unit < p.units0) return pass_unit(p, a);
+    if (NP == 1) { a.phase = 3; return; }
+    a.prob = 1;
+    a.phase = 1;
+    a.unit = pair - p.late;
+  }
+  const int dealt = p.extra * (step - p.late);
+  if (a.phase == 1) {
+    if (a.unit >= 0 && a.unit < min(dealt, p.units1)) return pass_unit(p, a);
+    a.phase = 2;
+    a.unit = dealt + pair;
+  }
+  if (a.unit < p.units1) return pass_unit(p, a);
+  a.phase = 3;
+}
+
+template <int NP>
+__device__ __forceinline__ void pass_first(const PairArgs<NP>& p, int pair, int step, Pass& a) {
+  a.prob = 0;
+  a.phase = 0;
+  a.unit = pair;
+  pass_settle(p, pair, step, a);
+}
+
+template <int NP>
+__device__ __forceinline__ void pass_next(const PairArgs<NP>& p, int pair, int step, Pass& a) {
   if (a.kb1 < a.end) {
     a.kb0 = a.kb1;
-    a.kb1 = min(a.kb0 + p.chunk, a.end);
-  } else {
-    pass_unit(p, a.unit + step, a);
+    a.kb1 = min(a.kb0 + p.q[NP == 1 ? 0 : a.prob].chunk, a.end);
+    return;
   }
+  a.unit += a.phase == 1 ? step - p.late : step;
+  pass_settle(p, pair, step, a);
 }
 
 // A staged fp32 box added to out. Each element of out is added to by one warp,
@@ -538,11 +585,9 @@ __device__ __forceinline__ void put_box(const OutArgs& o, const uint8_t* box, in
   }
 }
 
-template <int EW>
+template <int EW, int NP>
 __global__ void __launch_bounds__(64 + 32 * EW, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                const __grid_constant__ CUtensorMap tmO, PairArgs p) {
+    pair_kernel(const __grid_constant__ PairMaps<NP> maps, const __grid_constant__ PairArgs<NP> p) {
   using C = PairCfg<EW>;
   constexpr int kStages = C::kStages;
   pdl_launch_dependents();
@@ -561,10 +606,10 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tshared + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = gemm::cluster_rank();
-  const int num_m = (p.o.M + 255) / 256, num_n = (p.o.N + 255) / 256;
-  const int units = num_m * num_n * p.splits;
-  const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
-  constexpr int kGroup = gemm::kGroupM / 2;
+  const int pair = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+  auto coords = [&](const Problem& q, int tile, int& mb, int& nb) {
+    gemm::tile_coords(tile, (q.o.M + 255) / 256, (q.o.N + 255) / 256, gemm::kGroupM / 2, mb, nb);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -584,12 +629,13 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x == 32 * 2) {
-    prefetch_map(&tmA);
-    prefetch_map(&tmB);
-    prefetch_map(&tmSA);
-    prefetch_map(&tmSB);
-    if (p.tma_out) prefetch_map(&tmO);
+  if (threadIdx.x >= 32 * 2 && threadIdx.x < 32 * 2 + NP) {
+    const ProblemMaps& m = maps.m[threadIdx.x - 32 * 2];
+    prefetch_map(&m.a);
+    prefetch_map(&m.b);
+    prefetch_map(&m.sa);
+    prefetch_map(&m.sb);
+    prefetch_map(&m.o);
   }
   fence_before();
   gemm::cluster_sync();
@@ -603,9 +649,10 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       uint32_t phase = 0;
       bool ok = true;
       Pass a;
-      for (pass_unit(p, first, a); ok && a.unit < units; pass_next(p, step, a)) {
+      for (pass_first(p, pair, step, a); ok && a.phase < 3; pass_next(p, pair, step, a)) {
+        const ProblemMaps& m = maps.m[NP == 1 ? 0 : a.prob];
         int mb, nb;
-        gemm::tile_coords(a.tile, num_m, num_n, kGroup, mb, nb);
+        coords(p.q[NP == 1 ? 0 : a.prob], a.tile, mb, nb);
         const int a_row = mb * 256 + (int)rank * BM, b_row = nb * 256 + (int)rank * BM;
         for (int kb = a.kb0; kb < a.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, kStatusTimeoutEmpty)) { ok = false; break; }
@@ -613,12 +660,12 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
           // the even CTA's barrier expects both CTAs' bytes
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * (C::kStageBytes + (scales ? C::kScaleBytes : 0)));
           const uint32_t bar = gemm::map_to_cta(&full[stage], 0);
-          gemm::tma_load_2d_pair(smA + stage * C::kHalfBytes, &tmA, kb * kSlab, a_row, bar);
-          gemm::tma_load_2d_pair(smB + stage * C::kHalfBytes, &tmB, kb * kSlab, b_row, bar);
+          gemm::tma_load_2d_pair(smA + stage * C::kHalfBytes, &m.a, kb * kSlab, a_row, bar);
+          gemm::tma_load_2d_pair(smB + stage * C::kHalfBytes, &m.b, kb * kSlab, b_row, bar);
           if (scales) {
             uint8_t* s = smS + stage * C::kScaleBytes;
-            gemm::tma_load_2d_pair(s, &tmSA, a_row, kb >> 2, bar);
-            gemm::tma_load_2d_pair(s + 512, &tmSB, nb * 256, kb >> 2, bar);
+            gemm::tma_load_2d_pair(s, &m.sa, a_row, kb >> 2, bar);
+            gemm::tma_load_2d_pair(s + 512, &m.sb, nb * 256, kb >> 2, bar);
           }
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
@@ -637,7 +684,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       bool ok = true;
       uint32_t set = 0;
       Pass a;
-      for (pass_unit(p, first, a); ok && a.unit < units; pass_next(p, step, a), ++local) {
+      for (pass_first(p, pair, step, a); ok && a.phase < 3; pass_next(p, pair, step, a), ++local) {
         const int acc = local & 1;
         if (!mbar_wait(&tempty[acc], ((uint32_t)(local >> 1) & 1u) ^ 1u, kStatusTimeoutAcc)) { ok = false; break; }
         // the previous tile's shared columns
@@ -673,7 +720,6 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
     const int q = warp & 3, e = warp - 2, part = e >> 2;
     uint8_t* boxes = smE + e * C::kBoxes * kEpiBox;
     float* sb = smBias + e * C::kWarpCols;
-    const bool out16 = p.o.out_dt != APA_DT_F32;
     int local = 0;
     int slot = 0, inflight = 0;           // staging ring; TMA stores that may still read their box
     const uint32_t te0 = gemm::map_to_cta(&tempty[0], 0), te1 = gemm::map_to_cta(&tempty[1], 0);
@@ -684,21 +730,25 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       if (lane == 0) arrive_peer(bar);
     };
     Pass a;
-    for (pass_unit(p, first, a); a.unit < units; pass_next(p, step, a), ++local) {
+    for (pass_first(p, pair, step, a); a.phase < 3; pass_next(p, pair, step, a), ++local) {
+      const Problem& prob = p.q[NP == 1 ? 0 : a.prob];
+      const OutArgs& o = prob.o;
+      const CUtensorMap* tmO = &maps.m[NP == 1 ? 0 : a.prob].o;
+      const bool out16 = o.out_dt != APA_DT_F32;
       int mb, nb;
-      gemm::tile_coords(a.tile, num_m, num_n, kGroup, mb, nb);
+      coords(prob, a.tile, mb, nb);
       const int acc = local & 1;
       const int row0 = mb * 256 + (int)rank * BM + q * 32;
-      const int orow = row0 + a.split * p.slice_rows;
+      const int orow = row0 + a.split * prob.slice_rows;
       const int col_base = nb * 256 + part * C::kWarpCols;
       // a unit's later chunks, and all of an accumulating product, are added to out
       const bool later = a.kb0 != a.first;
-      const bool add = later || p.o.accumulate;
-      const bool bias = p.o.bias != nullptr && !later;
+      const bool add = later || o.accumulate;
+      const bool bias = o.bias != nullptr && !later;
       if (bias) {
         __syncwarp();
         for (int c = lane; c < C::kWarpCols; c += 32)
-          sb[c] = col_base + c < p.o.N ? to_f32(p.o.bias, p.o.bias_dt, col_base + c) : 0.0f;
+          sb[c] = col_base + c < o.N ? to_f32(o.bias, o.bias_dt, col_base + c) : 0.0f;
         __syncwarp();
       }
       bool ready = true;
@@ -727,7 +777,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
         gemm::tmem_wait_ld();
         if (i == 0 && part == shared_part) arrive(ts);
         if (i == C::kUnits - 1) arrive(acc ? te1 : te0);
-        if (col0 >= p.o.N || row0 >= p.o.M) continue;      // warp-uniform
+        if (col0 >= o.N || row0 >= o.M) continue;      // warp-uniform
         if (bias) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
@@ -737,7 +787,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
           }
         }
         if (out16) {
-          if (p.o.out_dt == APA_DT_BF16) {
+          if (o.out_dt == APA_DT_BF16) {
 #pragma unroll
             for (int k = 0; k < 32; ++k) r[k] = bf16x2(fu(r[2 * k]), fu(r[2 * k + 1]));
           } else {
@@ -748,7 +798,7 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int x = col0 + 32 * b;
-          if ((out16 && b == 1) || x >= p.o.N) break;
+          if ((out16 && b == 1) || x >= o.N) break;
           uint8_t* box = boxes + slot * kEpiBox;
           if (inflight == C::kBoxes) {
             if (lane == 0) gemm::bulk_wait_read<C::kBoxes - 1>();
@@ -756,19 +806,19 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
           }
           __syncwarp();
           gemm::stage_row(box, lane, r + 32 * b);
-          if (p.tma_out) {
+          if (prob.tma_out) {
             gemm::fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (add) tma_add_2d(&tmO, box, x, orow);
-              else gemm::tma_store_2d(&tmO, box, x, orow);
+              if (add) tma_add_2d(tmO, box, x, orow);
+              else gemm::tma_store_2d(tmO, box, x, orow);
               gemm::bulk_commit();
             }
             ++inflight;
             slot = slot + 1 == C::kBoxes ? 0 : slot + 1;
           } else {
             __syncwarp();
-            put_box(p.o, box, lane, row0, x, add);
+            put_box(o, box, lane, row0, x, add);
           }
         }
       }
@@ -865,7 +915,7 @@ int out_map(CUtensorMap* tm, const OutArgs& o, int64_t rows) {
 }
 
 // CTA pairs of the kernel that run at once on the current device (0: none).
-template <int EW>
+template <int EW, int NP>
 int pair_slots() {
   using C = PairCfg<EW>;
   static unsigned long long attr = 0;
@@ -875,7 +925,7 @@ int pair_slots() {
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   dev &= 63;
   if (__atomic_load_n(&known, __ATOMIC_ACQUIRE) >> dev & 1ull) return slots[dev];
-  if (allow_smem(pair_kernel<EW>, C::kSmemBytes, &attr)) return 0;
+  if (allow_smem(pair_kernel<EW, NP>, C::kSmemBytes, &attr)) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * num_sms(), 1, 1);
   cfg.blockDim = dim3(C::kThreads, 1, 1);
@@ -888,7 +938,7 @@ int pair_slots() {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<EW>, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, pair_kernel<EW, NP>, &cfg) != cudaSuccess) {
     (void)cudaGetLastError();
     n = 0;
   }
@@ -935,50 +985,71 @@ __global__ void __launch_bounds__(256) block_sum_kernel(SumArgs p) {
 // A 16-bit output's own rounding is a thousand times that.
 constexpr int kChunkSlabs = 64;
 
-template <int EW>
-int launch_pair(const Operand& A, const Operand& B, int64_t K, OutArgs o, int splits, void* ws, cudaStream_t s) {
-  using C = PairCfg<EW>;
-  int slots = pair_slots<EW>();
-  if (slots < 1) return APA_ERR_UNSUPPORTED;
-  if (g_gemm_sm_limit > 0) slots = std::max(1, std::min(slots, g_gemm_sm_limit / 2));
+// Maps and arguments of one product; its slices lie in ws when it is split.
+int fill_problem(const Operand& A, const Operand& B, int64_t K, OutArgs o, int splits, void* ws, ProblemMaps* m,
+                 Problem* q) {
   const int64_t kb = (K + kSlab - 1) / kSlab;
-  CUtensorMap ta, tb, tsa, tsb, to;
-  if (int st = code_map(&ta, A.q, A.rows, K, A.ld, BM)) return st;
-  if (int st = code_map(&tb, B.q, B.rows, K, B.ld, BM)) return st;
-  if (int st = scale_map(&tsa, A.sc, A.rows, kb, 128)) return st;
-  if (int st = scale_map(&tsb, B.sc, B.rows, kb, 256)) return st;
-  const OutArgs final = o;
-  PairArgs p;
-  p.kb_count = (int)kb; p.splits = splits; p.slice_rows = 0;
+  if (int st = code_map(&m->a, A.q, A.rows, K, A.ld, BM)) return st;
+  if (int st = code_map(&m->b, B.q, B.rows, K, B.ld, BM)) return st;
+  if (int st = scale_map(&m->sa, A.sc, A.rows, kb, 128)) return st;
+  if (int st = scale_map(&m->sb, B.sc, B.rows, kb, 256)) return st;
+  q->kb_count = (int)kb; q->splits = splits; q->slice_rows = 0;
   int64_t out_rows = o.M;
   if (splits > 1) {
-    p.slice_rows = (int)slice_rows(o.M);
-    out_rows = p.slice_rows * (int64_t)splits;
+    q->slice_rows = (int)slice_rows(o.M);
+    out_rows = q->slice_rows * (int64_t)splits;
     o.out = ws; o.ldo = slice_ld(o.N); o.out_dt = APA_DT_F32; o.bias = nullptr; o.accumulate = 0; o.vec = 1;
     o.N = (int)o.ldo;
   }
   // only an fp32 output can be added to
-  p.chunk = o.out_dt == APA_DT_F32 ? kChunkSlabs : (int)kb;
-  p.o = o;
+  q->chunk = o.out_dt == APA_DT_F32 ? kChunkSlabs : (int)kb;
+  q->o = o;
   // a TMA store writes whole 16-byte pieces, past N too where N ends inside one
-  p.tma_out = o.vec && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0;
-  to = ta;
-  if (p.tma_out)
-    if (int st = out_map(&to, o, out_rows)) return st;
-  const int64_t units = cdiv64(o.M, 256) * cdiv64(o.N, 256) * splits;
-  if (units > (1ll << 31) - 1 - 2 * num_sms()) return APA_ERR_INVALID;
-  const int grid = 2 * (int)std::min<int64_t>(units, slots);
-  if (launch_kernel(pair_kernel<EW>, dim3(grid), dim3(C::kThreads), C::kSmemBytes, s, 2, ta, tb, tsa, tsb, to, p) !=
-      cudaSuccess)
-    return APA_ERR_CUDA;
-  if (splits > 1) {
-    SumArgs q{static_cast<const float*>(ws), p.slice_rows * o.ldo, o.ldo, splits, final};
-    const int64_t blocks = cdiv64(final.M * (o.ldo / 4), 256);
-    if (launch_kernel(block_sum_kernel, dim3((unsigned)std::min<int64_t>(blocks, 8 * num_sms())), dim3(256), 0, s, 1,
-                      q) != cudaSuccess)
-      return APA_ERR_CUDA;
-  }
+  q->tma_out = o.vec && ((int64_t)o.N * elem_bytes(o.out_dt)) % 16 == 0;
+  m->o = m->a;
+  if (q->tma_out)
+    if (int st = out_map(&m->o, o, out_rows)) return st;
   return APA_OK;
+}
+
+// The second kernel of a split product.
+int launch_sum(const OutArgs& o, int splits, const void* ws, cudaStream_t s) {
+  const int64_t ld = slice_ld(o.N);
+  const SumArgs q{static_cast<const float*>(ws), slice_rows(o.M) * ld, ld, splits, o};
+  const int64_t blocks = cdiv64(o.M * (ld / 4), 256);
+  return launch_kernel(block_sum_kernel, dim3((unsigned)std::min<int64_t>(blocks, 8 * num_sms())), dim3(256), 0, s, 1,
+                       q) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
+}
+
+int64_t pair_units(const OutArgs& o, int splits) { return cdiv64(o.M, 256) * cdiv64(o.N, 256) * splits; }
+
+template <int EW, int NP>
+int launch_pairs(const PairMaps<NP>& maps, PairArgs<NP>& p, int64_t units0, int64_t units1, cudaStream_t s) {
+  using C = PairCfg<EW>;
+  int slots = pair_slots<EW, NP>();
+  if (slots < 1) return APA_ERR_UNSUPPORTED;
+  if (g_gemm_sm_limit > 0) slots = std::max(1, std::min(slots, g_gemm_sm_limit / 2));
+  if (units0 + units1 > (1ll << 31) - 1 - 4 * (int64_t)num_sms()) return APA_ERR_INVALID;
+  const int pairs = (int)std::min<int64_t>(units0 + units1, slots);
+  p.units0 = (int)units0; p.units1 = (int)units1;
+  p.late = 0; p.extra = 0;
+  if (NP == 2) {
+    // how many of the second product's units a unit of the first is worth
+    const int64_t c0 = cdiv64(p.q[0].kb_count, p.q[0].splits) + 2, c1 = p.q[NP - 1].kb_count + 2;
+    p.late = (int)(units0 % pairs);
+    p.extra = p.late ? (int)std::min(std::max<int64_t>(1, (2 * c0 + c1) / (2 * c1)), cdiv64(units1, pairs - p.late)) : 0;
+  }
+  return launch_kernel(pair_kernel<EW, NP>, dim3(2 * pairs), dim3(C::kThreads), C::kSmemBytes, s, 2, maps, p) ==
+                 cudaSuccess ? APA_OK : APA_ERR_CUDA;
+}
+
+template <int EW>
+int launch_pair(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, int splits, void* ws, cudaStream_t s) {
+  PairMaps<1> m;
+  PairArgs<1> p;
+  if (int st = fill_problem(A, B, K, o, splits, ws, &m.m[0], &p.q[0])) return st;
+  if (int st = launch_pairs<EW, 1>(m, p, pair_units(o, splits), 0, s)) return st;
+  return splits > 1 ? launch_sum(o, splits, ws, s) : APA_OK;
 }
 
 // kind 0: split_kernel with `bn`, `split` and `swap`; 1: pair_kernel with `ew`
@@ -998,7 +1069,6 @@ struct BlockPlan { int kind, bn, split, swap, ew; };
 BlockPlan block_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
   const int64_t kb = cdiv64(K, kSlab);
   const int64_t small = std::min(M, N), big = std::max(M, N);
-  const double sms = g_gemm_sm_limit > 0 ? g_gemm_sm_limit : num_sms();
   BlockPlan best{0, 0, 1, M <= N ? 1 : 0, 8};
   best.bn = small <= 16 ? 16 : small <= 32 ? 32 : 64;
   const int64_t tiles = cdiv64(big, BM) * cdiv64(small, best.bn);
@@ -1011,7 +1081,7 @@ BlockPlan block_plan(int64_t M, int64_t N, int64_t K, bool aligned) {
     if (t < cost) { cost = t; best.split = split; }
   }
   const int64_t pt = cdiv64(M, 256) * cdiv64(N, 256);
-  const int64_t pairs = std::max<int64_t>(1, (int64_t)(sms / 2));
+  const int64_t pairs = std::max(1, num_sms() / 2);
   for (int split = 1; split <= 64 && split <= kb; ++split) {
     // a split pays where units would leave pairs idle, in whole waves
     if (split > 1 && pt * split > 2 * pairs) break;
@@ -1060,6 +1130,35 @@ int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, 
     case 32: return launch_split<32>(x, y, K, o, p.swap, p.split, s);
     default: return launch_split<64>(x, y, K, o, p.swap, p.split, s);
   }
+}
+
+// Two products in one launch, the first with units at least as long as the
+// second's: a backward's weight gradient and input gradient, which read
+// different casts of the same gradient. One launch less, and the second fills
+// the CTA pairs that the first leaves idle in its last round (4096 x 4096 over
+// 8192 tokens: 256 and 512 tiles on 74 pairs). The first is split when a tile
+// of it would take longer than an even share of all the work.
+int dual_split(const OutArgs& o0, int64_t K0, const OutArgs& o1, int64_t K1) {
+  const int64_t pairs = std::max(1, num_sms() / 2);
+  const int64_t kb0 = cdiv64(K0, kSlab), kb1 = cdiv64(K1, kSlab);
+  // two slabs' time to hand a tile over
+  const int64_t work = pair_units(o0, 1) * (kb0 + 2) + pair_units(o1, 1) * (kb1 + 2);
+  const int64_t share = std::max<int64_t>(cdiv64(work, pairs), kb1 + 2);
+  // a split unit of less than eight slabs costs more to add than it gains
+  return (int)std::max<int64_t>(1, std::min(std::min(cdiv64(kb0 + 2, share), kb0 / 8), (int64_t)64));
+}
+
+int block_gemm_dual(const Operand& A0, const Operand& B0, int64_t K0, const OutArgs& o0, const Operand& A1,
+                    const Operand& B1, int64_t K1, const OutArgs& o1, int split, void* ws, cudaStream_t s) {
+  PairMaps<2> m;
+  PairArgs<2> p;
+  if (int st = fill_problem(A0, B0, K0, o0, split, ws, &m.m[0], &p.q[0])) return st;
+  if (int st = fill_problem(A1, B1, K1, o1, 1, nullptr, &m.m[1], &p.q[1])) return st;
+  const int64_t u0 = pair_units(o0, split), u1 = pair_units(o1, 1);
+  // as in block_plan: eight epilogue warps for few slabs or a single round
+  const bool wide = cdiv64(K1, kSlab) < 8 || u0 + u1 <= num_sms() / 2;
+  if (int st = wide ? launch_pairs<8, 2>(m, p, u0, u1, s) : launch_pairs<4, 2>(m, p, u0, u1, s)) return st;
+  return split > 1 ? launch_sum(o0, split, ws, s) : APA_OK;
 }
 
 // y = x W^T for up to 16 rows that the product casts itself.

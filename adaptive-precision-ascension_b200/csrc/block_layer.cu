@@ -30,6 +30,8 @@ struct Packed {
 struct FwdSpace { int64_t xq, wq, gemm, gemm_bytes, total; };
 struct BwdSpace {
   int64_t dyq, dyt, xt, sums, dh, norm, gemm, norm_bytes, gemm_bytes, total;
+  int split;             // units per tile of the first of both products
+  bool dw_first;
 };
 
 // A few tokens through a kept weight: the product casts them itself.
@@ -78,12 +80,20 @@ int bwd_space(int64_t M, int64_t N, int64_t K, int flags, int dtype, int dw_dtyp
   if (dx && norm)
     if (int st = apa_rmsnorm_bwd_workspace(M, K, &s->norm_bytes)) return st;
   s->norm = take(s->norm_bytes);
-  int64_t a = 0, b = 0;
-  if (dw)
-    if (int st = apa_block_gemm_workspace(N, K, M, dw_dtype, APA_BLOCK_AUTO, &a)) return st;
-  if (dx)
-    if (int st = apa_block_gemm_workspace(M, K, N, norm ? APA_DT_F32 : dtype, APA_BLOCK_AUTO, &b)) return st;
-  s->gemm_bytes = std::max(a, b);
+  s->split = 1;
+  s->gemm_bytes = 0;
+  if (dw && dx) {
+    // both products in one launch, the one with the longer tiles first
+    OutArgs ow{}, ox{};
+    ow.M = (int)N; ow.N = (int)K; ox.M = (int)M; ox.N = (int)K;
+    s->dw_first = M >= N;
+    s->split = s->dw_first ? dual_split(ow, M, ox, N) : dual_split(ox, N, ow, M);
+    s->gemm_bytes = s->dw_first ? split_bytes(N, K, s->split) : split_bytes(M, K, s->split);
+  } else if (dw) {
+    if (int st = apa_block_gemm_workspace(N, K, M, dw_dtype, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
+  } else if (dx) {
+    if (int st = apa_block_gemm_workspace(M, K, N, norm ? APA_DT_F32 : dtype, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
+  }
   s->gemm = take(s->gemm_bytes);
   s->total = at;
   return APA_OK;
@@ -206,28 +216,36 @@ extern "C" int apa_block_linear_bwd(const void* dy, int dy_dtype, int64_t ld_dy,
     st = apa_block_colsum(sums, (M + 127) / 128, N, db, db_dtype, stream);
     if (st) return st;
   }
-  if (dw) {
-    const Packed XT(norm ? ws + s.xt : xt, K, M);
-    if (norm) {
-      // the norm's output again, from the stream, with scales along the tokens
-      st = apa_block_cast(r, dtype, M, K, ld_r, rstd, gamma, gamma_dtype, 0, nullptr, 0, nullptr, XT.q, XT.ld, XT.sc,
-                          nullptr, stream);
-      if (st) return st;
-    }
+  const Packed XT(norm ? ws + s.xt : xt, K, M);
+  if (dw && norm) {
+    // the norm's output again, from the stream, with scales along the tokens
+    st = apa_block_cast(r, dtype, M, K, ld_r, rstd, gamma, gamma_dtype, 0, nullptr, 0, nullptr, XT.q, XT.ld, XT.sc,
+                        nullptr, stream);
+    if (st) return st;
+  }
+  // behind a norm the gradient of its output stays in fp32: rounding it would
+  // add to the rounding of dx and of dgamma's terms
+  void* dh = norm ? static_cast<void*>(ws + s.dh) : dx;
+  const int dh_dtype = norm ? APA_DT_F32 : dtype;
+  const int64_t ld_dh = norm ? K : ld_dx;
+  if (dw && dx) {
+    auto out = [](void* p, int dt, int64_t ld, int64_t rows, int64_t cols) {
+      return OutArgs{p, ld, dt, nullptr, 0, 0, vec16(p, ld, elem_bytes(dt)) ? 1 : 0, (int)rows, (int)cols};
+    };
+    const Operand gw{DYT.q, DYT.ld, DYT.sc, N}, xw{XT.q, XT.ld, XT.sc, K}, gx{DY.q, DY.ld, DY.sc, M}, wx{WT.q, WT.ld, WT.sc, K};
+    const OutArgs ow = out(dw, dw_dtype, ld_dw, N, K), ox = out(dh, dh_dtype, ld_dh, M, K);
+    cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    st = s.dw_first ? block_gemm_dual(gw, xw, M, ow, gx, wx, N, ox, s.split, ws + s.gemm, cs)
+                    : block_gemm_dual(gx, wx, N, ox, gw, xw, M, ow, s.split, ws + s.gemm, cs);
+  } else if (dw) {
     st = apa_block_gemm(DYT.q, DYT.ld, DYT.sc, XT.q, XT.ld, XT.sc, nullptr, 0, dw, dw_dtype, ld_dw, N, K, M, 0,
                         APA_BLOCK_AUTO, ws + s.gemm, s.gemm_bytes, stream);
-    if (st) return st;
+  } else if (dx) {
+    st = apa_block_gemm(DY.q, DY.ld, DY.sc, WT.q, WT.ld, WT.sc, nullptr, 0, dh, dh_dtype, ld_dh, M, K, N, 0,
+                        APA_BLOCK_AUTO, ws + s.gemm, s.gemm_bytes, stream);
   }
-  if (dx) {
-    // behind a norm the gradient of its output stays in fp32: rounding it
-    // would add to the rounding of dx and of dgamma's terms
-    void* dh = norm ? static_cast<void*>(ws + s.dh) : dx;
-    st = apa_block_gemm(DY.q, DY.ld, DY.sc, WT.q, WT.ld, WT.sc, nullptr, 0, dh, norm ? APA_DT_F32 : dtype,
-                        norm ? K : ld_dx, M, K, N, 0, APA_BLOCK_AUTO, ws + s.gemm, s.gemm_bytes, stream);
-    if (st) return st;
-    if (norm)
-      st = apa_rmsnorm_bwd(dh, APA_DT_F32, K, r, ld_r, rstd, gamma, gamma_dtype, dr, ld_dr, dx, ld_dx, dtype, M, K,
-                           dgamma, ws + s.norm, s.norm_bytes, stream);
-  }
+  if (st || !dx || !norm) return st;
+  st = apa_rmsnorm_bwd(dh, APA_DT_F32, K, r, ld_r, rstd, gamma, gamma_dtype, dr, ld_dr, dx, ld_dx, dtype, M, K, dgamma,
+                       ws + s.norm, s.norm_bytes, stream);
   return st;
 }

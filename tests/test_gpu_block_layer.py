@@ -60,6 +60,31 @@ def test_exact_layer(m, k, n, dtype):
     assert np.array_equal(f64(lin.bias_master.grad), f64(dy).sum(0))
 
 
+@pytest.mark.parametrize("limit", [2, 4, 10])
+@pytest.mark.parametrize("m,k,n,dtype", [(700, 600, 300, torch.bfloat16), (2600, 300, 520, torch.float32),
+                                         (260, 530, 2050, torch.float16), (9000, 136, 264, torch.bfloat16)])
+def test_exact_gradients_in_rounds(m, k, n, dtype, limit):
+    """Both gradients' tiles share one launch: on few CTA pairs they take
+    several rounds, with the longer product's last round left incomplete, and
+    the longer one is split where its tiles outlast an even share."""
+    x, w, dy = whole((m, k), 1, 4), whole((n, k), 2, 4), whole((m, n), 3, 2)
+    lin = layer(w)
+    runs = []
+    for sms in (0, limit):             # workspaces are sized without the limit, as when another part sets it
+        xd = x.to(dtype).cuda().requires_grad_(True)
+        lin.weight_master.grad = None
+        blockscale._lib.check(blockscale._lib.lib().apa_set_gemm_sm_limit(sms), "limit")
+        try:
+            y = lin(xd)
+            y.backward(dy.to(dtype).cuda())
+        finally:
+            blockscale._lib.check(blockscale._lib.lib().apa_set_gemm_sm_limit(0), "limit")
+        runs.append((y.detach(), xd.grad, lin.weight_master.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    assert torch.equal(xd.grad.cpu(), torch.from_numpy(f64(dy) @ f64(w)).to(dtype))
+    assert np.array_equal(f64(lin.weight_master.grad), f64(dy).T @ f64(x))
+
+
 def test_gradients_against_differences():
     """On such operands the layer is exactly linear, so differences are exact too."""
     m, k, n = 40, 200, 70
