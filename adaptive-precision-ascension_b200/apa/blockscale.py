@@ -422,9 +422,9 @@ def _norm_backward(dh2, r2, rstd, g, dr2):
         return dx, dg.zero_()
     n = _norm_workspace(M, K, dev.index)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _REAL[dh2.dtype], _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(), g.data_ptr(),
-          _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K, _REAL[r2.dtype], M, K,
-          dg.data_ptr(), ws.data_ptr(), n)
+    _call(dev, "apa_rmsnorm_bwd", dh2.data_ptr(), _REAL[dh2.dtype], _ld(dh2), r2.data_ptr(), _ld(r2), rstd.data_ptr(),
+          g.data_ptr(), _REAL[g.dtype], _lib.ptr(dr2), _ld(dr2) if dr2 is not None else 0, dx.data_ptr(), K,
+          _REAL[r2.dtype], M, K, dg.data_ptr(), ws.data_ptr(), n)
     return dx, dg
 
 
@@ -630,7 +630,7 @@ class APABlockLinear(nn.Module):
     every forward casts the weight anew; without gradients the layer keeps its
     cast weight and renews it when the parameter changed (in place through
     autograd's version counter; call ``refresh_working_copy()`` after changes
-    made behind it, through ``.data``).
+    made behind it, through ``.data`` or by a replayed graph).
 
     ``forward(x, norm=None, residual=None)``: with ``norm`` (an ``APARMSNorm``)
     the layer is applied to ``norm(x)``, or to the normalised sum x + residual;
@@ -654,20 +654,58 @@ class APABlockLinear(nn.Module):
         else:
             self.register_parameter("bias_master", None)
         self._wq: Optional[APABlockTensor] = None
-        self._wq_key: Optional[Tuple] = None       # the parameter that _wq was cast from, and its state then
+        # the parameter that _wq was cast from, its state then, an event behind the cast, the streams behind that
+        self._wq_key: Optional[Tuple] = None
 
     def refresh_working_copy(self) -> None:
         """Cast the weight for calls without gradients (buffers are kept, so a
         captured graph of such a call sees the new values)."""
         W = self.weight_master
         _lib.require_cuda(W, "APABlockLinear.refresh_working_copy")
-        with torch.no_grad():
-            q, _ = _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True)
+        with torch.no_grad(), torch.cuda.device(W.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+            if capturing and self._wq is None:
+                raise RuntimeError("APABlockLinear.refresh_working_copy: nothing to renew in a captured graph; "
+                                   "call it once before the capture")
+            q = self._cast_weight(W)
             if self._wq is not None and self._wq.device == q.device:
                 self._wq.buffer.copy_(q.buffer)
             else:
                 self._wq = q
-        self._wq_key = (W, self._state(W))
+            if not capturing:          # a captured renewal happens when the graph runs
+                done = torch.cuda.Event()
+                done.record()
+                self._wq_key = (W, self._state(W), done, {_lib.stream_handle(W.device)})
+
+    @staticmethod
+    def _cast_weight(W: torch.Tensor) -> APABlockTensor:
+        return _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True)[0]
+
+    def _working_copy(self, W: torch.Tensor) -> APABlockTensor:
+        """The kept cast of W, renewed where W changed and ordered before the
+        current stream's work. A capture that would have to renew it records a
+        cast of its own, which nothing outside the graph sees."""
+        key = self._wq_key
+        handle = _lib.stream_handle(W.device)
+        if key is not None and key[0] is W and key[1] == self._state(W):
+            if handle in key[3]:
+                return self._wq
+            with torch.cuda.device(W.device):
+                if not torch.cuda.is_current_stream_capturing():      # a capture starts behind what it reads
+                    torch.cuda.current_stream().wait_event(key[2])
+                    self._wq.buffer.record_stream(torch.cuda.current_stream())
+                    key[3].add(handle)
+            return self._wq
+        with torch.cuda.device(W.device):
+            if torch.cuda.is_current_stream_capturing():
+                return self._cast_weight(W)
+        self.refresh_working_copy()
+        return self._wq
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        state["_wq"] = state["_wq_key"] = None       # a copy casts its own weight
+        return state
 
     @staticmethod
     def _state(W: torch.Tensor) -> Tuple:
@@ -696,14 +734,12 @@ class APABlockLinear(nn.Module):
                                         or (gamma is not None and gamma.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
             return _BlockLinearFn.apply(x, residual, gamma, W, b, eps)
-        key = self._wq_key
-        if key is None or key[0] is not W or key[1] != self._state(W):
-            self.refresh_working_copy()
+        wq = self._working_copy(W)
         if norm is None:
-            return block_linear(x, self._wq, b)
+            return block_linear(x, wq, b)
         out = rms_norm(x.detach(), gamma.detach(), residual.detach() if residual is not None else None, eps, True)
         q = out if residual is None else out[0]
-        y = block_matmul(q, self._wq, b, x.dtype).view(*x.shape[:-1], self.out_features)
+        y = block_matmul(q, wq, b, x.dtype).view(*x.shape[:-1], self.out_features)
         return y if residual is None else (y, out[1])
 
     def extra_repr(self) -> str:

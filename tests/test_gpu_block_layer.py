@@ -186,6 +186,62 @@ def test_kept_weight_follows_the_parameter():
         assert torch.equal(other(x), 4 * a)
 
 
+def test_kept_weight_and_streams():
+    """A first call on one stream keeps the weight for the next call on another."""
+    x, w = rnd((5, 2048), 1).cuda(), rnd((2048, 2048), 2)
+    want = layer(w)(x).detach()
+    lin = layer(w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for turn in range(3):
+        outs = []
+        with torch.no_grad():
+            for s in streams:
+                with torch.cuda.stream(s):
+                    outs.append(lin(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want * 2 ** turn) for o in outs)
+        with torch.no_grad():
+            lin.weight_master.mul_(2.0)
+        torch.cuda.synchronize()
+
+
+def test_kept_weight_and_captures():
+    """A capture that meets a changed weight casts it in the graph, and leaves
+    the kept one to calls outside."""
+    x, w = rnd((5, 256), 1).cuda(), rnd((192, 256), 2)
+    want = layer(w)(x).detach()
+    lin = layer(w)
+    with torch.no_grad():
+        block_cast(lin.weight_master, square=True), layer(w)(x)          # first launches before the capture
+        torch.cuda.synchronize()
+        fresh = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(fresh):
+            with pytest.raises(RuntimeError, match="before the capture"):
+                lin.refresh_working_copy()
+            y = lin(x)
+        assert lin._wq is None and torch.equal(lin(x), want)
+        fresh.replay()
+        assert torch.equal(y, want)
+        kept = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(kept):
+            z = lin(x)
+        lin.weight_master.mul_(2.0)
+        fresh.replay(), kept.replay()
+        assert torch.equal(y, 2 * want) and torch.equal(z, want)         # z reads the kept cast
+        assert torch.equal(lin(x), 2 * want)                             # renewed in place
+        kept.replay()
+        assert torch.equal(z, 2 * want)
+        lin.weight_master.mul_(2.0)
+        renew = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(renew):
+            lin.refresh_working_copy()
+        kept.replay()
+        assert torch.equal(z, 2 * want)
+        renew.replay(), kept.replay()
+        assert torch.equal(z, 4 * want) and torch.equal(lin(x), 4 * want)
+
+
 def test_kept_weight_of_another_parameter():
     import copy
     lin = layer(rnd((40, 64), 1))
