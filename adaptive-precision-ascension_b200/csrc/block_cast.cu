@@ -20,6 +20,11 @@
 // a thread leave room for two CTAs per SM. (8 x 8 pieces on 256 threads ran at
 // a third of the speed; persistent CTAs with the next tile fetched ahead by
 // cp.async gained nothing in bf16 and lost a third in fp32.)
+//
+// Measured on a B200, inputs in HBM, 8192 x 4096 (us, TB/s of what is read and
+// written): bf16 rows form 20.5, 4.9; cols 23.9, 4.2; both 30.3, 4.4, with ALU
+// pipe and issue slots 57 and 61 % busy; fp32 rows 26.3, 6.4; both 34.2, 5.9.
+// Dequantisation to bf16 19.4, 5.2.
 #include "block_scale.cuh"
 
 namespace apa {
@@ -329,7 +334,8 @@ CastArgs cast_args(const void* src, int es, int64_t rows, int64_t cols, int64_t 
                    const void* col_mul, int col_mul_dt, void* dst, int64_t ld_dst, void* sc, void* dst_t,
                    int64_t ld_dst_t, void* sc_t, float* colsum) {
   return CastArgs{src, rows, cols, ld_src, row_mul, col_mul, col_mul_dt, static_cast<uint8_t*>(dst), ld_dst,
-                  static_cast<uint8_t*>(sc), static_cast<uint8_t*>(dst_t), ld_dst_t, static_cast<uint8_t*>(sc_t), colsum,
+                  static_cast<uint8_t*>(sc), static_cast<uint8_t*>(dst_t), ld_dst_t, static_cast<uint8_t*>(sc_t),
+                  colsum,
                   vec16(src, ld_src, es) ? 1 : 0, vec16(col_mul, 8, 4) ? 1 : 0, (cols + 127) / 128};
 }
 

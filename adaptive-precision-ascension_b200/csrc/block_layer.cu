@@ -92,7 +92,8 @@ int bwd_space(int64_t M, int64_t N, int64_t K, int flags, int dtype, int dw_dtyp
   } else if (dw) {
     if (int st = apa_block_gemm_workspace(N, K, M, dw_dtype, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
   } else if (dx) {
-    if (int st = apa_block_gemm_workspace(M, K, N, norm ? APA_DT_F32 : dtype, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
+    const int dt = norm ? APA_DT_F32 : dtype;
+    if (int st = apa_block_gemm_workspace(M, K, N, dt, APA_BLOCK_AUTO, &s->gemm_bytes)) return st;
   }
   s->gemm = take(s->gemm_bytes);
   s->total = at;
@@ -162,10 +163,11 @@ extern "C" int apa_block_linear_fwd(const void* x, int x_dtype, int64_t ld_x, co
       st = apa_block_cast(w, w_dtype, N, K, ld_w, nullptr, nullptr, 0, 1, W.q, W.ld, W.sc, WT.q, WT.ld, WT.sc, nullptr,
                           stream);
   } else {
-    st = cast_pair(cast_args(w, elem_bytes(w_dtype), N, K, ld_w, nullptr, nullptr, 0, W.q, W.ld, W.sc, WT.q, WT.ld, WT.sc,
-                             nullptr), w_dtype,
-                   cast_args(x, elem_bytes(x_dtype), M, K, ld_x, nullptr, nullptr, 0, X.q, X.ld, X.sc, XT.q, XT.ld, XT.sc,
-                             nullptr), x_dtype, static_cast<cudaStream_t>(stream));
+    const CastArgs cw = cast_args(w, elem_bytes(w_dtype), N, K, ld_w, nullptr, nullptr, 0, W.q, W.ld, W.sc, WT.q,
+                                  WT.ld, WT.sc, nullptr);
+    const CastArgs cx = cast_args(x, elem_bytes(x_dtype), M, K, ld_x, nullptr, nullptr, 0, X.q, X.ld, X.sc, XT.q,
+                                  XT.ld, XT.sc, nullptr);
+    st = cast_pair(cw, w_dtype, cx, x_dtype, static_cast<cudaStream_t>(stream));
   }
   if (st) return st;
   return apa_block_gemm(X.q, X.ld, X.sc, W.q, W.ld, W.sc, bias, bias_dtype, y, y_dtype, ld_y, M, N, K, 0,
@@ -232,7 +234,8 @@ extern "C" int apa_block_linear_bwd(const void* dy, int dy_dtype, int64_t ld_dy,
     auto out = [](void* p, int dt, int64_t ld, int64_t rows, int64_t cols) {
       return OutArgs{p, ld, dt, nullptr, 0, 0, vec16(p, ld, elem_bytes(dt)) ? 1 : 0, (int)rows, (int)cols};
     };
-    const Operand gw{DYT.q, DYT.ld, DYT.sc, N}, xw{XT.q, XT.ld, XT.sc, K}, gx{DY.q, DY.ld, DY.sc, M}, wx{WT.q, WT.ld, WT.sc, K};
+    const Operand gw{DYT.q, DYT.ld, DYT.sc, N}, xw{XT.q, XT.ld, XT.sc, K};
+    const Operand gx{DY.q, DY.ld, DY.sc, M}, wx{WT.q, WT.ld, WT.sc, K};
     const OutArgs ow = out(dw, dw_dtype, ld_dw, N, K), ox = out(dh, dh_dtype, ld_dh, M, K);
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     st = s.dw_first ? block_gemm_dual(gw, xw, M, ow, gx, wx, N, ox, s.split, ws + s.gemm, cs)

@@ -397,3 +397,28 @@ def test_second_derivatives_are_refused():
         (g,) = torch.autograd.grad(out.sum(), [x], create_graph=True)
         with pytest.raises(RuntimeError):          # no gradient of it, or none a second time
             g.sum().backward()
+
+
+def test_offsets_past_32_bits():
+    """A training step over more than 2^31 activations, on whole numbers: the
+    weight gradient's sums stay below 2^24, so all of it is exact."""
+    m, k, n = 525_000, 4096, 72
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def draw(rows, cols, top):
+        return torch.randint(-top, top + 1, (rows, cols), generator=g, device="cuda", dtype=torch.int8)
+
+    x, dy, w = draw(m, k, 3).to(torch.bfloat16), draw(m, n, 2).to(torch.bfloat16), draw(n, k, 3).float()
+    assert x.numel() > 2 ** 31
+    lin = layer(w)
+    x.requires_grad_(True)
+    y = lin(x)
+    y.backward(dy)
+    want = torch.zeros(n, k, device="cuda", dtype=torch.float64)
+    with torch.no_grad():
+        for lo in range(0, m, 75_000):
+            want += dy[lo:lo + 75_000].double().T @ x[lo:lo + 75_000].double()
+        assert torch.equal(lin.weight_master.grad.double(), want)
+        for lo in (0, 262_100, m - 300):
+            assert torch.equal(y[lo:lo + 300], (x[lo:lo + 300].double() @ w.double().T).to(torch.bfloat16))
+            assert torch.equal(x.grad[lo:lo + 300], (dy[lo:lo + 300].double() @ w.double()).to(torch.bfloat16))

@@ -434,3 +434,36 @@ def test_column_sums_of_infinite_gradients():
     blockscale._cast(x.cuda(), True, True, colsum=sums)
     got = sums.sum(0).cpu()
     assert got[3] == float("inf") and torch.isnan(got[4]) and bool((got[5:] == 300).all())
+
+
+def whole_rows(m, k, seed, top):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(-top, top + 1, (m, k), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the source, the codes, the transposed codes
+    and the output: whole numbers, so every row is exact."""
+    from apa import blockscale
+    m, k, n = 525_000, 4096, 4104
+    x = whole_rows(m, k, 1, 7)
+    assert x.numel() > 2 ** 31
+    q, t = blockscale._cast(x, True, True)
+    back = q.dequantize(torch.bfloat16)
+    assert torch.equal(back, x)
+    del back
+    back = t.dequantize(torch.bfloat16)
+    for c in (0, 2049, 4095):
+        assert torch.equal(back[c], x[:, c])
+    del back
+    w = whole_rows(72, k, 2, 3)
+    y = block_matmul(q, block_cast(w, square=True), out_dtype=torch.float32)
+    for lo in (0, 262_100, m - 300):
+        assert torch.equal(y[lo:lo + 300].double(), x[lo:lo + 300].double() @ w.double().T)
+    del q, t, y, x
+    a, b = whole_rows(m, 128, 3, 7), whole_rows(n, 128, 4, 3)
+    out = block_matmul(block_cast(a), block_cast(b, square=True), out_dtype=torch.bfloat16)
+    assert out.numel() > 2 ** 31
+    for lo in (0, 262_100, m - 300):
+        want = (a[lo:lo + 300].double() @ b.double().T).to(torch.bfloat16)
+        assert torch.equal(out[lo:lo + 300], want)

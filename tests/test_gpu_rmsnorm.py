@@ -223,3 +223,25 @@ def test_deterministic_and_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+def test_offsets_past_32_bits():
+    """Rows behind 2^31 elements equal those of a call on them alone."""
+    m, k = 525_000, 4096
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(m, k, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    assert x.numel() > 2 ** 31
+    w = torch.rand(k, generator=g, device="cuda")
+    lo = m - 512
+    tail = x[lo:].clone()
+    y, r = rms_norm(x, w, residual=x)
+    y1, r1 = rms_norm(tail, w, residual=tail)
+    assert torch.equal(y[lo:], y1) and torch.equal(r[lo:], r1)
+    del y
+    q = rms_norm(r, w, quantize=True)
+    assert torch.equal(q.dequantize()[lo:], rms_norm(r1, w, quantize=True).dequantize())
+    del q
+    rstd = torch.rand(m, generator=g, device="cuda")
+    dx, _ = blockscale._norm_backward(x, r, rstd, w, x)
+    dx1, _ = blockscale._norm_backward(tail, r1, rstd[lo:].clone(), w, tail)
+    assert torch.equal(dx[lo:], dx1)
