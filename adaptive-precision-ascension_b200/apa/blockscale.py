@@ -232,10 +232,10 @@ _NONE = (None, 0, None)
 
 
 def _cast(x2: torch.Tensor, rows_form: bool, cols_form: bool, square: bool = False, colsum=None, row_mul=None,
-          col_mul=None):
+          col_mul=None, into: Optional[APABlockTensor] = None):
     rows, cols = x2.shape
     dev = x2.device
-    q = _new_block(rows, cols, dev) if rows_form else None
+    q = (into or _new_block(rows, cols, dev)) if rows_form else None
     qt = _new_block(cols, rows, dev) if cols_form else None
     if rows == 0:
         return q, qt
@@ -320,12 +320,16 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     """x W^T + bias for serving. x [..., K] is cast to E4M3 here, or comes as an
     APABlockTensor (from ``rms_norm(..., quantize=True)``); ``weight`` [N, K] is
     ``block_cast(w, square=True)``. ``out_dtype`` defaults to x's type
-    (bfloat16 for an APABlockTensor). Not differentiable."""
+    (bfloat16 for an APABlockTensor). Not differentiable (an x that wants a
+    gradient is refused)."""
     if isinstance(x, APABlockTensor):
         return block_matmul(x, weight, bias, out_dtype or torch.bfloat16)
     if not isinstance(weight, APABlockTensor):
         raise TypeError("block_linear: the weight must be an APABlockTensor (block_cast(w, square=True))")
     x2 = _matrix(x, "block_linear")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("block_linear: has no gradient; call it under torch.no_grad(), or train through "
+                           "APABlockLinear")
     code = _real(x2.dtype, "block_linear")
     _lib.require_cuda(x2, "block_linear")
     M, K = x2.shape
@@ -667,19 +671,19 @@ class APABlockLinear(nn.Module):
             if capturing and self._wq is None:
                 raise RuntimeError("APABlockLinear.refresh_working_copy: nothing to renew in a captured graph; "
                                    "call it once before the capture")
-            q = self._cast_weight(W)
-            if self._wq is not None and self._wq.device == q.device:
-                self._wq.buffer.copy_(q.buffer)
-            else:
-                self._wq = q
+            kept = self._wq
+            if kept is not None and (kept.device != W.device or kept.shape != W.shape):
+                kept = None
+            self._wq = self._cast_weight(W, kept)
             if not capturing:          # a captured renewal happens when the graph runs
                 done = torch.cuda.Event()
                 done.record()
                 self._wq_key = (W, self._state(W), done, {_lib.stream_handle(W.device)})
 
     @staticmethod
-    def _cast_weight(W: torch.Tensor) -> APABlockTensor:
-        return _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True)[0]
+    def _cast_weight(W: torch.Tensor, into: Optional[APABlockTensor] = None) -> APABlockTensor:
+        # written by the kernel alone: a buffer made in inference mode allows no torch operation in place
+        return _cast(_matrix(W.detach(), "APABlockLinear: weight"), True, False, square=True, into=into)[0]
 
     def _working_copy(self, W: torch.Tensor) -> APABlockTensor:
         """The kept cast of W, renewed where W changed and ordered before the

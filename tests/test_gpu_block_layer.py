@@ -242,6 +242,21 @@ def test_kept_weight_and_captures():
         assert torch.equal(z, 4 * want) and torch.equal(lin(x), 4 * want)
 
 
+def test_kept_weight_made_in_inference_mode():
+    """Kept under inference_mode, renewed outside it."""
+    x, w = rnd((5, 256), 1).cuda(), rnd((192, 256), 2)
+    lin = layer(w)
+    with torch.inference_mode():
+        a = lin(x)
+    kept = lin._wq.buffer.data_ptr()
+    with torch.no_grad():
+        lin.weight_master.mul_(2.0)
+        b = lin(x)
+    assert torch.equal(b, 2 * a) and lin._wq.buffer.data_ptr() == kept
+    y = lin(x.clone().requires_grad_(True))
+    assert torch.equal(y.detach(), b)
+
+
 def test_kept_weight_of_another_parameter():
     import copy
     lin = layer(rnd((40, 64), 1))

@@ -467,3 +467,13 @@ def test_offsets_past_32_bits():
     for lo in (0, 262_100, m - 300):
         want = (a[lo:lo + 300].double() @ b.double().T).to(torch.bfloat16)
         assert torch.equal(out[lo:lo + 300], want)
+
+
+def test_linear_refuses_inputs_that_want_gradients():
+    x = torch.randn(3, 64, device="cuda", requires_grad=True)
+    w = block_cast(torch.randn(40, 64, device="cuda"), square=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        block_linear(x, w)
+    with torch.no_grad():
+        y = block_linear(x, w)
+    assert torch.equal(block_linear(x.detach(), w), y)
