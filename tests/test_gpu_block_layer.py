@@ -437,3 +437,54 @@ def test_offsets_past_32_bits():
         for lo in (0, 262_100, m - 300):
             assert torch.equal(y[lo:lo + 300], (x[lo:lo + 300].double() @ w.double().T).to(torch.bfloat16))
             assert torch.equal(x.grad[lo:lo + 300], (dy[lo:lo + 300].double() @ w.double()).to(torch.bfloat16))
+
+
+def test_two_steps_at_once():
+    """Two layers' training steps on two streams, queued in turn by two threads,
+    and then as two captured graphs replayed together: each gives what it gives
+    alone, bit for bit."""
+    import threading
+
+    parts = []
+    for seed, (m, k, n) in enumerate([(2100, 640, 1500), (700, 2048, 520)]):
+        lin = layer(rnd((n, k), seed), rnd((n,), seed + 5))
+        norm = APARMSNorm(k, config=APAConfig(device="cuda"))
+        x = rnd((m, k), seed + 10, torch.bfloat16).cuda().requires_grad_(True)
+        parts.append((lin, norm, x, rnd((m, n), seed + 20, torch.bfloat16).cuda(), torch.cuda.Stream()))
+
+    def step(p):
+        lin, norm, x, dy, _ = p
+        y = lin(x, norm=norm)
+        return (y.detach(),) + torch.autograd.grad(y, [x, norm.weight, lin.weight_master, lin.bias_master], dy)
+
+    alone = [step(p) for p in parts]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(parts[i][4]):
+            for _ in range(8):
+                got[i].append(step(parts[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        assert len(outs) == 8 and all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+
+    graphs = []
+    for p in parts:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=p[4]):
+            out = step(p)
+        graphs.append((g, out))
+    for _ in range(4):
+        for p, (g, _) in zip(parts, graphs):
+            with torch.cuda.stream(p[4]):
+                g.replay()
+    torch.cuda.synchronize()
+    for want, (_, out) in zip(alone, graphs):
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
