@@ -31,11 +31,13 @@
 //   overlap by 16 columns: the next tile's MMAs start as soon as the epilogue
 //   has read the shared columns, which it reads first. Measured: 8192 x 4096 x
 //   4096 (bf16 out) 106 us, 2.6 PFLOP/s, and 33 us with a reduction of 1024. A
-//   slab takes 634 cycles where the MMAs alone take 512: both CTAs of a pair
-//   read A and B from shared memory at its full rate, which bounds the kernel
-//   while the clock holds (a long run of it is held to 1.3 GHz by the power
-//   limit); handing over a tile costs 130 cycles. The scales cost 1.5 %
-//   (copies) and 4 % (a scaled MMA against a plain one).
+//   slab takes 634 cycles where the MMAs alone take 512: per slab an SM's shared
+//   memory takes in 32 KB and gives 48 KB (A's own rows, all of B) to the MMA,
+//   640 cycles at 128 bytes each. With eight slabs a tile it is 720, as the
+//   epilogue's staging passes there too, and 13 % of the time the operands are
+//   late: L2 delivers 13 TB/s. A long run is held to 1.3 GHz by the power limit.
+//   Handing over a tile costs 130 cycles, copying scales 1.5 %, a scaled MMA
+//   4 % over a plain one.
 #include <cuda.h>
 #include <cmath>
 #include "block_scale.cuh"
@@ -480,6 +482,12 @@ struct Problem {
 
 struct ProblemMaps { CUtensorMap a, b, sa, sb, o; };
 
+// Column sums of [parts, cols] fp32 partials (a bias gradient's, which the cast
+// of the gradient left), added in order and rounded once. In this launch they
+// save their own: a step of 1111 x 520 x 1000 takes 33.5 us with, 37 without,
+// 16384 x 384 x 1536 89.8 and 91.1.
+struct ColumnSums { const float* part; int parts, cols; void* out; int out_dt; };
+
 // NP products in one launch. Units (tile, split) go round the CTA pairs. With
 // two products, `units0` units of the first, the longer ones, are dealt first;
 // they may end in the middle of a round, so the pairs from `late` on, which
@@ -488,6 +496,7 @@ struct ProblemMaps { CUtensorMap a, b, sa, sb, o; };
 template <int NP> struct PairArgs {
   Problem q[NP];
   int units0, units1, late, extra;
+  ColumnSums sums;
 };
 template <int NP> struct PairMaps { ProblemMaps m[NP]; };
 
@@ -728,6 +737,23 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
     const int q = warp & 3, e = warp - 2, part = e >> 2;
     uint8_t* boxes = smE + e * C::kBoxes * kEpiBox;
     float* sb = smBias + e * C::kWarpCols;
+    if constexpr (NP == 2) {
+      // done while the first tile is under way; sixteen loads at a time
+      if (p.sums.part != nullptr) {
+        const ColumnSums& t = p.sums;
+        for (int c = ((int)blockIdx.x * EW + e) * 32 + lane; c < t.cols; c += (int)gridDim.x * EW * 32) {
+          float x = 0.0f;
+          for (int r = 0; r < t.parts; r += 16) {
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = r + k < t.parts ? __ldcg(t.part + (int64_t)(r + k) * t.cols + c) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x += v[k];
+          }
+          from_f32(t.out, t.out_dt, c, x);
+        }
+      }
+    }
     int local = 0;
     int slot = 0, inflight = 0;           // staging ring; TMA stores that may still read their box
     const uint32_t te0 = gemm::map_to_cta(&tempty[0], 0), te1 = gemm::map_to_cta(&tempty[1], 0);
@@ -1059,6 +1085,7 @@ template <int EW>
 int launch_pair(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, int splits, void* ws, cudaStream_t s) {
   PairMaps<1> m;
   PairArgs<1> p;
+  p.sums = ColumnSums{};
   if (int st = fill_problem(A, B, K, o, splits, ws, &m.m[0], &p.q[0])) return st;
   if (int st = launch_pairs<EW, 1>(m, p, pair_units(o, splits), 0, s)) return st;
   return splits > 1 ? launch_sum(o, splits, ws, s) : APA_OK;
@@ -1162,10 +1189,16 @@ int dual_split(const OutArgs& o0, int64_t K0, const OutArgs& o1, int64_t K1) {
   return (int)std::max<int64_t>(1, std::min(std::min(cdiv64(kb0 + 2, share), kb0 / 8), (int64_t)64));
 }
 
+// Whether the launch's epilogue warps can add `parts` rows of column sums
+// before their first tile is done: a row costs them 100 cycles, a slab 634.
+bool dual_adds(int64_t parts, int64_t K0, int split) { return parts <= 4 * cdiv64(cdiv64(K0, kSlab), split); }
+
 int block_gemm_dual(const Operand& A0, const Operand& B0, int64_t K0, const OutArgs& o0, const Operand& A1,
-                    const Operand& B1, int64_t K1, const OutArgs& o1, int split, void* ws, cudaStream_t s) {
+                    const Operand& B1, int64_t K1, const OutArgs& o1, const ColumnSums& sums, int split, void* ws,
+                    cudaStream_t s) {
   PairMaps<2> m;
   PairArgs<2> p;
+  p.sums = sums;
   if (int st = fill_problem(A0, B0, K0, o0, split, ws, &m.m[0], &p.q[0])) return st;
   if (int st = fill_problem(A1, B1, K1, o1, 1, nullptr, &m.m[1], &p.q[1])) return st;
   const int64_t u0 = pair_units(o0, split), u1 = pair_units(o1, 1);

@@ -214,8 +214,12 @@ extern "C" int apa_block_linear_bwd(const void* dy, int dy_dtype, int64_t ld_dy,
   int st = apa_block_cast(dy, dy_dtype, M, N, ld_dy, nullptr, nullptr, 0, 0, DY.q, DY.ld, DY.sc, DYT.q, DYT.ld, DYT.sc,
                           sums, stream);
   if (st) return st;
-  if (db) {
-    st = apa_block_colsum(sums, (M + 127) / 128, N, db, db_dtype, stream);
+  // with both products to come, their launch adds the column sums
+  const bool both = dw && dx;
+  const int64_t parts = (M + 127) / 128;
+  const bool later = db && both && dual_adds(parts, s.dw_first ? M : N, s.split);
+  if (db && !later) {
+    st = apa_block_colsum(sums, parts, N, db, db_dtype, stream);
     if (st) return st;
   }
   const Packed XT(norm ? ws + s.xt : xt, K, M);
@@ -230,16 +234,17 @@ extern "C" int apa_block_linear_bwd(const void* dy, int dy_dtype, int64_t ld_dy,
   void* dh = norm ? static_cast<void*>(ws + s.dh) : dx;
   const int dh_dtype = norm ? APA_DT_F32 : dtype;
   const int64_t ld_dh = norm ? K : ld_dx;
-  if (dw && dx) {
+  if (both) {
     auto out = [](void* p, int dt, int64_t ld, int64_t rows, int64_t cols) {
       return OutArgs{p, ld, dt, nullptr, 0, 0, vec16(p, ld, elem_bytes(dt)) ? 1 : 0, (int)rows, (int)cols};
     };
     const Operand gw{DYT.q, DYT.ld, DYT.sc, N}, xw{XT.q, XT.ld, XT.sc, K};
     const Operand gx{DY.q, DY.ld, DY.sc, M}, wx{WT.q, WT.ld, WT.sc, K};
     const OutArgs ow = out(dw, dw_dtype, ld_dw, N, K), ox = out(dh, dh_dtype, ld_dh, M, K);
+    const ColumnSums sum = later ? ColumnSums{sums, (int)parts, (int)N, db, db_dtype} : ColumnSums{};
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    st = s.dw_first ? block_gemm_dual(gw, xw, M, ow, gx, wx, N, ox, s.split, ws + s.gemm, cs)
-                    : block_gemm_dual(gx, wx, N, ox, gw, xw, M, ow, s.split, ws + s.gemm, cs);
+    st = s.dw_first ? block_gemm_dual(gw, xw, M, ow, gx, wx, N, ox, sum, s.split, ws + s.gemm, cs)
+                    : block_gemm_dual(gx, wx, N, ox, gw, xw, M, ow, sum, s.split, ws + s.gemm, cs);
   } else if (dw) {
     st = apa_block_gemm(DYT.q, DYT.ld, DYT.sc, XT.q, XT.ld, XT.sc, nullptr, 0, dw, dw_dtype, ld_dw, N, K, M, 0,
                         APA_BLOCK_AUTO, ws + s.gemm, s.gemm_bytes, stream);

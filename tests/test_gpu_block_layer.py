@@ -66,23 +66,25 @@ def test_exact_layer(m, k, n, dtype):
 def test_exact_gradients_in_rounds(m, k, n, dtype, limit):
     """Both gradients' tiles share one launch: on few CTA pairs they take
     several rounds, with the longer product's last round left incomplete, and
-    the longer one is split where its tiles outlast an even share."""
+    the longer one is split where its tiles outlast an even share. The bias
+    gradient's sums come from the same launch or, past few slabs, their own."""
     x, w, dy = whole((m, k), 1, 4), whole((n, k), 2, 4), whole((m, n), 3, 2)
-    lin = layer(w)
+    lin = layer(w, whole((n,), 4))
     runs = []
     for sms in (0, limit):             # workspaces are sized without the limit, as when another part sets it
         xd = x.to(dtype).cuda().requires_grad_(True)
-        lin.weight_master.grad = None
+        lin.weight_master.grad = lin.bias_master.grad = None
         blockscale._lib.check(blockscale._lib.lib().apa_set_gemm_sm_limit(sms), "limit")
         try:
             y = lin(xd)
             y.backward(dy.to(dtype).cuda())
         finally:
             blockscale._lib.check(blockscale._lib.lib().apa_set_gemm_sm_limit(0), "limit")
-        runs.append((y.detach(), xd.grad, lin.weight_master.grad))
+        runs.append((y.detach(), xd.grad, lin.weight_master.grad, lin.bias_master.grad))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
     assert torch.equal(xd.grad.cpu(), torch.from_numpy(f64(dy) @ f64(w)).to(dtype))
     assert np.array_equal(f64(lin.weight_master.grad), f64(dy).T @ f64(x))
+    assert np.array_equal(f64(lin.bias_master.grad), f64(dy).sum(0))
 
 
 def test_gradients_against_differences():
