@@ -1058,6 +1058,13 @@ int launch_sum(const OutArgs& o, int splits, const void* ws, cudaStream_t s) {
                        q) == cudaSuccess ? APA_OK : APA_ERR_CUDA;
 }
 
+// A unit's time in slabs, two of them to hand a tile over. Where TMA cannot store
+// the rows, a tile takes twelve for its epilogue at least (both gradients of
+// 100000 x 100 x 100 74 us, counted by slabs alone 97). A floor of six for the
+// other tiles, their epilogue's time, made the split too coarse: 512 x 4096 x
+// 4096 35 us against 31.
+int64_t unit_cost(int64_t slabs, bool tma_out) { return (tma_out ? slabs : std::max<int64_t>(slabs, 12)) + 2; }
+
 int64_t pair_units(const OutArgs& o, int splits) { return cdiv64(o.M, 256) * cdiv64(o.N, 256) * splits; }
 
 template <int EW, int NP>
@@ -1072,7 +1079,8 @@ int launch_pairs(const PairMaps<NP>& maps, PairArgs<NP>& p, int64_t units0, int6
   p.late = 0; p.extra = 0;
   if (NP == 2) {
     // how many of the second product's units a unit of the first is worth
-    const int64_t c0 = cdiv64(p.q[0].kb_count, p.q[0].splits) + 2, c1 = p.q[NP - 1].kb_count + 2;
+    const Problem &a = p.q[0], &b = p.q[NP - 1];
+    const int64_t c0 = unit_cost(cdiv64(a.kb_count, a.splits), a.tma_out), c1 = unit_cost(b.kb_count, b.tma_out);
     p.late = (int)(units0 % pairs);
     const int64_t worth = std::max<int64_t>(1, (2 * c0 + c1) / (2 * c1));
     p.extra = p.late ? (int)std::min(worth, cdiv64(units1, pairs - p.late)) : 0;
@@ -1177,16 +1185,20 @@ int block_gemm(const Operand& A, const Operand& B, int64_t K, const OutArgs& o, 
 // different casts of the same gradient. One launch less, and the second fills
 // the CTA pairs that the first leaves idle in its last round (4096 x 4096 over
 // 8192 tokens: 256 and 512 tiles on 74 pairs; the training step of that layer
-// takes 392 us with both in one launch, 410 with two). The first is split when
-// a tile of it would take longer than an even share of all the work.
+// takes 392 us with both in one launch, 410 with two; the casts and both
+// gradients alone, in one launch and in two: 1 x 4096 x 4096 29.5 and 31, 512 x
+// 4096 x 4096 31 and 44, 16384 x 384 x 1536 58 and 66, 33280 x 512 x 512 49 and
+// 58). The first is split when a tile of it would take longer than an even share
+// of all the work.
 int dual_split(const OutArgs& o0, int64_t K0, const OutArgs& o1, int64_t K1) {
   const int64_t pairs = std::max(1, num_sms() / 2);
   const int64_t kb0 = cdiv64(K0, kSlab), kb1 = cdiv64(K1, kSlab);
-  // two slabs' time to hand a tile over
-  const int64_t work = pair_units(o0, 1) * (kb0 + 2) + pair_units(o1, 1) * (kb1 + 2);
-  const int64_t share = std::max<int64_t>(cdiv64(work, pairs), kb1 + 2);
+  const auto tma = [](const OutArgs& o) { return (int64_t)o.N * elem_bytes(o.out_dt) % 16 == 0; };
+  const int64_t c0 = unit_cost(kb0, tma(o0)), c1 = unit_cost(kb1, tma(o1));
+  const int64_t work = pair_units(o0, 1) * c0 + pair_units(o1, 1) * c1;
+  const int64_t share = std::max<int64_t>(cdiv64(work, pairs), c1);
   // a split unit of less than eight slabs costs more to add than it gains
-  return (int)std::max<int64_t>(1, std::min(std::min(cdiv64(kb0 + 2, share), kb0 / 8), (int64_t)64));
+  return (int)std::max<int64_t>(1, std::min(std::min(cdiv64(c0, share), kb0 / 8), (int64_t)64));
 }
 
 // Whether the launch's epilogue warps can add `parts` rows of column sums

@@ -85,7 +85,8 @@ int bwd_space(int64_t M, int64_t N, int64_t K, int flags, int dtype, int dw_dtyp
   if (dw && dx) {
     // both products in one launch, the one with the longer tiles first
     OutArgs ow{}, ox{};
-    ow.M = (int)N; ow.N = (int)K; ox.M = (int)M; ox.N = (int)K;
+    ow.M = (int)N; ow.N = (int)K; ow.out_dt = dw_dtype;
+    ox.M = (int)M; ox.N = (int)K; ox.out_dt = norm ? APA_DT_F32 : dtype;
     s->dw_first = M >= N;
     s->split = s->dw_first ? dual_split(ow, M, ox, N) : dual_split(ox, N, ow, M);
     s->gemm_bytes = s->dw_first ? split_bytes(N, K, s->split) : split_bytes(M, K, s->split);
