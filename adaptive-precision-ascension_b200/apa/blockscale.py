@@ -634,7 +634,9 @@ class APABlockLinear(nn.Module):
     every forward casts the weight anew; without gradients the layer keeps its
     cast weight and renews it when the parameter changed (in place through
     autograd's version counter; call ``refresh_working_copy()`` after changes
-    made behind it, through ``.data`` or by a replayed graph).
+    made behind it, through ``.data`` or by a replayed graph). A weight made
+    under ``torch.inference_mode()`` has no such counter and is cast on every
+    call.
 
     ``forward(x, norm=None, residual=None)``: with ``norm`` (an ``APARMSNorm``)
     the layer is applied to ``norm(x)``, or to the normalised sum x + residual;
@@ -689,6 +691,10 @@ class APABlockLinear(nn.Module):
         """The kept cast of W, renewed where W changed and ordered before the
         current stream's work. A capture that would have to renew it records a
         cast of its own, which nothing outside the graph sees."""
+        if W.is_inference():
+            # it has no version counter, and inference mode may change it in place: nothing shows whether a cast still holds
+            with torch.cuda.device(W.device):
+                return self._cast_weight(W)
         key = self._wq_key
         handle = _lib.stream_handle(W.device)
         if key is not None and key[0] is W and key[1] == self._state(W):
@@ -713,7 +719,7 @@ class APABlockLinear(nn.Module):
 
     @staticmethod
     def _state(W: torch.Tensor) -> Tuple:
-        # tensors made in inference mode have no version; they cannot change in place outside it
+        # a tensor made in inference mode has no version, so its cast is never taken as current
         return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):

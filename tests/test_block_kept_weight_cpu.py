@@ -1,0 +1,116 @@
+"""The cast weight that a block layer keeps, without a GPU: streams, events and
+the cast are stand-ins that note what happens in which order."""
+import contextlib
+import threading
+
+import pytest
+import torch
+
+from apa import APABlockLinear, APAConfig, _lib, blockscale
+
+W0 = torch.arange(12.0).view(3, 4)
+
+
+class Stream:
+    def __init__(self, handle, log):
+        self.cuda_stream, self.log, self.capturing = handle, log, False
+
+    def wait_event(self, event):
+        self.log.append(("wait", self.cuda_stream, event.after))
+
+    def wait_stream(self, other):
+        self.log.append(("wait", self.cuda_stream, ("stream", other.cuda_stream)))
+
+
+class Buffer:
+    """Stands for the packed cast: holds the values it was cast from."""
+    device = torch.device("cpu")
+
+    def __init__(self, shape, log):
+        self.shape, self.buffer, self.log, self.values = shape, self, log, None
+
+    def record_stream(self, stream):
+        self.log.append(("record", id(self), stream.cuda_stream))
+
+    def data_ptr(self):
+        return id(self)
+
+
+@pytest.fixture
+def stage(monkeypatch):
+    """A layer whose casts, streams and events are noted in ``stage.log``."""
+    class Stage:
+        pass
+    stage = Stage()
+    stage.log, stage.local = [], threading.local()
+    stage.streams = {h: Stream(h, stage.log) for h in (1, 2, 3)}
+    stage.during_cast = lambda: None
+    here = lambda *a: stage.streams[getattr(stage.local, "handle", 1)]
+
+    class Event:
+        after = None
+
+        def record(self, stream=None):
+            self.after = ("event", (stream or here()).cuda_stream)
+
+    @contextlib.contextmanager
+    def on(stream):
+        before = getattr(stage.local, "handle", 1)
+        stage.local.handle = stream if isinstance(stream, int) else stream.cuda_stream
+        try:
+            yield
+        finally:
+            stage.local.handle = before
+
+    def cast(W, into=None):
+        buf = into or Buffer(W.shape, stage.log)
+        stage.log.append(("cast", here().cuda_stream, id(buf)))
+        stage.during_cast()
+        buf.values = W.detach().clone()
+        return buf
+
+    stage.on = on
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", here)
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: here().capturing)
+    monkeypatch.setattr(_lib, "stream_handle", lambda d=None: here().cuda_stream)
+    monkeypatch.setattr(_lib, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(APABlockLinear, "_cast_weight", staticmethod(cast))
+
+    def make():
+        lin = APABlockLinear(4, 3, bias=False, config=APAConfig(device="cpu"))
+        with torch.no_grad():
+            lin.weight_master.copy_(W0)
+        return lin
+
+    stage.make = make
+    stage.casts = lambda: [e for e in stage.log if e[0] == "cast"]
+    return stage
+
+
+def served(lin):
+    """The values that a call without gradients would use now."""
+    return lin._working_copy(lin.weight_master).values
+
+
+def test_cast_once_while_nothing_changes(stage):
+    lin = stage.make()
+    for _ in range(3):
+        assert torch.equal(served(lin), W0)
+    assert len(stage.casts()) == 1
+    with torch.no_grad():
+        lin.weight_master.mul_(2.0)
+    assert torch.equal(served(lin), 2 * W0) and len(stage.casts()) == 2
+
+
+def test_weight_made_and_changed_in_inference_mode(stage):
+    with torch.inference_mode():
+        lin = stage.make()
+        assert torch.equal(served(lin), W0)
+        lin.weight_master.mul_(2.0)
+        assert torch.equal(served(lin), 2 * W0)
+        lin.refresh_working_copy()
+        lin.load_state_dict({"weight_master": W0 + 1})
+        assert torch.equal(served(lin), W0 + 1)

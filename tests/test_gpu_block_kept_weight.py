@@ -1,0 +1,41 @@
+"""The cast weight that a block layer keeps for calls without gradients, on the
+GPU: every change of the parameter shows in the next call, whatever made it.
+Scaling a weight by a power of two scales the layer's output exactly, and whole
+numbers of few bits make every product exact, so all comparisons are bit for bit."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from apa import APABlockLinear, APAConfig
+
+
+def rnd(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def layer(w, dtype=torch.float32):
+    lin = APABlockLinear(w.shape[1], w.shape[0], bias=False, dtype=dtype, config=APAConfig(device="cuda"))
+    with torch.no_grad():
+        lin.weight_master.copy_(w)
+    return lin
+
+
+def test_weight_changed_in_place_in_inference_mode():
+    """A weight made there has no version counter."""
+    w, x = rnd((40, 64), 1), rnd((3, 64), 2).cuda()
+    with torch.no_grad():
+        want = layer(w)(x)
+    with torch.inference_mode():
+        lin = layer(w)
+        assert lin.weight_master.is_inference() and torch.equal(lin(x), want)
+        lin.weight_master.mul_(2.0)
+        assert torch.equal(lin(x), 2 * want)
+        lin.load_state_dict({"weight_master": 4 * w.cuda()})
+        assert torch.equal(lin(x), 4 * want)
+        lin.refresh_working_copy()
+        lin.weight_master.mul_(2.0)
+        assert torch.equal(lin(x), 8 * want)
+    with torch.no_grad():
+        assert torch.equal(lin(x), 8 * want)
