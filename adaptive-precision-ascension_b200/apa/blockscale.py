@@ -43,6 +43,7 @@ from typing import Optional, Tuple, Union
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
+from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from . import _lib
 from .config import APAConfig
@@ -625,6 +626,19 @@ class _BlockLinearFn(torch.autograd.Function):
         return (dx if need[0] else None, dx if has_res and need[1] else None, dg if need[2] else None, dw, db, None)
 
 
+_optimizer_steps = 0
+
+
+def _count_optimizer_step(*_) -> None:
+    global _optimizer_steps
+    _optimizer_steps += 1
+
+
+# Fused optimizers change parameters without raising their version counters, so
+# a step of any torch.optim optimizer (subclasses too) counts as a change.
+register_optimizer_step_post_hook(_count_optimizer_step)
+
+
 class APABlockLinear(nn.Module):
     """A linear layer whose three products run on block-scaled E4M3 operands.
 
@@ -632,11 +646,12 @@ class APABlockLinear(nn.Module):
     parameters in ``dtype`` (float32 masters, or bfloat16); their gradients come
     in the same type. Output and input gradient have x's type. In training
     every forward casts the weight anew; without gradients the layer keeps its
-    cast weight and renews it when the parameter changed (in place through
-    autograd's version counter; call ``refresh_working_copy()`` after changes
-    made behind it, through ``.data`` or by a replayed graph). A weight made
-    under ``torch.inference_mode()`` has no such counter and is cast on every
-    call.
+    cast weight and renews it when the parameter was replaced, when autograd's
+    version counter shows a change in place, after a training forward and after
+    any ``torch.optim`` optimizer's step. Call ``refresh_working_copy()`` after
+    changes behind all of these: through ``.data`` or by a replayed graph. A
+    weight made under ``torch.inference_mode()`` has no version counter and is
+    cast on every call.
 
     ``forward(x, norm=None, residual=None)``: with ``norm`` (an ``APARMSNorm``)
     the layer is applied to ``norm(x)``, or to the normalised sum x + residual;
@@ -720,7 +735,7 @@ class APABlockLinear(nn.Module):
     @staticmethod
     def _state(W: torch.Tensor) -> Tuple:
         # a tensor made in inference mode has no version, so its cast is never taken as current
-        return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype)
+        return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype, _optimizer_steps)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
         # nn.Module's attribute lookup takes a microsecond
@@ -743,6 +758,8 @@ class APABlockLinear(nn.Module):
         if torch.is_grad_enabled() and (W.requires_grad or x.requires_grad or (b is not None and b.requires_grad)
                                         or (gamma is not None and gamma.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
+            if W.requires_grad:
+                self._wq_key = None         # an update follows, by whatever means
             return _BlockLinearFn.apply(x, residual, gamma, W, b, eps)
         wq = self._working_copy(W)
         if norm is None:

@@ -114,3 +114,36 @@ def test_weight_made_and_changed_in_inference_mode(stage):
         lin.refresh_working_copy()
         lin.load_state_dict({"weight_master": W0 + 1})
         assert torch.equal(served(lin), W0 + 1)
+
+
+@pytest.mark.parametrize("kind", ["fused", "foreach", "own"])
+def test_weight_changed_by_an_optimizer(stage, kind):
+    """Fused optimizers leave the version counter as it was."""
+    lin = stage.make()
+    W = lin.weight_master
+
+    class Raw(torch.optim.Optimizer):
+        def step(self, closure=None):
+            for g in self.param_groups:
+                for p in g["params"]:
+                    p.data.sub_(p.grad)
+
+    if kind == "own":
+        opt = Raw([W], {})
+    else:
+        opt = torch.optim.SGD([W], lr=1.0, **{kind: True})
+    for turn in range(3):
+        assert torch.equal(served(lin), W0 - turn)
+        W.grad = torch.ones_like(W)
+        opt.step()
+    assert torch.equal(served(lin), W0 - 3)
+
+
+def test_weight_changed_between_a_training_forward_and_a_call(stage, monkeypatch):
+    """An update that no counter shows: the training forward before it is enough."""
+    monkeypatch.setattr(blockscale._BlockLinearFn, "apply", staticmethod(lambda *a: a[0]))
+    lin = stage.make()
+    assert torch.equal(served(lin), W0)
+    lin(torch.ones(2, 4))
+    lin.weight_master.data.mul_(2.0)
+    assert torch.equal(served(lin), 2 * W0)

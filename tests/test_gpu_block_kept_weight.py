@@ -39,3 +39,33 @@ def test_weight_changed_in_place_in_inference_mode():
         assert torch.equal(lin(x), 8 * want)
     with torch.no_grad():
         assert torch.equal(lin(x), 8 * want)
+
+
+@pytest.mark.parametrize("kind", ["fused", "foreach", "apa"])
+def test_evaluation_after_an_optimizer_step(kind):
+    """Evaluate, train, evaluate: every evaluation uses the stepped weight, also
+    when steps follow each other without a forward between them."""
+    from apa import APAManager
+    from apa.optim import APAAdamW
+
+    w, x = rnd((40, 64), 1), rnd((3, 64), 2).cuda()
+    lin = layer(w)
+    if kind == "apa":
+        opt = APAAdamW(APAManager(torch.nn.Sequential(lin), APAConfig(device="cuda")), lr=0.1)
+    else:
+        opt = torch.optim.AdamW(lin.parameters(), lr=0.1, **{kind: True})
+
+    def check():
+        with torch.no_grad():
+            fresh = layer(lin.weight_master)
+            assert torch.equal(lin(x), fresh(x))
+
+    check()
+    for _ in range(3):
+        lin(x).sum().backward()
+        opt.step()
+        before = lin.weight_master.detach().clone()
+        check()
+        opt.step()
+        assert not torch.equal(lin.weight_master, before)
+        check()
