@@ -38,6 +38,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import threading
 from typing import Optional, Tuple, Union
 
 import torch
@@ -639,6 +640,17 @@ def _count_optimizer_step(*_) -> None:
 register_optimizer_step_post_hook(_count_optimizer_step)
 
 
+class _KeptWeight:
+    """A layer's cast weight: the block tensor, the parameter that it was cast
+    from and that one's state then, an event behind the cast, and the handles of
+    the streams that are ordered behind it."""
+
+    __slots__ = ("block", "weight", "state", "done", "streams")
+
+    def __init__(self, block, weight, state, done, streams):
+        self.block, self.weight, self.state, self.done, self.streams = block, weight, state, done, streams
+
+
 class APABlockLinear(nn.Module):
     """A linear layer whose three products run on block-scaled E4M3 operands.
 
@@ -674,28 +686,44 @@ class APABlockLinear(nn.Module):
             self.bias_master = nn.Parameter(torch.empty(out_features, dtype=dtype, device=dev).uniform_(-bound, bound))
         else:
             self.register_parameter("bias_master", None)
-        self._wq: Optional[APABlockTensor] = None
-        # the parameter that _wq was cast from, its state then, an event behind the cast, the streams behind that
-        self._wq_key: Optional[Tuple] = None
+        self._kept: Optional[_KeptWeight] = None
+        self._lock = threading.Lock()        # around renewing _kept and adding streams to it
+
+    @property
+    def _wq(self) -> Optional[APABlockTensor]:
+        kept = self._kept
+        return None if kept is None else kept.block
 
     def refresh_working_copy(self) -> None:
         """Cast the weight for calls without gradients (buffers are kept, so a
         captured graph of such a call sees the new values)."""
         W = self.weight_master
         _lib.require_cuda(W, "APABlockLinear.refresh_working_copy")
-        with torch.no_grad(), torch.cuda.device(W.device):
-            capturing = torch.cuda.is_current_stream_capturing()
-            if capturing and self._wq is None:
-                raise RuntimeError("APABlockLinear.refresh_working_copy: nothing to renew in a captured graph; "
-                                   "call it once before the capture")
-            kept = self._wq
-            if kept is not None and (kept.device != W.device or kept.shape != W.shape):
-                kept = None
-            self._wq = self._cast_weight(W, kept)
-            if not capturing:          # a captured renewal happens when the graph runs
-                done = torch.cuda.Event()
-                done.record()
-                self._wq_key = (W, self._state(W), done, {_lib.stream_handle(W.device)})
+        with self._lock, torch.cuda.device(W.device):
+            self._renew(W)
+
+    def _renew(self, W: torch.Tensor) -> Optional[_KeptWeight]:
+        """Cast W into the kept buffer. The caller holds the lock and has made
+        W's device current."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        old = self._kept
+        if capturing and old is None:
+            raise RuntimeError("APABlockLinear.refresh_working_copy: nothing to renew in a captured graph; "
+                               "call it once before the capture")
+        into = None
+        if old is not None and old.block.device == W.device and old.block.shape == W.shape:
+            into = old.block
+        state = self._state(W)               # before the cast: a change during it shows later
+        block = self._cast_weight(W, into)
+        if capturing:                        # the cast happens when the graph runs
+            if into is None:
+                self._kept = _KeptWeight(block, None, None, None, set())
+            return None
+        done = torch.cuda.Event()
+        done.record()
+        # one store: a reader sees the old buffer with its stream set or the new one with its own
+        self._kept = kept = _KeptWeight(block, W, state, done, {_lib.stream_handle(W.device)})
+        return kept
 
     @staticmethod
     def _cast_weight(W: torch.Tensor, into: Optional[APABlockTensor] = None) -> APABlockTensor:
@@ -710,27 +738,36 @@ class APABlockLinear(nn.Module):
             # it has no version counter, and inference mode may change it in place: nothing shows whether a cast still holds
             with torch.cuda.device(W.device):
                 return self._cast_weight(W)
-        key = self._wq_key
         handle = _lib.stream_handle(W.device)
-        if key is not None and key[0] is W and key[1] == self._state(W):
-            if handle in key[3]:
-                return self._wq
-            with torch.cuda.device(W.device):
-                if not torch.cuda.is_current_stream_capturing():      # a capture starts behind what it reads
-                    torch.cuda.current_stream().wait_event(key[2])
-                    self._wq.buffer.record_stream(torch.cuda.current_stream())
-                    key[3].add(handle)
-            return self._wq
+        kept = self._kept
+        if kept is not None and kept.weight is W and handle in kept.streams and kept.state == self._state(W):
+            return kept.block
         with torch.cuda.device(W.device):
             if torch.cuda.is_current_stream_capturing():
-                return self._cast_weight(W)
-        self.refresh_working_copy()
-        return self._wq
+                # a capture starts behind what it reads
+                return kept.block if self._current(kept, W) else self._cast_weight(W)
+            with self._lock:
+                kept = self._kept
+                if not self._current(kept, W):
+                    kept = self._renew(W)
+                elif handle not in kept.streams:
+                    torch.cuda.current_stream().wait_event(kept.done)
+                    kept.block.buffer.record_stream(torch.cuda.current_stream())
+                    kept.streams.add(handle)
+                return kept.block
+
+    def _current(self, kept: Optional[_KeptWeight], W: torch.Tensor) -> bool:
+        return kept is not None and kept.weight is W and kept.state == self._state(W)
 
     def __getstate__(self):
         state = self.__dict__.copy()
-        state["_wq"] = state["_wq_key"] = None       # a copy casts its own weight
+        state["_kept"] = None                # a copy casts its own weight
+        del state["_lock"]
         return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._kept, self._lock = None, threading.Lock()
 
     @staticmethod
     def _state(W: torch.Tensor) -> Tuple:
@@ -758,8 +795,9 @@ class APABlockLinear(nn.Module):
         if torch.is_grad_enabled() and (W.requires_grad or x.requires_grad or (b is not None and b.requires_grad)
                                         or (gamma is not None and gamma.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
-            if W.requires_grad:
-                self._wq_key = None         # an update follows, by whatever means
+            kept = self._kept
+            if W.requires_grad and kept is not None:
+                kept.state = None           # an update follows, by whatever means
             return _BlockLinearFn.apply(x, residual, gamma, W, b, eps)
         wq = self._working_copy(W)
         if norm is None:

@@ -44,7 +44,7 @@ def stage(monkeypatch):
     stage = Stage()
     stage.log, stage.local = [], threading.local()
     stage.streams = {h: Stream(h, stage.log) for h in (1, 2, 3)}
-    stage.during_cast = lambda: None
+    stage.during_cast = stage.during_record = lambda: None
     here = lambda *a: stage.streams[getattr(stage.local, "handle", 1)]
 
     class Event:
@@ -52,6 +52,7 @@ def stage(monkeypatch):
 
         def record(self, stream=None):
             self.after = ("event", (stream or here()).cuda_stream)
+            stage.during_record()
 
     @contextlib.contextmanager
     def on(stream):
@@ -147,3 +148,65 @@ def test_weight_changed_between_a_training_forward_and_a_call(stage, monkeypatch
     lin(torch.ones(2, 4))
     lin.weight_master.data.mul_(2.0)
     assert torch.equal(served(lin), 2 * W0)
+
+
+def ordered(log, handle, block):
+    """Whether work of stream `handle` that reads `block` comes behind its last cast."""
+    by = [e[1] for e in log if e[0] == "cast" and e[2] == id(block)][-1]
+    return by == handle or ("wait", handle, ("event", by)) in log
+
+
+def test_first_calls_of_two_threads(stage):
+    """Two streams, a thread each. Where both casts can be under way together,
+    the second one's buffer is stored before the first call returns."""
+    lin = stage.make()
+    casting, both, recorded, second = (threading.Event() for _ in range(4))
+    got = {}
+
+    def during_cast():
+        if threading.current_thread().name == "first":
+            casting.set()
+            both.wait(0.3)
+        else:
+            both.set()
+            recorded.wait(0.3)
+
+    def during_record():
+        if threading.current_thread().name == "first":
+            recorded.set()
+            second.wait(0.3)
+
+    stage.during_cast, stage.during_record = during_cast, during_record
+
+    def call(handle):
+        with stage.on(handle):
+            got[handle] = lin._working_copy(lin.weight_master)
+        if handle == 2:
+            second.set()
+
+    a = threading.Thread(target=call, args=(1,), name="first")
+    b = threading.Thread(target=call, args=(2,), name="second")
+    a.start()
+    casting.wait()
+    b.start()
+    a.join()
+    b.join()
+    for handle, block in got.items():
+        assert ordered(stage.log, handle, block), (handle, stage.log)
+    # and so does the next call of a third stream
+    with stage.on(3):
+        block = lin._working_copy(lin.weight_master)
+    assert ordered(stage.log, 3, block)
+
+
+def test_copies_and_pickles_have_their_own(stage):
+    import copy
+    import pickle
+
+    lin = stage.make()
+    served(lin)
+    for other in (copy.deepcopy(lin), pickle.loads(pickle.dumps(lin))):
+        assert other._wq is None and torch.equal(served(other), W0)
+        with torch.no_grad():
+            other.weight_master.mul_(2.0)
+        assert torch.equal(served(other), 2 * W0) and torch.equal(served(lin), W0)

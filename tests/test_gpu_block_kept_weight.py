@@ -69,3 +69,31 @@ def test_evaluation_after_an_optimizer_step(kind):
         opt.step()
         assert not torch.equal(lin.weight_master, before)
         check()
+
+
+def test_first_calls_of_two_threads():
+    """A stream and a thread each, released together onto fresh layers."""
+    import threading
+
+    w, x = rnd((1024, 1024), 1), rnd((5, 1024), 2).cuda()
+    with torch.no_grad():
+        want = layer(w)(x)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    layers = [layer(w) for _ in range(10)]
+    torch.cuda.synchronize()
+    gate = threading.Barrier(len(streams))
+    outs = [[] for _ in streams]
+
+    def work(i):
+        with torch.no_grad(), torch.cuda.stream(streams[i]):
+            for lin in layers:
+                gate.wait()
+                outs[i].append(lin(x))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(streams))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(len(o) == len(layers) and all(torch.equal(y, want) for y in o) for o in outs)
