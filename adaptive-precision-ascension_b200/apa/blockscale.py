@@ -640,10 +640,17 @@ def _count_optimizer_step(*_) -> None:
 register_optimizer_step_post_hook(_count_optimizer_step)
 
 
+def _capturing(stream) -> bool:
+    """Whether a capture is under way on ``stream``: it can be neither waited
+    for nor, since a capture begins behind what its stream held, need be."""
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class _KeptWeight:
     """A layer's cast weight: the block tensor, the parameter that it was cast
-    from and that one's state then, an event behind the cast, and the handles of
-    the streams that are ordered behind it."""
+    from and that one's state then, an event behind the cast, and the streams
+    that are ordered behind it and may read it, by handle."""
 
     __slots__ = ("block", "weight", "state", "done", "streams")
 
@@ -696,7 +703,9 @@ class APABlockLinear(nn.Module):
 
     def refresh_working_copy(self) -> None:
         """Cast the weight for calls without gradients (buffers are kept, so a
-        captured graph of such a call sees the new values)."""
+        captured graph of such a call sees the new values). Products queued
+        before are waited for, on whichever stream the layer was called;
+        replays of captured calls are the caller's to order."""
         W = self.weight_master
         _lib.require_cuda(W, "APABlockLinear.refresh_working_copy")
         with self._lock, torch.cuda.device(W.device):
@@ -713,16 +722,23 @@ class APABlockLinear(nn.Module):
         into = None
         if old is not None and old.block.device == W.device and old.block.shape == W.shape:
             into = old.block
+        stream = torch.cuda.current_stream()
+        if into is not None and not capturing:
+            # products queued on other streams may still read the buffer that is rewritten
+            for handle, other in old.streams.items():
+                if handle != stream.cuda_stream and not _capturing(other):
+                    stream.wait_stream(other)
+            into.buffer.record_stream(stream)
         state = self._state(W)               # before the cast: a change during it shows later
         block = self._cast_weight(W, into)
         if capturing:                        # the cast happens when the graph runs
             if into is None:
-                self._kept = _KeptWeight(block, None, None, None, set())
+                self._kept = _KeptWeight(block, None, None, None, {})
             return None
         done = torch.cuda.Event()
         done.record()
-        # one store: a reader sees the old buffer with its stream set or the new one with its own
-        self._kept = kept = _KeptWeight(block, W, state, done, {_lib.stream_handle(W.device)})
+        # one store: a reader sees the old event and streams or the new ones
+        self._kept = kept = _KeptWeight(block, W, state, done, {stream.cuda_stream: stream})
         return kept
 
     @staticmethod
@@ -751,9 +767,10 @@ class APABlockLinear(nn.Module):
                 if not self._current(kept, W):
                     kept = self._renew(W)
                 elif handle not in kept.streams:
-                    torch.cuda.current_stream().wait_event(kept.done)
-                    kept.block.buffer.record_stream(torch.cuda.current_stream())
-                    kept.streams.add(handle)
+                    stream = torch.cuda.current_stream()
+                    stream.wait_event(kept.done)
+                    kept.block.buffer.record_stream(stream)
+                    kept.streams[handle] = stream
                 return kept.block
 
     def _current(self, kept: Optional[_KeptWeight], W: torch.Tensor) -> bool:

@@ -210,3 +210,42 @@ def test_copies_and_pickles_have_their_own(stage):
         with torch.no_grad():
             other.weight_master.mul_(2.0)
         assert torch.equal(served(other), 2 * W0) and torch.equal(served(lin), W0)
+
+
+@pytest.mark.parametrize("how", ["replaced", "data", "refresh"])
+def test_renewal_waits_for_readers_on_other_streams(stage, how):
+    """A replaced weight needs no ordering, so products of the old one may still be queued."""
+    lin = stage.make()
+    for handle in (1, 2):
+        with stage.on(handle):
+            served(lin)
+    kept = lin._wq
+    stage.log.clear()
+    if how == "replaced":
+        lin.weight_master = torch.nn.Parameter(2 * W0)
+    else:
+        lin.weight_master.data = 2 * W0
+    with stage.on(3):
+        if how == "refresh":
+            lin.refresh_working_copy()
+        assert torch.equal(served(lin), 2 * W0)
+    assert lin._wq is kept                       # captured graphs see the new values
+    cast = stage.log.index(("cast", 3, id(kept)))
+    for entry in (("wait", 3, ("stream", 1)), ("wait", 3, ("stream", 2)), ("record", id(kept), 3)):
+        assert stage.log.index(entry) < cast
+    assert len(stage.casts()) == 1
+    # what comes next waits for the new cast
+    with stage.on(1):
+        assert torch.equal(served(lin), 2 * W0) and ordered(stage.log, 1, kept)
+
+
+def test_renewal_beside_a_capture(stage):
+    """A stream that is being captured cannot be waited for."""
+    lin = stage.make()
+    with stage.on(2):
+        served(lin)
+    stage.streams[2].capturing = True
+    with torch.no_grad():
+        lin.weight_master.mul_(2.0)
+    assert torch.equal(served(lin), 2 * W0)
+    assert ("wait", 1, ("stream", 2)) not in stage.log

@@ -97,3 +97,29 @@ def test_first_calls_of_two_threads():
         t.join()
     torch.cuda.synchronize()
     assert all(len(o) == len(layers) and all(torch.equal(y, want) for y in o) for o in outs)
+
+
+@pytest.mark.parametrize("how", ["replaced", "data"])
+def test_replaced_while_another_stream_still_reads(how):
+    """A product queued behind other work reads the weight it was called with."""
+    w, x = rnd((2048, 2048), 1), rnd((64, 2048), 2).cuda()
+    lin = layer(w)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    new = -w.cuda()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        with torch.cuda.stream(a):
+            want = lin(x)
+        with torch.cuda.stream(b):
+            lin(x)                                    # b is behind the cast
+            torch.cuda.synchronize()
+            torch.cuda._sleep(100_000_000)            # 50 ms of the GPU's clock
+            old = lin(x)
+        if how == "replaced":
+            lin.weight_master = torch.nn.Parameter(new)
+        else:
+            lin.weight_master.data = new
+        with torch.cuda.stream(a):
+            fresh = lin(x)
+    torch.cuda.synchronize()
+    assert torch.equal(old, want) and torch.equal(fresh, -want)
