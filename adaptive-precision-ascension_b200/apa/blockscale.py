@@ -464,26 +464,25 @@ class _RMSNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.has_res = residual is not None
         ctx.shape = x.shape
-        ctx.rstd = rstd
         flat = x.dim() == 2
         if not flat:
             y = y.view(x.shape)
         if residual is None:
-            ctx.save_for_backward(x, weight)
+            ctx.save_for_backward(x, weight, rstd)
             return y
         if not flat:
             stream = stream.view(x.shape)
-        ctx.save_for_backward(stream, weight)
+        ctx.save_for_backward(stream, weight, rstd)
         return y, stream
 
     @staticmethod
     @_first_order
     def backward(ctx, dy, dr=None):
-        r, weight = ctx.saved_tensors
+        r, weight, rstd = ctx.saved_tensors
         K = weight.shape[0]
         if dy is None:
             return dr, None, dr if ctx.has_res else None, None
-        dx, dg = _norm_backward(_grad_matrix(dy, r.dtype, K), _matrix(r, "rms_norm"), ctx.rstd, weight.contiguous(),
+        dx, dg = _norm_backward(_grad_matrix(dy, r.dtype, K), _matrix(r, "rms_norm"), rstd, weight.contiguous(),
                                 _grad_matrix(dr, r.dtype, K))
         if dx.shape != ctx.shape:
             dx = dx.view(ctx.shape)
@@ -573,15 +572,18 @@ class _BlockLinearFn(torch.autograd.Function):
                             p if n_xt else None, None, p + n_xt if n_wt else None,
                             _vector(bias, N, dev, "APABlockLinear: bias") if bias is not None else None, y, code, M, N,
                             K)
-        ctx.keep, ctx.n_xt, ctx.rstd = keep, n_xt, rstd
+        ctx.n_xt = n_xt
         ctx.has_res, ctx.has_norm = residual is not None, has_norm
         ctx.meta = (x.shape, M, N, K, x.dtype, weight.dtype, bias.dtype if bias is not None else None)
         if y.shape[:-1] != x.shape[:-1]:
             y = y.view(*x.shape[:-1], N)
+        # saved as tensors: freed by the backward, refused to a second one, and
+        # seen by hooks (checkpointing, offloading)
         if not has_norm:
+            ctx.save_for_backward(keep)
             return y
         stream = x if stream is None else stream.view(x.shape)
-        ctx.save_for_backward(stream, gamma)
+        ctx.save_for_backward(keep, rstd, stream, gamma)
         return (y, stream) if residual is not None else y
 
     @staticmethod
@@ -591,6 +593,8 @@ class _BlockLinearFn(torch.autograd.Function):
         has_norm, has_res = ctx.has_norm, ctx.has_res
         if dy is None:
             return (dr if need[0] else None, dr if has_res and need[1] else None, None, None, None, None)
+        saved = ctx.saved_tensors
+        keep = saved[0]
         shape, M, N, K, dtype, wdtype, bdtype = ctx.meta
         need_in = need[0] or need[1] or need[2]
         dev = dy.device
@@ -598,9 +602,9 @@ class _BlockLinearFn(torch.autograd.Function):
         dw = torch.empty(N, K, dtype=wdtype, device=dev) if need[3] else None
         db = torch.empty(N, dtype=bdtype, device=dev) if need[4] else None
         dg = None
-        stream = gamma = None
+        rstd = stream = gamma = None
         if has_norm:
-            stream, gamma = ctx.saved_tensors
+            _, rstd, stream, gamma = saved
             if need_in:
                 dg = torch.empty(K, dtype=gamma.dtype, device=dev)
         if M:
@@ -612,9 +616,9 @@ class _BlockLinearFn(torch.autograd.Function):
             flags = (1 if need_in else 0) | (2 if need[3] else 0) | (4 if need[4] else 0) | (8 if has_norm else 0)
             n = _linear_workspace(M, N, K, flags, code, wcode, dev.index)
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            p = ctx.keep.data_ptr() if ctx.keep is not None else 0
+            p = keep.data_ptr() if keep is not None else 0
             _call(dev, "apa_block_linear_bwd", dy2.data_ptr(), code, _ld(dy2), p + ctx.n_xt if need_in else None,
-                  p if ctx.n_xt else None, _lib.ptr(stream), _ld(stream) if has_norm else 0, _lib.ptr(ctx.rstd),
+                  p if ctx.n_xt else None, _lib.ptr(stream), _ld(stream) if has_norm else 0, _lib.ptr(rstd),
                   _lib.ptr(gamma), _REAL[gamma.dtype] if has_norm else 0, _lib.ptr(dr2),
                   _ld(dr2) if dr2 is not None else 0, _lib.ptr(dx), code, K, _lib.ptr(dg), _lib.ptr(dw), wcode, K,
                   _lib.ptr(db), _REAL[bdtype] if db is not None else 0, M, N, K, ws.data_ptr(), n)
