@@ -281,6 +281,12 @@ def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accum
           out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n)
 
 
+def _no_gradient(what: str, x, bias) -> None:
+    if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        raise RuntimeError(f"{what}: has no gradient; call it under torch.no_grad(), or train through APABlockLinear")
+
+
 def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tensor] = None,
                  out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
                  accumulate: bool = False) -> torch.Tensor:
@@ -288,7 +294,8 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
 
     Accumulated in fp32 and rounded once to ``out_dtype`` (float32, float16
     or bfloat16). ``out``: written in place (unit column stride); with
-    ``accumulate`` the product is added to a float32 ``out``."""
+    ``accumulate`` the product is added to a float32 ``out``. Not
+    differentiable (a bias that wants a gradient is refused)."""
     if not isinstance(a, APABlockTensor) or not isinstance(b, APABlockTensor):
         raise TypeError("block_matmul: both operands must be APABlockTensors")
     _lib.require_cuda(a.buffer, "block_matmul")
@@ -300,6 +307,7 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
         raise ValueError("block_matmul: the second operand has no rows")
     if bias is not None:
         bias = _vector(bias, N, a.device, "block_matmul: bias")
+        _no_gradient("block_matmul", None, bias)
     if accumulate and out is None:
         raise ValueError("block_matmul: accumulate needs out")
     if out is None:
@@ -322,16 +330,14 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     """x W^T + bias for serving. x [..., K] is cast to E4M3 here, or comes as an
     APABlockTensor (from ``rms_norm(..., quantize=True)``); ``weight`` [N, K] is
     ``block_cast(w, square=True)``. ``out_dtype`` defaults to x's type
-    (bfloat16 for an APABlockTensor). Not differentiable (an x that wants a
-    gradient is refused)."""
+    (bfloat16 for an APABlockTensor). Not differentiable (an x or a bias that
+    wants a gradient is refused)."""
     if isinstance(x, APABlockTensor):
         return block_matmul(x, weight, bias, out_dtype or torch.bfloat16)
     if not isinstance(weight, APABlockTensor):
         raise TypeError("block_linear: the weight must be an APABlockTensor (block_cast(w, square=True))")
     x2 = _matrix(x, "block_linear")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("block_linear: has no gradient; call it under torch.no_grad(), or train through "
-                           "APABlockLinear")
+    _no_gradient("block_linear", x, bias)
     code = _real(x2.dtype, "block_linear")
     _lib.require_cuda(x2, "block_linear")
     M, K = x2.shape

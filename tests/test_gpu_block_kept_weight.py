@@ -123,3 +123,25 @@ def test_replaced_while_another_stream_still_reads(how):
             fresh = lin(x)
     torch.cuda.synchronize()
     assert torch.equal(old, want) and torch.equal(fresh, -want)
+
+
+def test_serving_without_gradients():
+    """The layer's parts called one by one, as its parameters are, equal the layer."""
+    from apa import APARMSNorm, block_cast, block_linear, block_matmul, rms_norm
+
+    cfg = APAConfig(device="cuda")
+    norm, up = APARMSNorm(256, config=cfg), APABlockLinear(256, 384, config=cfg)
+    x, h = rnd((7, 256), 1, torch.bfloat16).cuda(), rnd((7, 256), 2, torch.bfloat16).cuda()
+    with torch.no_grad():
+        w = block_cast(up.weight_master, square=True)
+        q, r = rms_norm(x, norm.weight, residual=h, quantize=True)
+        y = block_linear(q, w, up.bias_master)
+        z = block_matmul(q, w, up.bias_master, out_dtype=torch.bfloat16)
+        want, stream = up(x, norm=norm, residual=h)
+        assert torch.equal(y, want) and torch.equal(z, want) and torch.equal(r, stream)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm(x, norm.weight, residual=h, quantize=True)
+    for call in (lambda: block_linear(q, w, up.bias_master), lambda: block_linear(x, w, up.bias_master),
+                 lambda: block_matmul(q, w, up.bias_master)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
