@@ -281,9 +281,8 @@ def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accum
           out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n)
 
 
-def _no_gradient(what: str, x, bias) -> None:
-    if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+def _no_gradient(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what}: has no gradient; call it under torch.no_grad(), or train through APABlockLinear")
 
 
@@ -295,7 +294,7 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
     Accumulated in fp32 and rounded once to ``out_dtype`` (float32, float16
     or bfloat16). ``out``: written in place (unit column stride); with
     ``accumulate`` the product is added to a float32 ``out``. Not
-    differentiable (a bias that wants a gradient is refused)."""
+    differentiable (a bias or an ``out`` that wants a gradient is refused)."""
     if not isinstance(a, APABlockTensor) or not isinstance(b, APABlockTensor):
         raise TypeError("block_matmul: both operands must be APABlockTensors")
     _lib.require_cuda(a.buffer, "block_matmul")
@@ -307,10 +306,11 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
         raise ValueError("block_matmul: the second operand has no rows")
     if bias is not None:
         bias = _vector(bias, N, a.device, "block_matmul: bias")
-        _no_gradient("block_matmul", None, bias)
+    _no_gradient("block_matmul", bias, out)
     if accumulate and out is None:
         raise ValueError("block_matmul: accumulate needs out")
-    if out is None:
+    given = out is not None
+    if not given:
         _real(out_dtype, "block_matmul: out_dtype")
         out = torch.empty(M, N, dtype=out_dtype, device=a.device)
     else:
@@ -322,6 +322,9 @@ def block_matmul(a: APABlockTensor, b: APABlockTensor, bias: Optional[torch.Tens
             raise ValueError("block_matmul: accumulate needs a float32 out")
     if M:
         _matmul(a, b, bias, out, accumulate)
+        if given and not out.is_inference():
+            # autograd refuses a backward that would read the values from before
+            torch.autograd.graph.increment_version(out)
     return out
 
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from apa import APABlockTensor, _lib, block_linear, block_matmul
+from apa import APABlockTensor, _lib, block_linear, block_matmul, blockscale
 
 
 def block(rows, cols):
@@ -19,3 +19,24 @@ def test_a_bias_that_wants_a_gradient(monkeypatch):
                  lambda: block_matmul(block(3, 64), w, bias), lambda: block_linear(x.requires_grad_(True), w)):
         with pytest.raises(RuntimeError, match="no gradient"):
             call()
+
+
+def test_out_is_written_in_place(monkeypatch):
+    """As torch's own out=: refused where it wants a gradient, and counted as a
+    change, so that a backward which would read its old values is refused."""
+    monkeypatch.setattr(_lib, "require_cuda", lambda t, what: None)
+    monkeypatch.setattr(blockscale, "_matmul", lambda a, b, bias, out, accumulate: None)
+    a, w = block(3, 64), block(8, 64)
+    leaf = torch.zeros(3, 8, requires_grad=True)
+    for out in (leaf, leaf * 1.0):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            block_matmul(a, w, out=out)
+    with torch.no_grad():
+        assert block_matmul(a, w, out=leaf) is leaf
+    s = torch.ones(3, 8)
+    loss = (leaf * s).sum()
+    block_matmul(a, w, out=s, accumulate=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        block_matmul(a, w, out=torch.ones(3, 8))
