@@ -137,14 +137,22 @@ class APABlockTensor:
     """A [rows, cols] matrix held as E4M3 codes with one scale per row and 128
     columns. ``data`` holds the codes; ``scales`` one byte per block (2^(b-127))
     in the order the tensor cores take, see ``exponents()`` for the plain one.
+    ``buffer`` is a flat uint8 tensor on a 16-byte boundary: the codes, row by
+    row with a pitch of ``cols`` rounded up to 16, then the scales.
     """
 
     __slots__ = ("buffer", "rows", "cols")
 
     def __init__(self, buffer: torch.Tensor, rows: int, cols: int):
-        self.buffer = buffer          # uint8: the codes, row by row with a pitch of _pitch(cols), then the scales
-        self.rows = rows
-        self.cols = cols
+        # the kernels read as many bytes as rows and cols say
+        if not isinstance(buffer, torch.Tensor) or buffer.dtype != torch.uint8 or buffer.dim() != 1:
+            raise TypeError("APABlockTensor: buffer must be a flat uint8 tensor")
+        if rows < 0 or cols <= 0:
+            raise ValueError(f"APABlockTensor: bad shape [{rows}, {cols}]")
+        if buffer.numel() < _packed_bytes(rows, cols) or not buffer.is_contiguous() or buffer.data_ptr() % 16:
+            raise ValueError(f"APABlockTensor: [{rows}, {cols}] takes {_packed_bytes(rows, cols)} contiguous bytes on a "
+                             "16-byte boundary")
+        self.buffer, self.rows, self.cols = buffer, rows, cols
 
     @property
     def data(self) -> torch.Tensor:
@@ -153,7 +161,7 @@ class APABlockTensor:
 
     @property
     def scales(self) -> torch.Tensor:
-        return self.buffer[self.rows * _pitch(self.cols):]
+        return self.buffer[self.rows * _pitch(self.cols):_packed_bytes(self.rows, self.cols)]
 
     @property
     def shape(self) -> torch.Size:
@@ -227,7 +235,10 @@ class APABlockTensor:
 
 
 def _new_block(rows: int, cols: int, device) -> APABlockTensor:
-    return APABlockTensor(torch.empty(_packed_bytes(rows, cols), dtype=torch.uint8, device=device), rows, cols)
+    t = object.__new__(APABlockTensor)       # what the constructor checks holds
+    t.buffer = torch.empty(_packed_bytes(rows, cols), dtype=torch.uint8, device=device)
+    t.rows, t.cols = rows, cols
+    return t
 
 
 _NONE = (None, 0, None)

@@ -40,3 +40,19 @@ def test_out_is_written_in_place(monkeypatch):
         loss.backward()
     with torch.inference_mode():
         block_matmul(a, w, out=torch.ones(3, 8))
+
+
+def test_buffers_too_small_for_their_shape():
+    """A product reads what the shape says, so the shape has to fit."""
+    t = block(5, 200)
+    again = APABlockTensor(t.buffer, 5, 200)
+    assert torch.equal(again.exponents(), t.exponents())
+    longer = APABlockTensor(torch.cat([t.buffer, torch.zeros(64, dtype=torch.uint8)]), 5, 200)
+    assert torch.equal(longer.exponents(), t.exponents())
+    for args in ((t.buffer, 6, 200), (t.buffer, 5, 209), (t.buffer[:-1], 5, 200), (t.buffer, -1, 200), (t.buffer, 5, 0),
+                 (longer.buffer[8:], 5, 200), (torch.zeros(2 * t.buffer.numel(), dtype=torch.uint8)[::2], 5, 200)):
+        with pytest.raises(ValueError):
+            APABlockTensor(*args)
+    for bad in (t.buffer.view(1, -1), t.buffer.float(), t.buffer.numpy()):
+        with pytest.raises(TypeError):
+            APABlockTensor(bad, 5, 200)
