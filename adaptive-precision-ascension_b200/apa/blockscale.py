@@ -394,6 +394,14 @@ def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bi
 # ---------------------------------------------------------------------------
 # root-mean-square norm
 # ---------------------------------------------------------------------------
+def _parameter(module: nn.Module, name: str):
+    """A module's parameter. nn.Module's own lookup takes a microsecond; it serves
+    a parameter that something else computes (a parametrization, pruning, a
+    replica of DataParallel)."""
+    p = module._parameters
+    return p[name] if name in p else getattr(module, name)
+
+
 def _norm_args(x, weight, residual, what: str):
     x2 = _matrix(x, what)
     _real(x2.dtype, what)
@@ -545,8 +553,7 @@ class APARMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(features, dtype=dtype, device=torch.device(config.device)))
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, quantize: bool = False):
-        # nn.Module's attribute lookup takes a microsecond
-        return rms_norm(x, self._parameters["weight"], residual, self.eps, quantize)
+        return rms_norm(x, _parameter(self, "weight"), residual, self.eps, quantize)
 
     def extra_repr(self) -> str:
         return f"{self.features}, eps={self.eps}"
@@ -816,9 +823,7 @@ class APABlockLinear(nn.Module):
         return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype, _optimizer_steps)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
-        # nn.Module's attribute lookup takes a microsecond
-        p = self._parameters
-        W, b = p["weight_master"], p["bias_master"]
+        W, b = _parameter(self, "weight_master"), _parameter(self, "bias_master")
         if not isinstance(x, torch.Tensor):
             raise TypeError(f"APABlockLinear: expected a tensor, got {type(x).__name__}")
         if x.dim() < 1 or x.shape[-1] != self.in_features:
@@ -827,7 +832,7 @@ class APABlockLinear(nn.Module):
         if norm is not None:
             if norm.features != self.in_features:
                 raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
-            gamma, eps = norm._parameters["weight"], norm.eps
+            gamma, eps = _parameter(norm, "weight"), norm.eps
         elif residual is not None:
             raise ValueError("APABlockLinear: residual needs norm")
         _real(x.dtype, "APABlockLinear")
