@@ -95,10 +95,10 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     d = x.dim()
     if d < 1:
         raise ValueError(f"{what}: expected at least one dimension")
-    m = x if d == 2 else x.reshape(-1, x.shape[-1])
-    n = m.shape[1]
+    n = x.shape[-1]
     if n == 0:
         raise ValueError(f"{what}: has no columns")
+    m = x if d == 2 else x.reshape(-1, n)
     if not m.is_contiguous() and ((n > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < n)):
         m = m.contiguous()
     return m
@@ -116,6 +116,8 @@ def _same_device(what: str, device: torch.device, *tensors) -> None:
 
 
 def _vector(t: torch.Tensor, n: int, device: torch.device, what: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what}: expected shape [{n}], got {list(t.shape)}")
     _real(t.dtype, what)
@@ -351,7 +353,6 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     if not isinstance(weight, APABlockTensor):
         raise TypeError("block_linear: the weight must be an APABlockTensor (block_cast(w, square=True))")
     x2 = _matrix(x, "block_linear")
-    _no_gradient("block_linear", x, bias)
     code = _real(x2.dtype, "block_linear")
     _lib.require_cuda(x2, "block_linear")
     M, K = x2.shape
@@ -362,6 +363,7 @@ def block_linear(x: Union[torch.Tensor, APABlockTensor], weight: APABlockTensor,
     _same_device("block_linear", dev, weight.buffer)
     if bias is not None:
         bias = _vector(bias, N, dev, "block_linear: bias")
+    _no_gradient("block_linear", x, bias)
     out_code = code if out_dtype is None else _real(out_dtype, "block_linear: out_dtype")
     y = torch.empty(M, N, dtype=out_dtype or x2.dtype, device=dev)
     if M:
@@ -412,6 +414,8 @@ def _norm_args(x, weight, residual, what: str):
     g = _vector(weight, K, x2.device, f"{what}: weight")
     r2 = None
     if residual is not None:
+        if not isinstance(residual, torch.Tensor):
+            raise TypeError(f"{what}: residual: expected a tensor, got {type(residual).__name__}")
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"{what}: residual {residual.dtype} {list(residual.shape)} does not match x {x.dtype} "
                              f"{list(x.shape)}")
@@ -530,11 +534,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     eps = _check_eps(eps, "rms_norm")
     if not quantize:
         return _RMSNormFn.apply(x, weight, residual, eps)
+    x2, g, res2 = _norm_args(x, weight, residual, "rms_norm")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm: the E4M3 output has no gradient; call it under torch.no_grad(), or train through "
                            "APABlockLinear(...)(x, norm=norm, residual=residual)")
-    x2, g, res2 = _norm_args(x, weight, residual, "rms_norm")
     q, stream, _ = _norm_forward(x2, g, res2, eps, True, False)
     return q if residual is None else (q, stream.view(x.shape))
 
@@ -833,6 +837,8 @@ class APABlockLinear(nn.Module):
             if norm.features != self.in_features:
                 raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
             gamma, eps = _parameter(norm, "weight"), norm.eps
+            if residual is not None and not isinstance(residual, torch.Tensor):
+                raise TypeError(f"APABlockLinear: residual: expected a tensor, got {type(residual).__name__}")
         elif residual is not None:
             raise ValueError("APABlockLinear: residual needs norm")
         _real(x.dtype, "APABlockLinear")

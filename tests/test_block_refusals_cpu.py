@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from apa import APABlockTensor, _lib, block_linear, block_matmul, blockscale
+from apa import (APABlockLinear, APABlockTensor, APAConfig, APARMSNorm, _lib, block_cast, block_linear, block_matmul,
+                 blockscale, rms_norm)
 
 
 def block(rows, cols):
@@ -56,3 +57,23 @@ def test_buffers_too_small_for_their_shape():
     for bad in (t.buffer.view(1, -1), t.buffer.float(), t.buffer.numpy()):
         with pytest.raises(TypeError):
             APABlockTensor(bad, 5, 200)
+
+
+def test_arguments_that_are_no_tensors(monkeypatch):
+    monkeypatch.setattr(_lib, "require_cuda", lambda t, what: None)
+    cpu = APAConfig(device="cpu")
+    x, g, w = torch.randn(3, 64), torch.ones(64), block(8, 64)
+    lin, norm = APABlockLinear(64, 8, config=cpu), APARMSNorm(64, config=cpu)
+    for call in (lambda: block_linear(x, w, [0.0] * 8), lambda: block_matmul(block(3, 64), w, 1.0),
+                 lambda: rms_norm(x, [1.0] * 64, quantize=True), lambda: rms_norm(x, 1.0),
+                 lambda: rms_norm(x, g, 2.0), lambda: rms_norm(x, g, 2.0, quantize=True),
+                 lambda: rms_norm([1.0], g, quantize=True), lambda: lin(x, norm=norm, residual=1.0)):
+        with pytest.raises(TypeError, match="expected a tensor"):
+            call()
+
+
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (2, 3, 0), (0, 4, 0)])
+def test_no_columns(shape):
+    for call in (lambda x: block_cast(x), lambda x: rms_norm(x, torch.ones(0))):
+        with pytest.raises(ValueError, match="has no columns"):
+            call(torch.empty(shape))
