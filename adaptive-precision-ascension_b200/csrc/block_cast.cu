@@ -13,8 +13,10 @@
 // residual stream), and the column sums of the source come along (the bias
 // gradient), per 128 rows.
 //
-// Bound by HBM for fp32 sources, by the conversion's instructions (ALU pipe) for
-// 16-bit ones: every element is read once and written once per form. One
+// Every element is read once and written once per form. fp32 sources run at
+// HBM's rate. 16-bit ones reach no unit's limit (ALU pipe 57 %, issue slots
+// 61 %): two CTAs fill the register file, 46 % of the warps, and each passes up
+// to three barriers a tile, so what a tile waits for is not hidden. One
 // 128 x 128 tile per CTA of 512 threads; a thread holds a 4 x 8 piece in
 // registers, so both forms and all maxima come from one read, and 64 registers
 // a thread leave room for two CTAs per SM. (8 x 8 pieces on 256 threads ran at
@@ -22,9 +24,8 @@
 // cp.async gained nothing in bf16 and lost a third in fp32.)
 //
 // Measured on a B200, inputs in HBM, 8192 x 4096 (us, TB/s of what is read and
-// written): bf16 rows form 20.5, 4.9; cols 23.9, 4.2; both 30.3, 4.4, with ALU
-// pipe and issue slots 57 and 61 % busy; fp32 rows 26.3, 6.4; both 34.2, 5.9.
-// Dequantisation to bf16 19.4, 5.2.
+// written): bf16 rows form 20.5, 4.9; cols 23.9, 4.2; both 30.3, 4.4; fp32 rows
+// 26.3, 6.4; both 34.2, 5.9. Dequantisation to bf16 19.4, 5.2.
 #include "block_scale.cuh"
 
 namespace apa {
@@ -50,7 +51,8 @@ struct CastShared {
 };
 
 // One 128 x 128 tile. NORM: the source is src * row_mul * col_mul. (Maxima of
-// 16-bit sources on packed pairs, half the instructions, were no faster.)
+// 16-bit sources on packed pairs, half the instructions, were no faster at two
+// CTAs per SM.)
 template <int SRC, bool SQUARE, bool NORM>
 __device__ __forceinline__ void cast_tile(const CastArgs& p, int64_t tile, CastShared& sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
