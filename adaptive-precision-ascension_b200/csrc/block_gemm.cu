@@ -744,7 +744,8 @@ __global__ void __launch_bounds__(64 + 32 * EW, 1)
       // done while the first tile is under way; sixteen loads at a time
       if (p.sums.part != nullptr) {
         const ColumnSums& t = p.sums;
-        for (int c = ((int)blockIdx.x * EW + e) * 32 + lane; c < t.cols; c += (int)gridDim.x * EW * 32) {
+        // 64 bits: the last step passes 2^31 where cols is near it
+        for (int64_t c = ((int)blockIdx.x * EW + e) * 32 + lane; c < t.cols; c += (int)gridDim.x * EW * 32) {
           float x = 0.0f;
           for (int r = 0; r < t.parts; r += 16) {
             float v[16];
