@@ -703,9 +703,9 @@ class APABlockLinear(nn.Module):
     cast weight and renews it when the parameter was replaced, when autograd's
     version counter shows a change in place, after a training forward and after
     any ``torch.optim`` optimizer's step. Call ``refresh_working_copy()`` after
-    changes behind all of these: through ``.data`` or by a replayed graph. A
-    weight made under ``torch.inference_mode()`` has no version counter and is
-    cast on every call.
+    changes behind all of these: through ``.data``, by a collective or by a
+    replayed graph. A weight made under ``torch.inference_mode()`` has no version
+    counter and is cast on every call.
 
     ``forward(x, norm=None, residual=None)``: with ``norm`` (an ``APARMSNorm``)
     the layer is applied to ``norm(x)``, or to the normalised sum x + residual;
