@@ -294,8 +294,9 @@ def _matmul(a: APABlockTensor, b: APABlockTensor, bias, out: torch.Tensor, accum
           out.data_ptr(), dt, _ld(out), M, N, K, int(accumulate), plan, _lib.ptr(ws), n)
 
 
-def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradient(what: str, a, b) -> None:
+    """Refuses what wants a gradient (each may be None)."""
+    if ((a is not None and a.requires_grad) or (b is not None and b.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError(f"{what}: has no gradient; call it under torch.no_grad(), or train through APABlockLinear")
 
 
@@ -396,12 +397,14 @@ def _linear_forward(x2, code, res2, gamma, eps, stream, rstd, w2, xt, wq, wt, bi
 # ---------------------------------------------------------------------------
 # root-mean-square norm
 # ---------------------------------------------------------------------------
-def _parameter(module: nn.Module, name: str):
-    """A module's parameter. nn.Module's own lookup takes a microsecond; it serves
-    a parameter that something else computes (a parametrization, pruning, a
+def _norm_weight(norm: nn.Module):
+    """A norm module's weight. nn.Module's own lookup takes a microsecond; it
+    serves a weight that something else computes (a parametrization, pruning, a
     replica of DataParallel)."""
-    p = module._parameters
-    return p[name] if name in p else getattr(module, name)
+    try:
+        return norm._parameters["weight"]
+    except KeyError:
+        return norm.weight
 
 
 def _norm_args(x, weight, residual, what: str):
@@ -557,7 +560,7 @@ class APARMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(features, dtype=dtype, device=torch.device(config.device)))
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, quantize: bool = False):
-        return rms_norm(x, _parameter(self, "weight"), residual, self.eps, quantize)
+        return rms_norm(x, _norm_weight(self), residual, self.eps, quantize)
 
     def extra_repr(self) -> str:
         return f"{self.features}, eps={self.eps}"
@@ -827,7 +830,11 @@ class APABlockLinear(nn.Module):
         return (None if W.is_inference() else W._version, W.data_ptr(), W.dtype, _optimizer_steps)
 
     def forward(self, x: torch.Tensor, norm: Optional[APARMSNorm] = None, residual: Optional[torch.Tensor] = None):
-        W, b = _parameter(self, "weight_master"), _parameter(self, "bias_master")
+        p = self._parameters           # as in _norm_weight
+        try:
+            W, b = p["weight_master"], p["bias_master"]
+        except KeyError:
+            W, b = self.weight_master, self.bias_master
         if not isinstance(x, torch.Tensor):
             raise TypeError(f"APABlockLinear: expected a tensor, got {type(x).__name__}")
         if x.dim() < 1 or x.shape[-1] != self.in_features:
@@ -836,7 +843,7 @@ class APABlockLinear(nn.Module):
         if norm is not None:
             if norm.features != self.in_features:
                 raise ValueError(f"APABlockLinear: norm over {norm.features} features, expected {self.in_features}")
-            gamma, eps = _parameter(norm, "weight"), norm.eps
+            gamma, eps = _norm_weight(norm), norm.eps
             if residual is not None and not isinstance(residual, torch.Tensor):
                 raise TypeError(f"APABlockLinear: residual: expected a tensor, got {type(residual).__name__}")
         elif residual is not None:
