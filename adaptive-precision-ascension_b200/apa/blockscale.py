@@ -152,8 +152,8 @@ class APABlockTensor:
         if rows < 0 or cols <= 0:
             raise ValueError(f"APABlockTensor: bad shape [{rows}, {cols}]")
         if buffer.numel() < _packed_bytes(rows, cols) or not buffer.is_contiguous() or buffer.data_ptr() % 16:
-            raise ValueError(f"APABlockTensor: [{rows}, {cols}] takes {_packed_bytes(rows, cols)} contiguous bytes on a "
-                             "16-byte boundary")
+            raise ValueError(f"APABlockTensor: [{rows}, {cols}] takes {_packed_bytes(rows, cols)} contiguous bytes "
+                             "on a 16-byte boundary")
         self.buffer, self.rows, self.cols = buffer, rows, cols
 
     @property
@@ -789,7 +789,8 @@ class APABlockLinear(nn.Module):
         current stream's work. A capture that would have to renew it records a
         cast of its own, which nothing outside the graph sees."""
         if W.is_inference():
-            # it has no version counter, and inference mode may change it in place: nothing shows whether a cast still holds
+            # it has no version counter, and inference mode may change it in
+            # place: nothing shows whether a cast still holds
             with torch.cuda.device(W.device):
                 return self._cast_weight(W)
         handle = _lib.stream_handle(W.device)
